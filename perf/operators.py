@@ -396,7 +396,7 @@ def _evict(s, c):
     lens_out = lens.clamp(max=budget)
     i = torch.arange(n, device=dev)
     kept = torch.where(i < lens_out, best, cap).sort(-1).values
-    ok = i < lens_out
+    ok = (i < lens_out).expand(B, Hkv, n)
     at = kept.clamp(max=cap - 1)
     out_cap = s["out_table"].shape[1] * page
     src = s["page_table"].long().unsqueeze(1).expand(B, Hkv, -1).gather(2, at // page), at % page
