@@ -28,6 +28,23 @@ ALGO_AUTO, ALGO_GEMV, ALGO_TCGEN05, ALGO_MX, ALGO_FUSED, ALGO_TCGEN05_PAIR = 0, 
 _c = ctypes
 _vp, _i64, _i32, _f32, _sz = _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_size_t
 
+
+
+class Heads(_c.Structure):
+    """bs_heads of include/bs_moe.h: a [B, T, heads, D] tensor, strides in elements."""
+    _fields_ = [("ptr", _vp), ("stride_b", _i64), ("stride_t", _i64), ("stride_h", _i64)]
+
+
+class KVCache(_c.Structure):
+    """bs_kv_cache of include/bs_moe.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("pages", _i64), ("page_size", _i64), ("heads", _i64), ("dim", _i64),
+                ("k_stride_page", _i64), ("k_stride_slot", _i64), ("k_stride_head", _i64),
+                ("v_stride_page", _i64), ("v_stride_slot", _i64), ("v_stride_head", _i64),
+                ("page_table", _vp), ("table_width", _i64), ("table_stride", _i64), ("lens", _vp), ("batch", _i64)]
+
+
+_heads, _cache = _c.POINTER(Heads), _c.POINTER(KVCache)
+
 # name -> (restype, argtypes); mirrors include/bs_moe.h
 SIGNATURES = {
     "bs_version": (_i32, []),
@@ -72,6 +89,16 @@ SIGNATURES = {
     "bs_mxfp4_matmul_backward": (_i32, [_vp, _i64, _i64, _vp, _vp, _i64, _vp, _vp, _sz, _vp]),
     "bs_moe_forward": (_i32, [_vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _i32, _vp, _vp,
                               _vp, _vp, _vp, _vp, _vp, _vp, _i32, _f32, _f32, _vp, _vp, _sz, _i32, _vp]),
+    "bs_rope": (_i32, [_heads, _heads, _heads, _heads, _i32, _i64, _i64, _i64, _i64, _i64, _vp, _i64, _i64, _vp,
+                       _i32, _i32, _i32, _vp]),
+    "bs_rope_append": (_i32, [_heads, _heads, _heads, _heads, _cache, _i64, _i64, _vp, _i64, _i64, _vp, _i32, _i32,
+                              _vp]),
+    "bs_tree_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "bs_tree_attention": (_i32, [_heads, _cache, _i64, _i64, _vp, _vp, _i64, _vp, _i64, _f32, _vp, _vp, _vp, _sz,
+                                 _vp]),
+    "bs_tree_commit": (_i32, [_cache, _i64, _vp, _i64, _vp]),
+    "bs_kv_scores_add": (_i32, [_heads, _cache, _i64, _i64, _vp, _vp, _i64, _f32, _vp, _vp, _i64, _vp]),
+    "bs_kv_evict": (_i32, [_cache, _vp, _i64, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp]),
 }
 
 _lock = threading.Lock()

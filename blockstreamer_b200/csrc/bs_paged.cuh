@@ -1,0 +1,103 @@
+// The paged key/value cache as the attention kernels see it, and the warp-level
+// tensor-core pieces they share.
+#pragma once
+
+#include "bs_common.cuh"
+#include "bs_ptx.cuh"
+
+namespace bs {
+
+// Division by a page size: shift when it is a power of two, else a 32-bit
+// divide (slots are below 2^31).
+struct PageDiv {
+  int size, shift;  // shift < 0: not a power of two
+  __device__ __forceinline__ void split(int slot, int& page, int& row) const {
+    page = shift >= 0 ? slot >> shift : slot / size;
+    row = slot - page * size;
+  }
+};
+
+struct PagedCache {
+  __nv_bfloat16* k;
+  __nv_bfloat16* v;
+  int64_t kp, ks, kh, vp, vs, vh;  // strides in elements: page, slot, head
+  const int32_t* table;
+  int64_t table_stride;
+  const int32_t* lens;
+  int pages, heads, dim, capacity;  // capacity: slots of a sequence's table row
+  PageDiv div;
+  int* status;
+
+  // Committed length of sequence b, clamped so that `extra` slots follow it.
+  __device__ __forceinline__ int len(int b, int extra) const {
+    const int n = lens[b];
+    const int top = capacity - extra;
+    if (n < 0 || n > top) {
+      record_status(status, BS_ERR_CAPACITY);
+      return n < 0 ? 0 : top;
+    }
+    return n;
+  }
+  // Page of a slot below capacity, clamped into the pool.
+  __device__ __forceinline__ int page_of(int b, int index) const {
+    const int p = __ldg(table + b * table_stride + index);
+    if ((unsigned)p >= (unsigned)pages) {
+      record_status(status, BS_ERR_CAPACITY);
+      return p < 0 ? 0 : pages - 1;
+    }
+    return p;
+  }
+};
+
+// Checks a bs_kv_cache and fills the kernels' form of it (attention.cu).
+int paged_cache(const char* fn, const bs_kv_cache* c, int64_t extra, bool need_v, PagedCache* out);
+
+namespace mma {
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t r[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm_x4_trans(uint32_t addr, uint32_t r[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// d[16 x 8] += a[16 x 16] b[16 x 8], bf16 in, f32 accumulate.
+__device__ __forceinline__ void bf16_16816(float d[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16-byte asynchronous copy; zero bytes are read and zeros written when !on.
+__device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
+               : "memory");
+}
+
+// Byte offset of 16-byte chunk `c` of row `r` in a tile of DP bf16 per row,
+// chunks permuted within the row so that eight consecutive rows' chunks of one
+// column fall into eight different 16-byte bank groups.
+template <int DP>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  constexpr int kChunks = DP / 8;
+  if constexpr (kChunks == 4)
+    return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
+  else if constexpr (kChunks == 12)  // 192-byte rows: pairs of rows share a phase
+    return (uint32_t)(r * 192 + ((c ^ ((r >> 1) & 3)) << 4));
+  else
+    return (uint32_t)(r * (DP * 2) + ((c ^ (r & 7)) << 4));
+}
+
+}  // namespace mma
+}  // namespace bs

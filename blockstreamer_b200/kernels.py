@@ -422,3 +422,220 @@ def mxfp4_matmul_backward(grad_out: torch.Tensor, blocks: torch.Tensor, scales: 
         _lib.call("bs_mxfp4_matmul_backward", _p(go), m, N, _p(_contig("blocks", blocks)),
                   _p(_contig("scales", scales)), K, _p(out), _p(ws), ws.numel(), _stream(go))
     return out
+
+
+# ---------------------------------------------------------------- attention half of the decoder layer
+def _heads(name: str, t: torch.Tensor | None):
+    """bs_heads of a [B, T, heads, D] or [T, heads, D] tensor (views are fine, D contiguous)."""
+    if t is None:
+        return _lib.Heads(None, 0, 0, 0)
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    return _lib.Heads(t.data_ptr(), st[0] if len(st) == 4 else 0, st[-3], st[-2])
+
+
+def _kv_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor | None, page_table: torch.Tensor,
+              cache_lens: torch.Tensor):
+    if k_cache.dim() != 4 or (v_cache is not None and v_cache.shape != k_cache.shape):
+        raise ValueError(f"{name}: the caches must be [pages, page_size, heads, D] of one shape")
+    v = k_cache if v_cache is None else v_cache
+    if k_cache.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+        raise ValueError(f"{name}: the caches must be bf16")
+    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
+                                                                    and page_table.stride(1) != 1):
+        raise ValueError(f"{name}: page_table must be int32 [B, pages of a sequence] with contiguous rows")
+    B = page_table.shape[0]
+    if cache_lens.shape != (B,) or cache_lens.dtype != torch.int32 or not cache_lens.is_contiguous():
+        raise ValueError(f"{name}: cache_lens must be contiguous int32 [{B}]")
+    P, S, H, D = k_cache.shape
+    ks, vs = k_cache.stride(), v.stride()
+    if D > 1 and (ks[3] != 1 or vs[3] != 1):
+        raise ValueError(f"{name}: the caches' last dimension must be contiguous")
+    return _lib.KVCache(k_cache.data_ptr(), v.data_ptr(), P, S, H, D, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+                        page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(), B)
+
+
+def _positions(name: str, positions: torch.Tensor, shape, dtypes=(torch.int32, torch.int64)) -> torch.Tensor:
+    if tuple(positions.shape) != tuple(shape) or positions.dtype not in dtypes:
+        raise ValueError(f"{name}: positions must be {' or '.join(str(d) for d in dtypes)} {tuple(shape)}, got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    return _contig(f"{name}: positions", positions)
+
+
+def _rope_table(name: str, table: torch.Tensor, D: int) -> int:
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or not table.is_contiguous():
+        raise ValueError(f"{name}: table must be contiguous f32 [max_pos, rot/2, 2]")
+    if 2 * table.shape[1] > D:
+        raise ValueError(f"{name}: the table turns {2 * table.shape[1]} values of a head of {D}")
+    return 2 * table.shape[1]
+
+
+def rope(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor,
+         interleaved: bool = False, inverse: bool = False):
+    """Rotary positions of q [B, T, Hq, D] (or [T, Hq, D]) and k, one launch (bs_rope).
+
+    ``table`` [max_pos, rot/2, 2] f32 holds (cos, sin) per position and pair
+    (``attention.rotary_table``); pairs are (i, i + rot/2), or neighbours when
+    ``interleaved``; values beyond rot are copied.  ``positions`` has q's shape
+    without its last two dimensions; a negative one gives zeros.  ``inverse``
+    turns back, which is the gradient.  Returns (q', k') contiguous (k' None
+    without k)."""
+    _cuda("rope", q, k, table, positions)
+    if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
+                                                    or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype)):
+        raise ValueError("rope: q and k must be [B, T, heads, D] or [T, heads, D], alike but for the heads")
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("rope: q and k must be bf16 or f32")
+    D = q.shape[-1]
+    rot = _rope_table("rope", table, D)
+    positions = _positions("rope", positions, q.shape[:-2])
+    B, T = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    with torch.cuda.device(q.device):
+        _lib.call("bs_rope", _heads("rope", q), _heads("rope", k), _heads("rope", qo), _heads("rope", ko),
+                  _DT[q.dtype], B, T, q.shape[-2], 0 if k is None else k.shape[-2], D, _p(table), table.shape[0],
+                  rot, _p(positions), _DT[positions.dtype], int(interleaved), int(inverse), _stream(q))
+    return qo, ko
+
+
+def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, positions: torch.Tensor,
+                k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+                interleaved: bool = False) -> torch.Tensor:
+    """The serving form of ``rope`` (bs_rope_append): returns the turned q
+    [B, T, Hq, D] and writes the turned k and v [B, T, Hkv, D] into the cache at
+    slots cache_lens[b] + t.  Rows of negative position write nothing."""
+    _cuda("rope_append", q, k, v, table, positions, k_cache, v_cache, page_table, cache_lens)
+    cache = _kv_cache("rope_append", k_cache, v_cache, page_table, cache_lens)
+    if q.dim() != 4 or q.dtype != torch.bfloat16 or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError("rope_append: q, k and v must be bf16 [B, T, heads, D]")
+    B, T, Hq, D = q.shape
+    if B != cache.batch or D != cache.dim or tuple(k.shape) != (B, T, cache.heads, D) or v.shape != k.shape:
+        raise ValueError(f"rope_append: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not match a "
+                         f"cache of {cache.batch} sequences, {cache.heads} heads of {cache.dim}")
+    rot = _rope_table("rope_append", table, D)
+    positions = _positions("rope_append", positions, (B, T))
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    with torch.cuda.device(q.device):
+        _lib.call("bs_rope_append", _heads("rope_append", q), _heads("rope_append", k), _heads("rope_append", v),
+                  _heads("rope_append", qo), cache, T, Hq, _p(table), table.shape[0], rot, _p(positions),
+                  _DT[positions.dtype], int(interleaved), _stream(q))
+    return qo
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                   cache_lens: torch.Tensor, positions: torch.Tensor, tree_mask: torch.Tensor | None = None,
+                   sinks: torch.Tensor | None = None, window: int = 0, scale: float | None = None):
+    """Attention of drafted tokens over the paged cache (bs_tree_attention).
+
+    q [B, T, Hq, D] bf16, whose keys and values are already in the cache at
+    slots cache_lens[b] + t; ``positions`` [B, T] int32 (negative: unused draft
+    slot); ``tree_mask`` bool/uint8 [T, T] or [B, T, T]: which drafts a token
+    attends, itself included (None: a chain); ``sinks`` [Hq] f32; ``window`` 0
+    for none; ``scale`` defaults to D**-0.5.  Returns (out [B, T, Hq, D] bf16,
+    lse [B, T, Hq] f32)."""
+    _cuda("tree_attention", q, k_cache, v_cache, page_table, cache_lens, positions, tree_mask, sinks)
+    cache = _kv_cache("tree_attention", k_cache, v_cache, page_table, cache_lens)
+    if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != cache.batch or q.shape[3] != cache.dim:
+        raise ValueError(f"tree_attention: q must be bf16 [{cache.batch}, T, Hq, {cache.dim}], got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    positions = _positions("tree_attention", positions, (B, T), (torch.int32,))
+    mask_stride = 0
+    if tree_mask is not None:
+        if tree_mask.dtype not in (torch.bool, torch.uint8) or tuple(tree_mask.shape) not in ((T, T), (B, T, T)):
+            raise ValueError(f"tree_attention: tree_mask must be bool or uint8 [{T}, {T}] or [{B}, {T}, {T}]")
+        if tree_mask.dim() == 3:
+            mask_stride = tree_mask.stride(0)
+        if not (tree_mask if tree_mask.dim() == 2 else tree_mask[0] if B else tree_mask).is_contiguous():
+            raise ValueError("tree_attention: every sequence's tree_mask must be contiguous")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (Hq,) or not sinks.is_contiguous()):
+        raise ValueError(f"tree_attention: sinks must be contiguous f32 [{Hq}]")
+    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, T, Hq), dtype=torch.float32, device=q.device)
+    ws_bytes = _lib.load().bs_tree_attention_workspace_bytes(B, T, Hq, cache.heads, D)
+    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
+    with torch.cuda.device(q.device):
+        _lib.call("bs_tree_attention", _heads("tree_attention", q), cache, T, Hq, _p(positions), _p(tree_mask),
+                  mask_stride, _p(sinks), window, D ** -0.5 if scale is None else scale, _p(out), _p(lse), _p(ws),
+                  ws_bytes, _stream(q))
+    return out, lse
+
+
+def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+                accepted: torch.Tensor, drafted: int) -> None:
+    """Moves the accepted drafts' keys and values from slots cache_lens[b] +
+    accepted[b, i] to cache_lens[b] + i (bs_tree_commit).  ``accepted`` [B, A]
+    int32 holds ascending draft indices, then negative ones; ``drafted`` is the
+    step's T.  cache_lens is left for the caller to advance."""
+    _cuda("tree_commit", k_cache, v_cache, page_table, cache_lens, accepted)
+    cache = _kv_cache("tree_commit", k_cache, v_cache, page_table, cache_lens)
+    if accepted.dim() != 2 or accepted.dtype != torch.int32 or accepted.shape[0] != cache.batch:
+        raise ValueError(f"tree_commit: accepted must be int32 [{cache.batch}, A]")
+    accepted = _contig("tree_commit: accepted", accepted)
+    with torch.cuda.device(k_cache.device):
+        _lib.call("bs_tree_commit", cache, drafted, _p(accepted), accepted.shape[1], _stream(k_cache))
+
+
+def kv_scores_add(scores: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor,
+                  page_table: torch.Tensor, cache_lens: torch.Tensor, accepted: torch.Tensor | None = None,
+                  scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """scores [B, Hkv, capacity] f32 plus the attention weight that each cached
+    key received from a step's accepted tokens (bs_kv_scores_add): token i of
+    the accepted ones (all of q's T when ``accepted`` is None) sits at slot
+    cache_lens[b] + i and attended every slot up to its own.  q and ``lse`` are
+    those of ``tree_attention``; entries of ``accepted`` [B, A] int32 outside
+    [0, T) are skipped.  ``out`` may be ``scores``."""
+    _cuda("kv_scores_add", scores, q, lse, k_cache, page_table, cache_lens, accepted, out)
+    cache = _kv_cache("kv_scores_add", k_cache, None, page_table, cache_lens)
+    if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != cache.batch or q.shape[3] != cache.dim:
+        raise ValueError(f"kv_scores_add: q must be bf16 [{cache.batch}, T, Hq, {cache.dim}], got {q.dtype} "
+                         f"{tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    if scores.dtype != torch.float32 or scores.dim() != 3 or tuple(scores.shape[:2]) != (B, cache.heads):
+        raise ValueError(f"kv_scores_add: scores must be f32 [{B}, {cache.heads}, capacity]")
+    if lse.dtype != torch.float32 or tuple(lse.shape) != (B, T, Hq):
+        raise ValueError(f"kv_scores_add: lse must be f32 [{B}, {T}, {Hq}]")
+    if accepted is not None and (accepted.dim() != 2 or accepted.dtype != torch.int32 or accepted.shape[0] != B):
+        raise ValueError(f"kv_scores_add: accepted must be int32 [{B}, A]")
+    scores, lse = _contig("kv_scores_add: scores", scores), _contig("kv_scores_add: lse", lse)
+    if accepted is not None:
+        accepted = _contig("kv_scores_add: accepted", accepted)
+    if out is None:
+        out = torch.empty_like(scores)
+    elif out.shape != scores.shape or out.dtype != scores.dtype or not out.is_contiguous():
+        raise ValueError("kv_scores_add: out must be contiguous and of the shape of scores")
+    with torch.cuda.device(q.device):
+        _lib.call("bs_kv_scores_add", _heads("kv_scores_add", q), cache, T, Hq, _p(lse), _p(accepted),
+                  T if accepted is None else accepted.shape[1], D ** -0.5 if scale is None else scale, _p(scores),
+                  _p(out), scores.shape[2], _stream(q))
+    return out
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+             scores: torch.Tensor, budget: int, out_page_table: torch.Tensor, keep_first: int = 0,
+             keep_last: int = 0):
+    """Cuts every (sequence, kv head) to ``budget`` slots (bs_kv_evict): the
+    first ``keep_first``, the last ``keep_last`` and the others of the highest
+    scores (ties: lowest slot), copied in order into the pages of
+    ``out_page_table`` [B, width].  Returns (kept [B, Hkv, budget] int32 slots
+    then -1, new lengths [B] int32, scores of the new slots [B, Hkv, width *
+    page_size] f32)."""
+    _cuda("kv_evict", k_cache, v_cache, page_table, cache_lens, scores, out_page_table)
+    cache = _kv_cache("kv_evict", k_cache, v_cache, page_table, cache_lens)
+    B, Hkv = cache.batch, cache.heads
+    if scores.dtype != torch.float32 or scores.dim() != 3 or tuple(scores.shape[:2]) != (B, Hkv):
+        raise ValueError(f"kv_evict: scores must be f32 [{B}, {Hkv}, capacity]")
+    if out_page_table.dtype != torch.int32 or out_page_table.dim() != 2 or out_page_table.shape[0] != B:
+        raise ValueError(f"kv_evict: out_page_table must be int32 [{B}, width]")
+    scores = _contig("kv_evict: scores", scores)
+    out_page_table = _contig("kv_evict: out_page_table", out_page_table)
+    dev, width = k_cache.device, out_page_table.shape[1]
+    kept = torch.empty((B, Hkv, max(budget, 0)), dtype=torch.int32, device=dev)
+    lens = torch.empty((B,), dtype=torch.int32, device=dev)
+    new = torch.empty((B, Hkv, width * cache.page_size), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        _lib.call("bs_kv_evict", cache, _p(scores), scores.shape[2], budget, keep_first, keep_last,
+                  _p(out_page_table), width, _p(kept), _p(lens), _p(new), _stream(k_cache))
+    return kept, lens, new

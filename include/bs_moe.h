@@ -344,6 +344,128 @@ int bs_moe_block_forward(const void* x, int64_t T, int64_t H, int64_t I, int64_t
                          int bias_dtype, float alpha, float limit, void* out, void* workspace,
                          size_t workspace_bytes, int algo, void* stream);
 
+/* ------------------------------------------------------------------------
+ * The attention half of a gpt-oss decoder layer at decode sizes: rotary
+ * positions, attention of drafted tokens over a paged key/value cache, and the
+ * eviction of cached keys by the attention weight they received.  The reference
+ * leaves these steps to transformers (models/gpt_oss/modeling_gpt_oss.py,
+ * GptOssRotaryEmbedding, _apply_rotary_emb, GptOssAttention.forward with
+ * eager_attention_forward's sinks, and its cache classes).
+ *
+ * A [B, T, heads, D] tensor is given by a bs_heads: strides in elements, the
+ * last dimension contiguous (views of a fused projection are taken as they
+ * are).  A bs_kv_cache describes bf16 pages k, v [pages, page_size, heads, dim]
+ * (any strides with dim contiguous, so [pages, heads, page_size, dim] pools
+ * too) and the sequences in them: slot j of sequence b is row j % page_size of
+ * page page_table[b * table_stride + j / page_size]; lens[b] slots hold
+ * committed keys and a step's T drafted tokens sit at slots lens[b] + t.  Both
+ * structs are read during the call only.  Strides and pointers of the cache are
+ * multiples of 16 bytes; dim is a multiple of 8 up to 128.
+ *
+ * lens, positions and page tables are device data that the host does not read:
+ * the kernels clamp what they index with.  A length outside [0, table_width *
+ * page_size - T] or a page outside [0, pages) records BS_ERR_CAPACITY in the
+ * status word (bs_device_status); a write there is dropped, a read takes the
+ * nearest valid length or page.  A position below zero marks a row not in use. */
+typedef struct bs_heads {
+  void* ptr;
+  int64_t stride_b, stride_t, stride_h;
+} bs_heads;
+
+typedef struct bs_kv_cache {
+  void* k;
+  void* v;
+  int64_t pages, page_size, heads, dim;
+  int64_t k_stride_page, k_stride_slot, k_stride_head;
+  int64_t v_stride_page, v_stride_slot, v_stride_head;
+  const int32_t* page_table;
+  int64_t table_width, table_stride;
+  const int32_t* lens;
+  int64_t batch;
+} bs_kv_cache;
+
+/* Rotary positions: the first rot of the D values of every head of q (and of
+ * k, unless its ptr is NULL) turned pairwise, values beyond rot copied.  With
+ * (c, s) = table[position][i] and the pair (x[i], x[i + rot/2]), or
+ * (x[2i], x[2i+1]) when interleaved:
+ *   out = (a c - b s, b c + a s);   inverse != 0: the same with -s, which is
+ * the gradient of the forward turn.  Any scaling of long contexts, and any
+ * factor on cos and sin, is in the table [max_pos, rot/2, 2] f32.
+ * dtype bf16 or f32 (of q, k and the outputs); positions [B, T] int32 or int64
+ * contiguous; a row whose position is negative, or not below max_pos (that one
+ * records BS_ERR_INVALID_ARGUMENT), becomes zeros.  fp32 arithmetic, one
+ * rounding.  Outputs must not overlap inputs of other rows; in place is fine.
+ * Replaces modeling_gpt_oss.py _apply_rotary_emb / apply_rotary_pos_emb. */
+int bs_rope(const bs_heads* q, const bs_heads* k, const bs_heads* q_out, const bs_heads* k_out,
+            int dtype, int64_t B, int64_t T, int64_t Hq, int64_t Hk, int64_t D, const float* table,
+            int64_t max_pos, int64_t rot, const void* positions, int pos_dtype, int interleaved,
+            int inverse, void* stream);
+
+/* The serving form: q turned into q_out, k turned into the cache and v copied
+ * there, at slots lens[b] + t; rows of negative position write nothing to the
+ * cache and zeros to q_out.  bf16; k and v have cache->heads heads. */
+int bs_rope_append(const bs_heads* q, const bs_heads* k, const bs_heads* v, const bs_heads* q_out,
+                   const bs_kv_cache* cache, int64_t T, int64_t Hq, const float* table,
+                   int64_t max_pos, int64_t rot, const void* positions, int pos_dtype,
+                   int interleaved, void* stream);
+
+/* Attention of T drafted tokens per sequence (a tree; T = 1 is plain decoding)
+ * over the cache.  Row (t, h) attends slot j of its sequence, with n = lens[b]:
+ *   j < n, or j = n + u with mask[b][t][u] != 0 and positions[b][u] >= 0,
+ *   and, when window > 0, keypos(j) > max(positions[b][t], n) - window, where
+ *   keypos(j) = j below n and positions[b][u] at n + u.
+ * x_j = scale q . k_j;  z = sum exp(x_j) + exp(sinks[h]) (sinks may be NULL);
+ * out = sum exp(x_j) v_j / z;  lse = log z.  A row that attends nothing gives
+ * out 0 and lse sinks[h] (-inf without sinks); a row of negative position gives
+ * out 0 and lse -inf.  Slots that no row may attend are not read.
+ * q, out bf16 [B, T, Hq, dim] (out contiguous), Hq a multiple of cache->heads;
+ * mask uint8 [T, T] per sequence with mask_stride_b between sequences (0: one
+ * tree for all), NULL for a chain (u <= t); sinks [Hq] f32; positions [B, T]
+ * int32; lse [B, T, Hq] f32 (may be NULL); 1 <= T <= 256.  fp32 softmax
+ * statistics and sums; the weights are rounded to bf16 for the product with v.
+ * Workspace: bs_tree_attention_workspace_bytes(B, T, Hq, heads, dim) bytes. */
+size_t bs_tree_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D);
+int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, int64_t T, int64_t Hq,
+                      const int32_t* positions, const void* mask, int64_t mask_stride_b,
+                      const float* sinks, int64_t window, float scale, void* out, float* lse,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* After verification: moves the keys and values of the accepted drafts to
+ * consecutive slots, slot lens[b] + accepted[b][i] -> lens[b] + i.  accepted
+ * [B, A] int32: ascending draft indices, then negative ones; a list that is not
+ * ascending records BS_ERR_INVALID_ARGUMENT and its sequence is left as it is.
+ * lens is not changed.  A <= 256. */
+int bs_tree_commit(const bs_kv_cache* cache, int64_t T, const int32_t* accepted, int64_t A,
+                   void* stream);
+
+/* Adds to each cached key's score the attention weight it received from the
+ * accepted tokens of a step (after bs_tree_commit, with lens still the lengths
+ * before the step):
+ *   scores_out[b][h][j] = scores[b][h][j] + sum over i and the heads g of group
+ *   h of exp(scale q[b, u_i, g] . k_j - lse[b][u_i][g])   for j <= lens[b] + i,
+ * u_i = accepted[b][i] (NULL: u_i = i, A = T), entries outside [0, T) skipped,
+ * and rows whose lse is -inf too.  scores, scores_out [B, heads, capacity] f32
+ * contiguous (may be the same array); lse [B, T, Hq] f32 contiguous. */
+int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int64_t T, int64_t Hq,
+                     const float* lse, const int32_t* accepted, int64_t A, float scale,
+                     const float* scores, float* scores_out, int64_t capacity, void* stream);
+
+/* Eviction: of the n = lens[b] slots of every (sequence, kv head) keeps the
+ * first keep_first, the last keep_last and, up to budget in all, those of the
+ * highest score (ties: lowest slot; NaN ranks below every number), and copies
+ * their keys and values in ascending order to slots 0.. of out_page_table
+ * [B, out_width] (pages of the same pool that hold no slot being read, except
+ * that a sequence with n <= budget may keep its own pages).
+ * scores [B, heads, capacity] f32 contiguous.  Outputs: kept [B, heads, budget]
+ * int32 (the kept slots, then -1), out_lens [B] int32 = min(n, budget),
+ * out_scores [B, heads, out_width * page_size] f32 (the kept scores, then 0).
+ * keep_first + keep_last <= budget <= out_width * page_size, or the budget may
+ * exceed that where n cannot. */
+int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_t capacity, int64_t budget,
+                int64_t keep_first, int64_t keep_last, const int32_t* out_page_table,
+                int64_t out_width, int32_t* kept, int32_t* out_lens, float* out_scores,
+                void* stream);
+
 #ifdef __cplusplus
 }
 #endif
