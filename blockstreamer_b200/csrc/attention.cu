@@ -53,6 +53,24 @@ int paged_cache(const char* fn, const bs_kv_cache* c, int64_t extra, bool need_v
   return BS_OK;
 }
 
+int cache_box_rows(const bs_kv_cache* c, int most) {
+  int r = 1;
+  while (r < most && c->page_size % (2 * r) == 0) r *= 2;
+  return r;
+}
+
+int cache_maps(const bs_kv_cache* c, int rows, bool need_v, CacheMaps* o) {
+  const uint64_t dims[4] = {(uint64_t)c->dim, (uint64_t)c->heads, (uint64_t)c->page_size, (uint64_t)c->pages};
+  const uint32_t box[4] = {64, 1, (uint32_t)rows, 1};
+  // a dimension of one element may have any stride in the caller's tensor
+  auto bytes = [](int64_t stride, int64_t n) { return n > 1 ? (uint64_t)stride * 2 : (uint64_t)16; };
+  const uint64_t ks[3] = {bytes(c->k_stride_head, c->heads), bytes(c->k_stride_slot, c->page_size), bytes(c->k_stride_page, c->pages)};
+  BS_TRY(make_map_4d(&o->k, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c->k, dims, ks, box, CU_TENSOR_MAP_SWIZZLE_128B));
+  if (!need_v) return BS_OK;
+  const uint64_t vs[3] = {bytes(c->v_stride_head, c->heads), bytes(c->v_stride_slot, c->page_size), bytes(c->v_stride_page, c->pages)};
+  return make_map_4d(&o->v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c->v, dims, vs, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
 namespace {
 
 constexpr int kMaxDrafts = 256;
@@ -69,6 +87,7 @@ struct TreeArgs {
   const float* sinks;
   float scale2;  // scale * log2(e)
   int window, T, G, R, tiles, Hkv, B;
+  int box;          // slots of a TMA box, or 1
   __nv_bfloat16* out;
   float* lse;
   float* part_o;    // [2 * grid][tile rows][dim]
@@ -76,16 +95,22 @@ struct TreeArgs {
   int min_chunk;
 };
 
-// The key range of a sequence: [lo, n + T), n committed.
+// The keys of a sequence: n committed; slots [low, hi) may be attended; units
+// start at lo, low rounded down to where a TMA box may start.
 struct Keys {
-  int n, lo, hi;
+  int n, low, lo, hi;
 };
 __device__ __forceinline__ Keys keys_of(const TreeArgs& a, int b) {
   Keys k;
   k.n = a.c.len(b, a.T);
   k.hi = k.n + a.T;
-  k.lo = a.window ? max(0, k.n - a.window + 1) : 0;
+  k.low = a.window ? max(0, k.n - a.window + 1) : 0;
+  k.lo = k.low & -a.box;
   return k;
+}
+// Whether a slot holds a key that some row may attend (others may hold anything).
+__device__ __forceinline__ bool holds_key(const TreeArgs& a, int b, const Keys& k, int slot) {
+  return slot >= k.low && (slot < k.n || (slot < k.hi && __ldg(a.pos + (int64_t)b * a.T + slot - k.n) >= 0));
 }
 
 // Where the work of CTA `cta` of `grid` lies, units of kU keys: its range
@@ -100,6 +125,7 @@ __device__ __forceinline__ int64_t units_of(const TreeArgs& a, int b) {
   const Keys k = keys_of(a, b);
   return (k.hi - k.lo + kU - 1) / kU;
 }
+__device__ __forceinline__ void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 template <int kU>
 __device__ Range locate(const TreeArgs& a, int cta, int grid, int64_t* sums /* smem [6] */) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -109,7 +135,7 @@ __device__ Range locate(const TreeArgs& a, int cta, int grid, int64_t* sums /* s
 #pragma unroll
   for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) sums[warp] = total;
-  __syncthreads();
+  sync128();
   total = sums[0] + sums[1] + sums[2] + sums[3];
   Range r;
   r.chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
@@ -129,15 +155,15 @@ __device__ Range locate(const TreeArgs& a, int cta, int grid, int64_t* sums /* s
       const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += v;
     }
-    __syncthreads();
+    sync128();
     if (lane == 31) sums[warp] = incl;
-    __syncthreads();
+    sync128();
     int64_t start = run + incl - w;
     for (int i = 0; i < warp; ++i) start += sums[i];
     run += sums[0] + sums[1] + sums[2] + sums[3];
     if (w > 0 && start <= r.p0 && r.p0 < start + w) sums[4] = b, sums[5] = start;
   }
-  __syncthreads();
+  sync128();
   r.b = (int)sums[4];
   r.before = sums[5];
   return r;
@@ -145,26 +171,29 @@ __device__ Range locate(const TreeArgs& a, int cta, int grid, int64_t* sums /* s
 
 // ---------------------------------------------------------------- few rows
 // Row tiles of MT * 16 rows on mma.sync, four warps per CTA, each streaming its
-// own units of kU keys (16-byte asynchronous copies, kStages units per warp, no
-// barrier between warps) and holding its own (m, z, O); they meet at the end of
-// an item.  HBM-bound: 148 SMs x 2 CTAs x 4 warps keep ~190 KB per SM in flight.
+// own units of kU keys into its own ring (no barrier between warps) and holding
+// its own (m, z, O); they meet at the end of an item.  HBM-bound: two CTAs per SM
+// keep ~190 KB per SM in flight.
+// kTma: a unit is fetched by a few TMA boxes (pages of a multiple of 8 slots);
+// else by 16-byte asynchronous copies, whose address arithmetic and issue then
+// are most of the kernel's instructions.
 template <int DP>
 struct RowsCfg {
-  static constexpr int kU = DP <= 64 ? 32 : 16;
-  static constexpr int kStages = DP == 96 || DP == 32 ? 4 : 3;
+  static constexpr int kU = DP == 64 ? 32 : 16;
+  static constexpr int kStages = 3;
   static constexpr int kTile = kU * DP * 2;           // bytes of a K (or V) unit
   static constexpr int kWarpBytes = 2 * kTile * kStages;
 };
 template <int DP, int MT>
 struct RowsSmem {
   static constexpr int kRows = 16 * MT;
-  static constexpr int stages = 0;
   static constexpr int merge = 4 * RowsCfg<DP>::kWarpBytes;
   static constexpr int ml = merge + kRows * DP * 4;            // [4 warps][rows] float2
   static constexpr int bits = ml + 4 * kRows * 8;              // [rows][8] words
   static constexpr int thr = bits + kRows * (kMaxDrafts / 32) * 4;
   static constexpr int sums = (thr + kRows * 4 + 15) / 16 * 16;
-  static constexpr int total = sums + 64;
+  static constexpr int bars = sums + 64;                       // [4 warps][kStages]
+  static constexpr int total = bars + 4 * RowsCfg<DP>::kStages * 8 + 1024;
 };
 
 // The units of a CTA's range as one warp meets them (it takes every fourth
@@ -212,84 +241,113 @@ __device__ __forceinline__ bool walk_next(const TreeArgs& a, int64_t p1, Walk& w
   return true;
 }
 
-template <int DP, int MT>
-__global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant__ TreeArgs a) {
+template <int DP, int MT, bool kTma>
+__global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant__ TreeArgs a,
+                                                           const __grid_constant__ CacheMaps maps) {
   using Cfg = RowsCfg<DP>;
   using Sm = RowsSmem<DP, MT>;
   constexpr int kU = Cfg::kU, KS = DP / 16, NT = kU / 8, kRows = 16 * MT, kWords = kMaxDrafts / 32;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* merge = reinterpret_cast<float*>(smem + Sm::merge);
   float2* ml = reinterpret_cast<float2*>(smem + Sm::ml);
   uint32_t* bits = reinterpret_cast<uint32_t*>(smem + Sm::bits);
   int* thr = reinterpret_cast<int*>(smem + Sm::thr);
   const uint32_t base = ptx::smem_addr(smem) + warp * Cfg::kWarpBytes;
+  const uint32_t bar = ptx::smem_addr(smem) + Sm::bars + warp * Cfg::kStages * 8;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // columns dim..DP are zeros that no copy touches
-  if (a.c.dim < DP) {
+  if constexpr (kTma) {
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+      for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_init(bar + 8 * s, 1);
+      ptx::fence_mbar_init();
+    }
+  } else if (a.c.dim < DP) {
+    // columns dim..DP are zeros that no copy touches
     for (int i = threadIdx.x; i < 4 * Cfg::kWarpBytes / 16; i += 128)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
   }
+  __syncthreads();
   const Range r = locate<kU>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + Sm::sums));
   if (r.p0 >= r.p1) return;
 
-  // ---- loading: lane l < kU holds where row l of the next unit lies
+  // ---- loading.  Lane g holds the page and row of the next unit's g-th box (or,
+  // without TMA, slot); pages are looked up one unit ahead.
+  const int box = kTma ? min(a.box, kU) : 1, boxes = kU / box;
   Walk lw;
   walk_begin<kU>(a, r, lw);
   lw.u = lw.start + warp;
   bool more = true;
-  int next_page = 0, next_row = -1;  // row < 0: zeros
+  int next_page = 0, next_row = -1;  // row < 0: no key there
   auto find = [&]() {
     while (more && lw.u >= lw.end) {
       more = walk_next<kU>(a, r.p1, lw);
       lw.u = lw.start + warp;
     }
     next_row = -1;
-    if (!more || lane >= kU) return;
-    const int slot = lw.k.lo + lw.u * kU + lane;
-    bool on = slot < lw.k.hi;
-    if (on && slot >= lw.k.n) on = a.pos[(int64_t)lw.b * a.T + slot - lw.k.n] >= 0;
-    if (on) {
+    if (!more || lane >= boxes) return;
+    const int slot = lw.k.lo + lw.u * kU + lane * box;
+    if (kTma ? slot < lw.k.hi : holds_key(a, lw.b, lw.k, slot)) {
       int p;
       a.c.div.split(slot, p, next_row);
-      next_page = a.c.page_of(lw.b, p);
+      next_page = __ldg(a.c.table + lw.b * a.c.table_stride + p);
     }
   };
-  constexpr int kLanesRow = DP <= 64 ? 8 : 16;  // lanes that copy one row
   auto load = [&](int stage) {
     if (more) {
       const uint32_t kd = base + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
-      const int c = lane % kLanesRow;
-      const __nv_bfloat16* kb = a.c.k + lw.h * a.c.kh + c * 8;
-      const __nv_bfloat16* vb = a.c.v + lw.h * a.c.vh + c * 8;
-      const bool col = c * 8 < a.c.dim;
+      if (next_row >= 0 && (unsigned)next_page >= (unsigned)a.c.pages) {
+        record_status(a.c.status, BS_ERR_CAPACITY);
+        next_page = next_page < 0 ? 0 : a.c.pages - 1;
+      }
+      if constexpr (kTma) {
+        if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * stage, 2 * Cfg::kTile);
+        __syncwarp();
+        if (lane < boxes) {
+          // a box behind the last slot lies outside the descriptor's pages: zeros
+          const int page = next_row >= 0 ? next_page : a.c.pages, row = max(next_row, 0);
 #pragma unroll
-      for (int i = 0; i < kU * kLanesRow / 32; ++i) {
-        const int row = lane / kLanesRow + i * (32 / kLanesRow);
-        const int p = __shfl_sync(0xffffffffu, next_page, row);
-        const int x = __shfl_sync(0xffffffffu, next_row, row);
-        if (col) {
-          const uint32_t at = mma::tile_at<DP>(row, c);
-          const bool on = x >= 0;
-          mma::cp_async_16_or_zero(kd + at, on ? kb + p * a.c.kp + x * a.c.ks : kb, on);
-          mma::cp_async_16_or_zero(vd + at, on ? vb + p * a.c.vp + x * a.c.vs : vb, on);
+          for (int x = 0; x < DP / 64; ++x) {
+            const uint32_t at = x * (kU * 128) + lane * box * 128;
+            ptx::tma_load_4d(kd + at, &maps.k, bar + 8 * stage, x * 64, lw.h, row, page);
+            ptx::tma_load_4d(vd + at, &maps.v, bar + 8 * stage, x * 64, lw.h, row, page);
+          }
+        }
+      } else {
+        constexpr int kLanesRow = DP / 8;  // lanes that copy one row
+        const int c = lane % kLanesRow;
+        const __nv_bfloat16* kb = a.c.k + lw.h * a.c.kh + c * 8;
+        const __nv_bfloat16* vb = a.c.v + lw.h * a.c.vh + c * 8;
+        const bool col = c * 8 < a.c.dim;
+#pragma unroll
+        for (int i = 0; i < kU * kLanesRow / 32; ++i) {
+          const int row = lane / kLanesRow + i * (32 / kLanesRow);
+          const int p = __shfl_sync(0xffffffffu, next_page, row);
+          const int x = __shfl_sync(0xffffffffu, next_row, row);
+          if (col) {
+            const uint32_t at = mma::tile_at<kU>(row, c);
+            const bool on = x >= 0;
+            mma::cp_async_16_or_zero(kd + at, on ? kb + p * a.c.kp + x * a.c.ks : kb, on);
+            mma::cp_async_16_or_zero(vd + at, on ? vb + p * a.c.vp + x * a.c.vs : vb, on);
+          }
         }
       }
       lw.u += 4;
       find();
     }
-    ptx::cp_async_commit();
+    if constexpr (!kTma) ptx::cp_async_commit();
   };
   find();
 #pragma unroll
   for (int s = 0; s < Cfg::kStages - 1; ++s) load(s);
+  int stage = 0, phase = 0;
 
   // ---- pieces
   Walk cw;
   walk_begin<kU>(a, r, cw);
-  int stage = 0;
   while (true) {
     const int row0 = cw.tile * kRows, rows = min(kRows, a.R - row0);
     const int t0 = row0 / a.G, toks = (row0 + rows - 1) / a.G - t0 + 1;
@@ -349,11 +407,26 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
       for (int d = 0; d < DP / 8; ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.f;
     }
     for (int u = cw.start + warp; u < cw.end; u += 4) {
-      ptx::cp_async_wait<Cfg::kStages - 2>();
-      __syncwarp();
       const uint32_t kt = base + stage * 2 * Cfg::kTile, vt = kt + Cfg::kTile;
+      const int slot0 = cw.k.lo + u * kU;
+      if constexpr (kTma) {
+        ptx::mbar_wait(bar + 8 * stage, phase, &abort_flag);  // a wait that ran out is reported at the end
+        if (slot0 < cw.k.low || slot0 + kU > cw.k.n) {
+          // a box brings all its slots: those that hold no key become zeros in V
+          if (lane < kU && !holds_key(a, cw.b, cw.k, slot0 + lane)) {
+            uint8_t* v = smem + (vt - ptx::smem_addr(smem)) + lane * 128;
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i)
+              *reinterpret_cast<uint4*>(v + (i >> 3) * (kU * 128) + (i & 7) * 16) = make_uint4(0, 0, 0, 0);
+          }
+          ptx::fence_proxy_async_smem();
+        }
+      } else {
+        ptx::cp_async_wait<Cfg::kStages - 2>();
+      }
+      __syncwarp();
       load((stage + Cfg::kStages - 1) % Cfg::kStages);
-      stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
+      if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
 
       float s[MT][NT][4];
 #pragma unroll
@@ -365,14 +438,13 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 #pragma unroll
         for (int np = 0; np < NT / 2; ++np) {
           uint32_t f[4];
-          mma::ldsm_x4(kt + mma::tile_at<DP>(np * 16 + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)), f);
+          mma::ldsm_x4(kt + mma::tile_at<kU>(np * 16 + (lane >> 4) * 8 + (lane & 7), 2 * k + ((lane >> 3) & 1)), f);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
             mma::bf16_16816(s[mt][2 * np], qf[mt][k], f[0], f[1]);
             mma::bf16_16816(s[mt][2 * np + 1], qf[mt][k], f[2], f[3]);
           }
         }
-      const int slot0 = cw.k.lo + u * kU;
       const bool edge = slot0 + kU > cw.k.n || a.window;
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -408,10 +480,12 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
             p[nt][e] = pack_bf16x2(y0, y1);
           }
           z[mt][e] = z[mt][e] * f + sum;
+          if (__any_sync(0xffffffffu, f != 1.f)) {
 #pragma unroll
-          for (int d = 0; d < DP / 8; ++d) {
-            o[mt][d][2 * e] *= f;
-            o[mt][d][2 * e + 1] *= f;
+            for (int d = 0; d < DP / 8; ++d) {
+              o[mt][d][2 * e] *= f;
+              o[mt][d][2 * e + 1] *= f;
+            }
           }
         }
 #pragma unroll
@@ -420,7 +494,7 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 #pragma unroll
           for (int dp = 0; dp < DP / 16; ++dp) {
             uint32_t f[4];
-            mma::ldsm_x4_trans(vt + mma::tile_at<DP>(j * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * dp + (lane >> 4)), f);
+            mma::ldsm_x4_trans(vt + mma::tile_at<kU>(j * 16 + ((lane >> 3) & 1) * 8 + (lane & 7), 2 * dp + (lane >> 4)), f);
             mma::bf16_16816(o[mt][2 * dp], pf, f[0], f[1]);
             mma::bf16_16816(o[mt][2 * dp + 1], pf, f[2], f[3]);
           }
@@ -509,10 +583,473 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
     if (!walk_next<kU>(a, r.p1, cw)) break;
     __syncthreads();
   }
-  ptx::cp_async_wait_all();
+  if constexpr (kTma) {
+    if (*(volatile int*)&abort_flag) {
+      if (threadIdx.x == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
+      // copies in flight end before the CTA's memory is given back
+      volatile int gone = 0;
+      for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_wait(bar + 8 * s, phase ^ 1, &gone);
+    }
+  } else {
+    ptx::cp_async_wait_all();
+  }
 }
 
-// Joins the pieces of the items that several CTAs share, in CTA order.
+// ---------------------------------------------------------------- many rows
+// Row tiles of 128 on tcgen05: S = Q K^T (128 x 128 per tile of keys, both
+// operands in shared memory) into tensor memory, the weights P = 2^(x - m) back
+// into tensor memory as bf16, O += P V with P as the tensor-memory operand and V
+// as it lies in the cache (keys along K, the head contiguous).
+//
+// Two pipelines per CTA, each a group of four softmax warps (a thread per row)
+// and an MMA warp, so that one pipeline's products run while the other's
+// exponentials do.  With more than 128 rows to a kv head (kPair) they take two
+// row tiles and share every K and V tile; with fewer they take alternate tiles
+// of keys for the same rows and meet at the end of an item, where both read both
+// accumulators (same lanes of tensor memory).  One more warp fetches K and V by
+// TMA boxes of a page's slots into a ring of tiles.
+//
+// The running maximum is only moved when a row's scores exceed it by 2^8: P stays
+// far below the bf16 range, sums are fp32, and the accumulator is rarely rescaled.
+template <int DP>
+struct TilesCfg {
+  static constexpr int kSlot = 128 * DP * 2;             // a K or V tile, [DP / 64] panels of 128 rows x 128 bytes
+  static constexpr int kSlots = DP == 64 ? 10 : 4;
+  static constexpr int q = kSlots * kSlot;               // two Q tiles
+  static constexpr int bits = q + 2 * kSlot;             // [256 threads][8 words]
+  static constexpr int ml = bits + 256 * 32;             // [2][128] float2
+  static constexpr int bars = ml + 2 * 128 * 8;
+  static constexpr int total = bars + 256 + 1024;        // barriers; alignment of the base
+};
+constexpr int kTileThreads = 352;
+constexpr uint32_t kSCol = 128, kOCol = 256;             // pipeline p: S at p * kSCol, O at kOCol + p * 128
+constexpr float kRescale = 8.f;
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort));
+}
+// A K x N operand whose N extent is contiguous (64 values = 128 bytes per row
+// of K, 128B-swizzled): 8-row groups 1024 bytes apart, 64-value panels `panel`.
+__device__ __forceinline__ uint64_t sdesc_nmajor_sw128(uint32_t saddr, uint32_t panel) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+// Bits of a 256-bit row starting at bit `at` (which may lie outside).
+__device__ __forceinline__ uint32_t bits_from(const uint32_t* row, int at) {
+  const int w = at >> 5, s = at & 31;
+  const uint32_t lo = (unsigned)w < 8u ? row[w] : 0u;
+  const uint32_t hi = (unsigned)(w + 1) < 8u ? row[w + 1] : 0u;
+  return __funnelshift_r(lo, hi, s);
+}
+// Bits [a, b) of a word, a and b clamped to 0..32.
+__device__ __forceinline__ uint32_t bit_range(int a, int b) {
+  a = min(max(a, 0), 32);
+  b = min(max(b, 0), 32);
+  const uint32_t below_b = b == 32 ? 0xffffffffu : (1u << b) - 1u;
+  const uint32_t below_a = a == 32 ? 0xffffffffu : (1u << a) - 1u;
+  return below_b & ~below_a;
+}
+
+template <int DP, bool kPair>
+__global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __grid_constant__ TreeArgs a,
+                                                                     const __grid_constant__ CacheMaps maps) {
+  using Cfg = TilesCfg<DP>;
+  constexpr int kU = 128, kRows = kPair ? 256 : 128;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ int64_t sums[6];
+  __shared__ uint32_t tmem_at;
+  __shared__ int abort_flag;
+  __shared__ Range range;
+  volatile int* abort = &abort_flag;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t sbase = ptx::smem_addr(smem);
+  const uint32_t bar = sbase + Cfg::bars;
+  auto full = [&](int s) { return bar + 8 * s; };
+  auto empty = [&](int s) { return bar + 8 * (Cfg::kSlots + s); };
+  constexpr int kB = 16 * Cfg::kSlots;
+  auto sfull = [&](int p) { return bar + kB + 8 * p; };
+  auto pready = [&](int p) { return bar + kB + 16 + 8 * p; };
+  auto qfull = [&](int p) { return bar + kB + 32 + 8 * p; };
+  auto odone = [&](int p) { return bar + kB + 48 + 8 * p; };
+  auto drain = [&](int p) { return bar + kB + 64 + 8 * p; };
+  const uint32_t meet = bar + kB + 80;
+  static_assert(kB + 88 <= 256, "barriers");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (tid < 128) {
+    const Range r = locate<kU>(a, blockIdx.x, gridDim.x, sums);
+    if (tid == 0) range = r;
+  } else if (warp == 10) {
+    ptx::tmem_alloc(ptx::smem_addr(&tmem_at), 512);
+    ptx::tmem_relinquish();
+  } else if (tid == 128) {
+    abort_flag = 0;
+    for (int i = 0; i < Cfg::kSlots; ++i) {
+      ptx::mbar_init(full(i), 1);
+      ptx::mbar_init(empty(i), kPair ? 2 : 1);
+    }
+    for (int p = 0; p < 2; ++p) {
+      ptx::mbar_init(sfull(p), 1);
+      ptx::mbar_init(pready(p), 128);
+      ptx::mbar_init(qfull(p), 128);
+      ptx::mbar_init(odone(p), 1);
+      ptx::mbar_init(drain(p), 1);
+    }
+    ptx::mbar_init(meet, 256);
+    ptx::fence_mbar_init();
+  }
+  __syncwarp();
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const Range r = range;
+  const uint32_t tmem = tmem_at;
+  bool ok = true;
+
+  if (r.p0 < r.p1) {
+    Walk w;
+    walk_begin<kU>(a, r, w);
+    int base = 0;  // tiles of the pieces before this one
+    if (warp == 8) {
+      // ------------------------------------------------ loader: lane g fetches the g-th box of a tile
+      const int boxes = kU / a.box;
+      int page = 0, row = -1, i = w.start, s = 0;
+      auto find = [&]() {
+        row = -1;
+        const int slot = w.k.lo + i * kU + lane * a.box;
+        if (lane < boxes && slot < w.k.hi) {
+          int p;
+          a.c.div.split(slot, p, row);
+          page = __ldg(a.c.table + w.b * a.c.table_stride + p);
+        }
+      };
+      bool more = true;
+      find();
+      while (more && ok) {
+        if (row >= 0 && (unsigned)page >= (unsigned)a.c.pages) {
+          record_status(a.c.status, BS_ERR_CAPACITY);
+          page = page < 0 ? 0 : a.c.pages - 1;
+        }
+        // a box behind the last slot lies outside the descriptor's pages: zeros
+        const int y = w.h, x = row >= 0 ? page : a.c.pages, z = max(row, 0);
+        if (++i == w.end) {
+          more = walk_next<kU>(a, r.p1, w);
+          i = w.start;
+        }
+        if (more) find();  // while the copies below are issued
+        for (int kv = 0; kv < 2 && ok; ++kv, ++s) {
+          const int at = s % Cfg::kSlots;
+          if (s >= Cfg::kSlots) ok = warp_wait(empty(at), (s / Cfg::kSlots - 1) & 1, abort);
+          if (!ok) break;
+          if (lane == 0) ptx::mbar_arrive_expect_tx(full(at), Cfg::kSlot);
+          __syncwarp();
+          if (lane < boxes) {
+#pragma unroll
+            for (int c = 0; c < DP / 64; ++c)
+              ptx::tma_load_4d(sbase + at * Cfg::kSlot + c * 16384 + lane * a.box * 128, kv ? &maps.v : &maps.k, full(at),
+                               c * 64, y, z, x);
+          }
+        }
+      }
+      if (!ok) {
+        // copies in flight end before the CTA's memory is given back
+        volatile int gone = 0;
+        for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
+      }
+    } else if (warp >= 9) {
+      // ------------------------------------------------ MMA issue, one thread per pipeline
+      const int p = warp - 9;
+      if (lane == 0) {
+        const uint32_t idesc_s = ptx::idesc_bf16_f32(128, 128);
+        const uint32_t idesc_o = ptx::idesc_bf16_f32(128, DP) | (1u << 16);  // B with N contiguous
+        const uint32_t s_col = tmem + p * kSCol, o_col = tmem + kOCol + p * 128;
+        const uint32_t qs = sbase + Cfg::q + p * Cfg::kSlot;
+        int done = 0, pieces = 0;  // tiles and pieces of this pipeline so far
+        bool more = true;
+        while (more && ok) {
+          const int n = w.end - w.start;
+          const int first = kPair ? 0 : p, step = kPair ? 1 : 2;
+          if (first < n) {
+            ok = ptx::mbar_wait(qfull(p), pieces & 1, abort);
+            ++pieces;
+            for (int i = first; i < n && ok; i += step) {
+              const int ks = 2 * (base + i), vs = ks + 1;
+              const int ka = ks % Cfg::kSlots, va = vs % Cfg::kSlots;
+              ok = ptx::mbar_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              const uint32_t kt = sbase + ka * Cfg::kSlot;
+#pragma unroll
+              for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+                ptx::mma_ss_bf16(s_col, ptx::sdesc_kmajor_sw128(qs + off), ptx::sdesc_kmajor_sw128(kt + off), idesc_s,
+                                 k > 0);
+              }
+              ptx::tc_commit(sfull(p));
+              ptx::tc_commit(empty(ka));
+              ok = ptx::mbar_wait(pready(p), done & 1, abort) &&
+                   ptx::mbar_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
+              if (!ok) break;
+              ptx::tc_fence_after();
+              const uint32_t vt = sbase + va * Cfg::kSlot;
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                ptx::mma_ts_bf16(o_col, s_col + k * 8, sdesc_nmajor_sw128(vt + k * 2048, 16384), idesc_o,
+                                 i > first || k > 0);
+              ptx::tc_commit(empty(va));
+              if (i + step >= n) ptx::tc_commit(odone(p));
+              ++done;
+            }
+          }
+          base += n;
+          more = walk_next<kU>(a, r.p1, w);
+        }
+        if (!ok) {
+          // products in flight end before tensor memory is given back
+          volatile int gone = 0;
+          ptx::tc_commit(drain(p));
+          ptx::mbar_wait(drain(p), 0, &gone);
+        }
+      }
+      __syncwarp();
+    } else {
+      // ------------------------------------------------ softmax, a thread per row
+      const int p = warp >> 2, t = tid & 127;
+      const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // lane offset in a tensor-memory address
+      const uint32_t s_col = tmem + lanes + p * kSCol;
+      uint32_t* bits = reinterpret_cast<uint32_t*>(smem + Cfg::bits) + tid * 8;
+      float2* ml = reinterpret_cast<float2*>(smem + Cfg::ml);
+      int done = 0, pieces[2] = {0, 0}, meets = 0;
+      bool more = true;
+      while (more && ok) {
+        const int n = w.end - w.start;
+        const int first = kPair ? 0 : p, step = kPair ? 1 : 2;
+        const int row0 = w.tile * kRows + (kPair ? p * 128 : 0);
+        const int rows = min(128, a.R - row0);  // may be negative: the second tile of a pair is empty
+        const bool mine = t < rows, warp_on = (warp & 3) * 32 < rows;
+        const int tok = mine ? (row0 + t) / a.G : 0, g = mine ? row0 + t - tok * a.G : 0;
+        const int hq = w.h * a.G + g;
+        int below = -1;  // keys up to here are outside the row's window (a row not in use is zeroed at the end)
+        float m = -INFINITY, z = 0.f;
+        if (first < n) {
+          // Q, and which keys this row may attend
+          uint8_t* qs = smem + Cfg::q + p * Cfg::kSlot;
+          const __nv_bfloat16* q = a.q + w.b * a.qb + tok * a.qt + (int64_t)hq * a.qh;
+#pragma unroll
+          for (int c = 0; c < DP / 8; ++c) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (mine && c * 8 < a.c.dim) v = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
+            *reinterpret_cast<uint4*>(qs + (c >> 3) * 16384 + mma::tile_at<128>(t, c & 7)) = v;
+          }
+          ptx::fence_proxy_async_smem();
+          ptx::mbar_arrive(qfull(p));
+          if (a.window) below = max(a.pos[(int64_t)w.b * a.T + tok], w.k.n) - a.window;
+          const int words = (a.T + 31) / 32;
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) bits[i] = 0;
+          if (warp_on) {
+            const int t0 = __shfl_sync(0xffffffffu, tok, 0);
+            const int t1 = __reduce_max_sync(0xffffffffu, tok);
+            for (int x = t0; x <= t1; ++x)
+              for (int i = 0; i < words; ++i) {
+                const int u = i * 32 + lane;
+                const int32_t* pos = a.pos + (int64_t)w.b * a.T;
+                const int px = pos[x];
+                bool on = false;
+                if (px >= 0 && u < a.T) {
+                  const int pu = pos[u];
+                  on = pu >= 0 && (!a.window || pu > max(px, w.k.n) - a.window) &&
+                       (a.mask ? a.mask[w.b * a.mask_b + (int64_t)x * a.T + u] != 0 : u <= x);
+                }
+                const uint32_t v = __ballot_sync(0xffffffffu, on);
+                if (mine && tok == x) bits[i] = v;
+              }
+          }
+          for (int i = first; i < n; i += step) {
+            ok = warp_wait(sfull(p), done & 1, abort);
+            if (!ok) break;
+            ++done;
+            ptx::tc_fence_after();
+            const int key0 = w.k.lo + (w.start + i) * kU;
+            if (warp_on) {
+              const bool slow = key0 + kU > w.k.n || a.window || a.scale2 < 0.f;
+              float v[128];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(s_col + c * 32, reinterpret_cast<uint32_t*>(v + c * 32));
+              ptx::tmem_wait_ld();
+              if (slow) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                  const int k0 = key0 + c * 32;
+                  const uint32_t see = bit_range(below + 1 - k0, w.k.n - k0) | bits_from(bits, k0 - w.k.n);
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) v[c * 32 + e] = see >> e & 1 ? v[c * 32 + e] * a.scale2 : -INFINITY;
+                }
+              }
+              float top[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) top[e] = v[e];
+#pragma unroll
+              for (int e = 4; e < 128; ++e) top[e & 3] = fmaxf(top[e & 3], v[e]);
+              float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+              const float mul = slow ? 1.f : a.scale2;
+              mx *= mul;
+              const bool move = mx > m + kRescale || (m == -INFINITY && mx > -INFINITY);
+              if (__any_sync(0xffffffffu, move)) {
+                const float f = move ? mma::exp2_fast(m - mx) : 1.f;  // 0 from -inf
+                if (move) {
+                  z *= f;
+                  m = mx;
+                }
+                if (i > first) {
+                  const uint32_t o_col = tmem + lanes + kOCol + p * 128;
+#pragma unroll 1
+                  for (int c = 0; c < DP / 16; ++c) {
+                    uint32_t o[16];
+                    ptx::tmem_ld_32x32b_x16(o_col + c * 16, o);
+                    ptx::tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    ptx::tmem_st_32x32b_x16(o_col + c * 16, o);
+                  }
+                }
+              }
+              const float ref = m == -INFINITY ? 0.f : m;
+              float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+              for (int c = 0; c < 4; ++c) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  float2 x = mma::fma2(make_float2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), mul, -ref);
+                  x.x = mma::exp2_fast(x.x);
+                  x.y = mma::exp2_fast(x.y);
+                  sum = mma::add2(sum, x);
+                  pk[e] = pack_bf16x2(x.x, x.y);
+                }
+                ptx::tmem_st_32x32b_x16(s_col + c * 16, pk);
+              }
+              z += sum.x + sum.y;
+            }
+            if (key0 < w.k.low || key0 + kU > w.k.n) {
+              // the tile's boxes bring all their slots: those that hold no key become zeros in V
+              const int vs = 2 * (base + i) + 1, va = vs % Cfg::kSlots;
+              ok = warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
+              if (!ok) break;
+              if (!holds_key(a, w.b, w.k, key0 + t)) {
+                uint8_t* row = smem + va * Cfg::kSlot + t * 128;
+#pragma unroll
+                for (int c = 0; c < DP / 8; ++c)
+                  *reinterpret_cast<uint4*>(row + (c >> 3) * 16384 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+              }
+              ptx::fence_proxy_async_smem();
+            }
+            if (warp_on) ptx::tmem_wait_st();
+            ptx::tc_fence_before();
+            ptx::mbar_arrive(pready(p));
+          }
+        }
+        if (!ok) break;
+        // ---- end of the piece: read the accumulators
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          if ((kPair && x != p) || (kPair ? 0 : x) >= n) continue;
+          ok = ok && warp_wait(odone(x), pieces[x] & 1, abort);
+          ++pieces[x];
+        }
+        if (!ok) break;
+        ptx::tc_fence_after();
+        float f0 = 1.f, f1 = 0.f;
+        if (!kPair) {
+          // both pipelines hold the same rows: common maximum, sums together
+          ml[p * 128 + t] = make_float2(m, z);
+          ptx::mbar_arrive(meet);
+          ok = warp_wait(meet, meets & 1, abort);
+          if (!ok) break;
+          ++meets;
+          const float2 m0 = ml[t], m1 = ml[128 + t];
+          m = fmaxf(m0.x, m1.x);
+          f0 = m0.x == -INFINITY ? 0.f : mma::exp2_fast(m0.x - m);
+          f1 = m1.x == -INFINITY ? 0.f : mma::exp2_fast(m1.x - m);
+          z = m0.y * f0 + m1.y * f1;
+        }
+        const bool whole = w.start == 0 && w.end == w.units;
+        const int64_t slot = 2 * (int64_t)blockIdx.x + (w.start == 0 ? 1 : 0);
+        const int dim = a.c.dim, row = (kPair ? p * 128 : 0) + t;
+        const int64_t at = ((int64_t)w.b * a.T + tok) * a.Hkv * a.G + hq;
+        float scale_o = 1.f;
+        if (whole && mine) {
+          const bool used = a.pos[(int64_t)w.b * a.T + tok] >= 0;
+          const float sink = a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+          const float top = fmaxf(m, sink);
+          const float ref = top == -INFINITY ? 0.f : top;
+          const float f = m == -INFINITY ? 0.f : mma::exp2_fast(m - ref);
+          const float den = z * f + (a.sinks ? mma::exp2_fast(sink - ref) : 0.f);
+          scale_o = used && m > -INFINITY ? f / den : 0.f;
+          if (a.lse && (kPair || p == 0)) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
+        }
+        if (!whole && mine && (kPair || p == 0)) a.part_ml[slot * kRows + row] = make_float2(m, z);
+        if (warp_on) {
+          // columns of this group: all of its own tile, or one half of the shared one
+          constexpr int kHalf = kPair ? DP : DP / 2;
+          const int c0 = kPair ? 0 : p * kHalf;
+#pragma unroll 1
+          for (int c = c0; c < c0 + kHalf; c += 16) {
+            uint32_t o0[16], o1[16];
+            ptx::tmem_ld_32x32b_x16(tmem + lanes + kOCol + (kPair ? p * 128 : 0) + c, o0);
+            if (!kPair) ptx::tmem_ld_32x32b_x16(tmem + lanes + kOCol + 128 + c, o1);
+            ptx::tmem_wait_ld();
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              x[e] = f0 == 0.f ? 0.f : __uint_as_float(o0[e]) * f0;
+              if (!kPair && f1 != 0.f) x[e] += __uint_as_float(o1[e]) * f1;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (!mine || c + j * 8 >= dim) continue;
+              if (whole) {
+                uint32_t pk[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  pk[e] = scale_o == 0.f ? 0u : pack_bf16x2(x[j * 8 + 2 * e] * scale_o, x[j * 8 + 2 * e + 1] * scale_o);
+                *reinterpret_cast<uint4*>(a.out + at * dim + c + j * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              } else {
+                float* po = a.part_o + (slot * kRows + row) * dim + c + j * 8;
+                *reinterpret_cast<float4*>(po) = make_float4(x[j * 8], x[j * 8 + 1], x[j * 8 + 2], x[j * 8 + 3]);
+                *reinterpret_cast<float4*>(po + 4) = make_float4(x[j * 8 + 4], x[j * 8 + 5], x[j * 8 + 6], x[j * 8 + 7]);
+              }
+            }
+            __syncwarp();
+          }
+        }
+        ptx::tc_fence_before();
+        if (!kPair) {
+          // the other pipeline's accumulator has been read before it is written again
+          ptx::mbar_arrive(meet);
+          ok = warp_wait(meet, meets & 1, abort);
+          if (!ok) break;
+          ++meets;
+        }
+        base += n;
+        more = walk_next<kU>(a, r.p1, w);
+      }
+    }
+  }
+  __syncwarp();
+  if (!ok && lane == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 10) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the pieces of the items that several CTAs share, in CTA order; a block
+// takes kJoinRows rows of an item.
+constexpr int kJoinRows = 8;
 template <int kU, int kRows>
 __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ TreeArgs a, int grid) {
   __shared__ int64_t sums[8];
@@ -544,7 +1081,8 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
   const int c0 = (int)(s / chunk), c1 = (int)((e - 1) / chunk);
   if (c0 == c1) return;
   const int dim = a.c.dim, row0 = tile * kRows, rows = min(kRows, a.R - row0);
-  for (int i = threadIdx.x; i < rows * (dim / 4); i += 128) {
+  const int first = blockIdx.y * kJoinRows, last = min(rows, first + kJoinRows);
+  for (int i = first * (dim / 4) + threadIdx.x; i < last * (dim / 4); i += 128) {
     const int row = i / (dim / 4), c = i - row * (dim / 4);
     float mx = -INFINITY;
     for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, a.part_ml[(2 * (int64_t)x + (x == c0)) * kRows + row].x);
@@ -576,22 +1114,19 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
   }
 }
 
-int tile_rows(int64_t R, int64_t D) { return R <= 16 || D > 64 ? 16 : 32; }
+// Rows of a tile: 16 and 32 run on the HBM-bound kernel of few rows, 128 and
+// 256 (a pair of tiles) on tcgen05, which needs TMA boxes.  The workspace is
+// sized without the page size, for the larger.
+int tile_rows(int64_t R, int64_t D, bool tma) {
+  const int few = R <= 16 || D > 64 ? 16 : 32;
+  if (R <= few || !tma) return few;
+  return R <= 128 ? 128 : 256;
+}
 
-template <int DP, int MT>
-int launch_rows(TreeArgs& a, int grid, cudaStream_t st) {
-  constexpr int smem = RowsSmem<DP, MT>::total;
-  static bool set[64] = {};
-  int dev = 0;
-  BS_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !set[dev]) {
-    BS_CUDA(cudaFuncSetAttribute(tree_rows_kernel<DP, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    if (dev < 64) set[dev] = true;
-  }
-  tree_rows_kernel<DP, MT><<<grid, 128, smem, st>>>(a);
-  BS_LAUNCHED();
+template <int kU, int kRows>
+int launch_join(const TreeArgs& a, int grid, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.tiles));
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.tiles), (unsigned)cdiv(std::min(kRows, a.R), kJoinRows));
   cfg.blockDim = dim3(128);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -599,11 +1134,41 @@ int launch_rows(TreeArgs& a, int grid, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  BS_CUDA(cudaLaunchKernelEx(&cfg, tree_join_kernel<RowsCfg<DP>::kU, 16 * MT>, a, grid));
+  BS_CUDA(cudaLaunchKernelEx(&cfg, tree_join_kernel<kU, kRows>, a, grid));
   return BS_OK;
 }
 
-int grid_for(int64_t) { return 2 * sm_count(); }
+template <int DP, int MT, bool kTma>
+int launch_rows(TreeArgs& a, const CacheMaps& maps, int grid, cudaStream_t st) {
+  constexpr int smem = RowsSmem<DP, MT>::total;
+  static bool set[64] = {};
+  int dev = 0;
+  BS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    BS_CUDA(cudaFuncSetAttribute(tree_rows_kernel<DP, MT, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) set[dev] = true;
+  }
+  tree_rows_kernel<DP, MT, kTma><<<grid, 128, smem, st>>>(a, maps);
+  BS_LAUNCHED();
+  return launch_join<RowsCfg<DP>::kU, 16 * MT>(a, grid, st);
+}
+
+int grid_for(int rows) { return rows <= 32 ? 2 * sm_count() : sm_count(); }
+
+template <int DP, bool kPair>
+int launch_tiles(TreeArgs& a, const CacheMaps& maps, int grid, cudaStream_t st) {
+  constexpr int smem = TilesCfg<DP>::total;
+  static bool set[64] = {};
+  int dev = 0;
+  BS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    BS_CUDA(cudaFuncSetAttribute(tree_tiles_kernel<DP, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) set[dev] = true;
+  }
+  tree_tiles_kernel<DP, kPair><<<grid, kTileThreads, smem, st>>>(a, maps);
+  BS_LAUNCHED();
+  return launch_join<128, kPair ? 256 : 128>(a, grid, st);
+}
 
 }  // namespace
 }  // namespace bs
@@ -611,8 +1176,12 @@ int grid_for(int64_t) { return 2 * sm_count(); }
 extern "C" size_t bs_tree_attention_workspace_bytes(int64_t B, int64_t T, int64_t Hq, int64_t Hkv, int64_t D) {
   using namespace bs;
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
-  const int64_t rows = tile_rows(T * (Hq / Hkv), D);
-  return align_up((size_t)(2 * (int64_t)grid_for(D) * rows * (D * 4 + 8)), 256);
+  int64_t most = 0;
+  for (bool tma : {false, true}) {
+    const int rows = tile_rows(T * (Hq / Hkv), D, tma);
+    most = std::max(most, 2 * (int64_t)grid_for(rows) * rows * (D * 4 + 8));
+  }
+  return align_up((size_t)most, 256);
 }
 
 extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, int64_t T, int64_t Hq,
@@ -652,19 +1221,29 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.G = (int)(Hq / cache->heads);
   a.R = a.T * a.G;
   a.B = (int)cache->batch;
-  const int rows = tile_rows(a.R, D);
+  a.box = cache_box_rows(cache, 128);
+  const bool tma = a.box >= 8;
+  const int rows = tile_rows(a.R, D, tma);
   a.tiles = (int)cdiv(a.R, (int64_t)rows);
   BS_ARG((int64_t)a.B * a.Hkv * a.tiles < INT32_MAX, "%s: sizes too large", fn);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
-  const int grid = grid_for(D);
+  const int grid = grid_for(rows);
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * D);
-  a.min_chunk = 4;
+  a.min_chunk = rows <= 32 ? 4 : 2;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  if (D <= 32) return rows == 16 ? launch_rows<32, 1>(a, grid, st) : launch_rows<32, 2>(a, grid, st);
-  if (D <= 64) return rows == 16 ? launch_rows<64, 1>(a, grid, st) : launch_rows<64, 2>(a, grid, st);
-  if (D <= 96) return launch_rows<96, 1>(a, grid, st);
-  return launch_rows<128, 1>(a, grid, st);
+  CacheMaps maps = {};
+  if (tma) {
+    if (rows <= 32) a.box = std::min(a.box, D <= 64 ? RowsCfg<64>::kU : RowsCfg<128>::kU);
+    BS_TRY(cache_maps(cache, a.box, true, &maps));
+  } else {
+    a.box = 1;
+  }
+  if (rows == 128) return D <= 64 ? launch_tiles<64, false>(a, maps, grid, st) : launch_tiles<128, false>(a, maps, grid, st);
+  if (rows == 256) return D <= 64 ? launch_tiles<64, true>(a, maps, grid, st) : launch_tiles<128, true>(a, maps, grid, st);
+  if (D > 64) return tma ? launch_rows<128, 1, true>(a, maps, grid, st) : launch_rows<128, 1, false>(a, maps, grid, st);
+  if (rows == 32) return tma ? launch_rows<64, 2, true>(a, maps, grid, st) : launch_rows<64, 2, false>(a, maps, grid, st);
+  return tma ? launch_rows<64, 1, true>(a, maps, grid, st) : launch_rows<64, 1, false>(a, maps, grid, st);
 }

@@ -52,6 +52,16 @@ struct PagedCache {
 // Checks a bs_kv_cache and fills the kernels' form of it (attention.cu).
 int paged_cache(const char* fn, const bs_kv_cache* c, int64_t extra, bool need_v, PagedCache* out);
 
+// TMA descriptors of K and V (attention.cu): boxes of `rows` slots of one page
+// and head by 64 values, 128B-swizzled.  `rows` is the largest power of two that
+// divides the page size, at most `most`; below 8 (one swizzle atom) there is no
+// such box and the kernels copy 16 bytes at a time.
+struct CacheMaps {
+  CUtensorMap k, v;
+};
+int cache_box_rows(const bs_kv_cache* c, int most);
+int cache_maps(const bs_kv_cache* c, int rows, bool need_v, CacheMaps* out);
+
 namespace mma {
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t r[4]) {
@@ -79,24 +89,36 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// a * b + c and a + b on two values at once.
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+      "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "add.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
 // 16-byte asynchronous copy; zero bytes are read and zeros written when !on.
 __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool on) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0)
                : "memory");
 }
 
-// Byte offset of 16-byte chunk `c` of row `r` in a tile of DP bf16 per row,
-// chunks permuted within the row so that eight consecutive rows' chunks of one
-// column fall into eight different 16-byte bank groups.
-template <int DP>
+// Byte offset of 16-byte chunk `c` of row `r` in a tile of kR rows: panels of 64
+// values (128 bytes a row), chunks permuted within the row by the row's low three
+// bits.  It is the layout of a 128B-swizzled TMA box and of the tensor-core
+// descriptors, and leaves ldmatrix without bank conflicts.
+template <int kR>
 __device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  constexpr int kChunks = DP / 8;
-  if constexpr (kChunks == 4)
-    return (uint32_t)(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-  else if constexpr (kChunks == 12)  // 192-byte rows: pairs of rows share a phase
-    return (uint32_t)(r * 192 + ((c ^ ((r >> 1) & 3)) << 4));
-  else
-    return (uint32_t)(r * (DP * 2) + ((c ^ (r & 7)) << 4));
+  return (uint32_t)((c >> 3) * (kR * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 }  // namespace mma

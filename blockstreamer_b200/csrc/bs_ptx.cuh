@@ -91,6 +91,15 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint32_t bar, int x,
+                                            int y, int z, int w) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+      : "memory");
+}
+
 // 1-D bulk copy global -> shared (16-byte aligned addresses, size a multiple of 16).
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile(
@@ -432,6 +441,10 @@ __device__ __forceinline__ void mma_ts_bf16_pair(uint32_t d_tmem, uint32_t a_tme
 // strides in bytes of dims 1 and 2.
 int make_map_3d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, const uint64_t dims[3],
                 const uint64_t strides[2], const uint32_t box[3], CUtensorMapSwizzle sw);
+
+// Host: the same in four dimensions, strides of dims 1, 2 and 3.
+int make_map_4d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, const uint64_t dims[4],
+                const uint64_t strides[3], const uint32_t box[4], CUtensorMapSwizzle sw);
 
 // Host: encode a 2-D tiled TMA descriptor (runtime.cu).  `inner` is the
 // contiguous extent in elements, `row_bytes` the pitch of the outer dimension.

@@ -49,8 +49,8 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
 // One CTA per kKeys slots of a (sequence, kv head).  K is the 16-row operand of
 // the tensor-core product, the accepted rows its columns, so that a key's sum
 // over the rows stays in one lane group; no atomics, one store per slot.
-// HBM-bound: 2 dim + 8 bytes per slot and kv head; all K of the CTA is in
-// flight at once.
+// HBM-bound: 2 dim + 8 bytes per slot and kv head.  All K of the CTA is asked for
+// at once (TMA boxes where pages allow, else 16-byte copies), then the queries.
 struct ScoreArgs {
   PagedCache c;
   const __nv_bfloat16* q;
@@ -60,59 +60,94 @@ struct ScoreArgs {
   const float* scores;
   float* out;
   float scale2;
-  int T, A, i0, rows, G, Hq, capacity;  // accepted entries i0 .. i0 + rows / G
+  int T, A, i0, rows, G, Hq, capacity, box;  // accepted entries i0 .. i0 + rows / G
 };
 
 template <int DP>
 struct ScoreCfg {
-  static constexpr int kUnits = DP <= 64 ? 4 : 2;   // units of 32 keys per warp
+  static constexpr int kUnits = DP == 64 ? 4 : 2;   // units of 32 keys per warp
   static constexpr int kKeys = 4 * 32 * kUnits;
   static constexpr int kTile = 32 * DP * 2;
-  static constexpr int k = 0;
-  static constexpr int q = 4 * kUnits * kTile;      // then [rows] q, [rows] float2
-  static int smem(int rows) { return q + rows * (DP * 2 + 8); }
+  static constexpr int q = 4 * kUnits * kTile;      // then [rows] q, [rows] float2, barriers
+  static int smem(int rows) { return q + rows * (DP * 2 + 8) + 4 * kUnits * 8 + 1024; }
 };
 
-template <int DP>
-__global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ ScoreArgs a) {
+template <int DP, bool kTma>
+__global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ ScoreArgs a,
+                                                        const __grid_constant__ CacheMaps maps) {
   using Cfg = ScoreCfg<DP>;
-  constexpr int KS = DP / 16, kLanesRow = DP <= 64 ? 8 : 16;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  constexpr int KS = DP / 16, kLanesRow = DP / 8, kUnits = Cfg::kUnits;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int b = blockIdx.y / a.c.heads, h = blockIdx.y - b * a.c.heads;
   const int n = a.c.len(b, a.A);
   const int rows8 = (a.rows + 7) / 8 * 8;
-  const uint32_t kbase = ptx::smem_addr(smem) + warp * Cfg::kUnits * Cfg::kTile;
+  const uint32_t kbase = ptx::smem_addr(smem) + warp * kUnits * Cfg::kTile;
   uint8_t* qs = smem + Cfg::q;
   float2* info = reinterpret_cast<float2*>(qs + rows8 * DP * 2);  // (lse log2(e), last slot seen)
-  const int first = blockIdx.x * Cfg::kKeys + warp * 32 * Cfg::kUnits;
+  const uint32_t bar = ptx::smem_addr(info + rows8) + warp * kUnits * 8;
+  const int first = blockIdx.x * Cfg::kKeys + warp * 32 * kUnits;
   const int top = min(a.capacity, n + a.A);
+  auto qat = [&](int r, int c) { return (uint32_t)((c >> 3) * (rows8 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
 
-  if (blockIdx.x * Cfg::kKeys < top) {
-    if (a.c.dim < DP) {
-      for (int i = threadIdx.x; i < Cfg::q / 16; i += 128) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-      __syncthreads();
-    }
+  // the scores to add to: slot of lane in each unit
+  const int mine = lane / 4 + (lane & 3) * 8;
+  const int64_t base = (int64_t)blockIdx.y * a.capacity;
+  float before[kUnits];
 #pragma unroll
-    for (int u = 0; u < Cfg::kUnits; ++u) {
-      const int slot = first + u * 32 + lane;
-      int page = 0, row = -1;
-      if (slot < top) {
+  for (int u = 0; u < kUnits; ++u) {
+    const int slot = first + u * 32 + mine;
+    before[u] = slot < a.capacity ? a.scores[base + slot] : 0.f;
+  }
+  if (blockIdx.x * Cfg::kKeys < top) {
+    if constexpr (kTma) {
+      const int boxes = 32 / a.box, u = lane / boxes, x = lane - u * boxes;
+      const int slot = first + u * 32 + x * a.box;
+      const bool on = u < kUnits && first + u * 32 < top;
+      int page = a.c.pages, row = 0;  // a box behind the last slot lies outside the descriptor's pages: zeros
+      if (on && slot < top) {
         int p;
         a.c.div.split(slot, p, row);
         page = a.c.page_of(b, p);
       }
-      const int c = lane % kLanesRow;
-      const __nv_bfloat16* kb = a.c.k + h * a.c.kh + c * 8;
+      if (threadIdx.x == 0) abort_flag = 0;
+      if (lane < kUnits) ptx::mbar_init(bar + 8 * lane, 1);
+      ptx::fence_mbar_init();
+      __syncwarp();
+      if (lane < kUnits && first + lane * 32 < top) ptx::mbar_arrive_expect_tx(bar + 8 * lane, Cfg::kTile);
+      __syncwarp();
+      if (on) {
 #pragma unroll
-      for (int i = 0; i < kLanesRow; ++i) {
-        const int r = lane / kLanesRow + i * (32 / kLanesRow);
-        const int p = __shfl_sync(0xffffffffu, page, r), x = __shfl_sync(0xffffffffu, row, r);
-        if (c * 8 < a.c.dim)
-          mma::cp_async_16_or_zero(kbase + u * Cfg::kTile + mma::tile_at<DP>(r, c),
-                                   x >= 0 ? kb + p * a.c.kp + x * a.c.ks : kb, x >= 0);
+        for (int c = 0; c < DP / 64; ++c)
+          ptx::tma_load_4d(kbase + u * Cfg::kTile + c * 4096 + x * a.box * 128, &maps.k, bar + 8 * u, c * 64, h, row, page);
       }
-      ptx::cp_async_commit();
+    } else {
+      if (a.c.dim < DP) {
+        for (int i = threadIdx.x; i < Cfg::q / 16; i += 128) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+      }
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const int slot = first + u * 32 + lane;
+        int page = 0, row = -1;
+        if (slot < top) {
+          int p;
+          a.c.div.split(slot, p, row);
+          page = a.c.page_of(b, p);
+        }
+        const int c = lane % kLanesRow;
+        const __nv_bfloat16* kb = a.c.k + h * a.c.kh + c * 8;
+#pragma unroll
+        for (int i = 0; i < kLanesRow; ++i) {
+          const int r = lane / kLanesRow + i * (32 / kLanesRow);
+          const int p = __shfl_sync(0xffffffffu, page, r), x = __shfl_sync(0xffffffffu, row, r);
+          if (c * 8 < a.c.dim)
+            mma::cp_async_16_or_zero(kbase + u * Cfg::kTile + mma::tile_at<32>(r, c),
+                                     x >= 0 ? kb + p * a.c.kp + x * a.c.ks : kb, x >= 0);
+        }
+      }
     }
     for (int i = threadIdx.x; i < rows8 * (DP / 8); i += 128) {
       const int r = i / (DP / 8), c = i - r * (DP / 8), e = a.i0 + r / a.G;
@@ -128,40 +163,34 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
           if (l != -INFINITY) f = make_float2(l * kLog2e, __int_as_float(n + e));
         }
       }
-      *reinterpret_cast<uint4*>(qs + mma::tile_at<DP>(r, c)) = v;
+      *reinterpret_cast<uint4*>(qs + qat(r, c)) = v;
       if (c == 0) info[r] = f;
     }
+    if constexpr (!kTma) ptx::cp_async_wait_all();
     __syncthreads();
   }
-  const int64_t base = (int64_t)blockIdx.y * a.capacity;
   const uint32_t qaddr = ptx::smem_addr(qs);
 #pragma unroll
-  for (int u = 0; u < Cfg::kUnits; ++u) {
+  for (int u = 0; u < kUnits; ++u) {
     const int slot0 = first + u * 32;
     float sum[4] = {0.f, 0.f, 0.f, 0.f};  // slots slot0 + lane / 4 + 8 i
     if (slot0 < top) {
-      if constexpr (Cfg::kUnits == 4) {
-        if (u == 0) ptx::cp_async_wait<3>();
-        if (u == 1) ptx::cp_async_wait<2>();
-        if (u == 2) ptx::cp_async_wait<1>();
-        if (u == 3) ptx::cp_async_wait<0>();
-      } else {
-        if (u == 0) ptx::cp_async_wait<1>();
-        if (u == 1) ptx::cp_async_wait<0>();
+      if constexpr (kTma) {
+        ptx::mbar_wait(bar + 8 * u, 0, &abort_flag);  // a wait that ran out is reported at the end
+        __syncwarp();
       }
-      __syncwarp();
       uint32_t kf[2][KS][4];
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          mma::ldsm_x4(kbase + u * Cfg::kTile + mma::tile_at<DP>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), kf[mt][k]);
+          mma::ldsm_x4(kbase + u * Cfg::kTile + mma::tile_at<32>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), kf[mt][k]);
       for (int r = 0; r < rows8; r += 8) {
         float s[2][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
           uint32_t f[4];
-          mma::ldsm_x4(qaddr + mma::tile_at<DP>(r + (lane & 7), 2 * k + (lane >> 3)), f);
+          mma::ldsm_x4(qaddr + qat(r + (lane & 7), 2 * k + (lane >> 3)), f);
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
             mma::bf16_16816(s[mt], kf[mt][k], f[0], f[1]);
@@ -185,29 +214,37 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
       sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
       sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
     }
-    const int sel = lane & 3, slot = slot0 + lane / 4 + sel * 8;
+    const int sel = lane & 3, slot = slot0 + mine;
     const float add = sel == 0 ? sum[0] : sel == 1 ? sum[1] : sel == 2 ? sum[2] : sum[3];
-    if (slot < a.capacity && (slot < top || a.out != a.scores)) a.out[base + slot] = a.scores[base + slot] + add;
+    if (slot < a.capacity && (slot < top || a.out != a.scores)) a.out[base + slot] = before[u] + add;
+  }
+  if constexpr (kTma) {
+    if (first < top && *(volatile int*)&abort_flag) {
+      if (lane == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
+      // copies in flight end before the CTA's memory is given back
+      volatile int gone = 0;
+      for (int u = 0; u < kUnits && first + u * 32 < top; ++u) ptx::mbar_wait(bar + 8 * u, 0, &gone);
+    }
   }
 }
 
-template <int DP>
-int scores_launch(ScoreArgs a, int64_t Hkv, int64_t B, cudaStream_t st) {
+template <int DP, bool kTma>
+int scores_launch(ScoreArgs a, const CacheMaps& maps, int64_t Hkv, int64_t B, cudaStream_t st) {
   using Cfg = ScoreCfg<DP>;
   static bool set[64] = {};
   int dev = 0;
   BS_CUDA(cudaGetDevice(&dev));
   constexpr int kMost = 128 * 1024;
   if (dev >= 64 || !set[dev]) {
-    BS_CUDA(cudaFuncSetAttribute(kv_scores_kernel<DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    BS_CUDA(cudaFuncSetAttribute(kv_scores_kernel<DP, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     if (dev < 64) set[dev] = true;
   }
   // as many accepted entries at a time as their queries fit beside the keys
-  const int step = std::max(1, (kMost - Cfg::q) / (DP * 2 + 8) / 8 * 8 / a.G);
+  const int step = std::max(1, (kMost - Cfg::smem(0)) / (DP * 2 + 8) / 8 * 8 / a.G);
   const dim3 grid((unsigned)cdiv(a.capacity, (int64_t)Cfg::kKeys), (unsigned)(B * Hkv));
   for (a.i0 = 0; a.i0 < a.A; a.i0 += step) {
     a.rows = std::min(step, a.A - a.i0) * a.G;
-    kv_scores_kernel<DP><<<grid, 128, Cfg::smem((a.rows + 7) / 8 * 8), st>>>(a);
+    kv_scores_kernel<DP, kTma><<<grid, 128, Cfg::smem((a.rows + 7) / 8 * 8), st>>>(a, maps);
     BS_LAUNCHED();
     a.scores = a.out;
   }
@@ -470,10 +507,15 @@ extern "C" int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t D = cache->dim;
-  if (D <= 32) return scores_launch<32>(a, cache->heads, cache->batch, st);
-  if (D <= 64) return scores_launch<64>(a, cache->heads, cache->batch, st);
-  if (D <= 96) return scores_launch<96>(a, cache->heads, cache->batch, st);
-  return scores_launch<128>(a, cache->heads, cache->batch, st);
+  CacheMaps maps = {};
+  a.box = cache_box_rows(cache, 32);
+  if (a.box >= 8) {
+    BS_TRY(cache_maps(cache, a.box, false, &maps));
+    return D <= 64 ? scores_launch<64, true>(a, maps, cache->heads, cache->batch, st)
+                   : scores_launch<128, true>(a, maps, cache->heads, cache->batch, st);
+  }
+  return D <= 64 ? scores_launch<64, false>(a, maps, cache->heads, cache->batch, st)
+                 : scores_launch<128, false>(a, maps, cache->heads, cache->batch, st);
 }
 
 extern "C" int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_t capacity, int64_t budget,
