@@ -90,7 +90,7 @@ struct TreeArgs {
   int box;          // slots of a TMA box, or 1
   __nv_bfloat16* out;
   float* lse;
-  float* part_o;    // [2 * grid][tile rows][dim]
+  float4* part_o;   // [2 * grid][dim / 4][tile rows]: rows adjacent, as the writers' threads are
   float2* part_ml;  // [2 * grid][tile rows]
   int min_chunk;
 };
@@ -352,20 +352,16 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
     const int row0 = cw.tile * kRows, rows = min(kRows, a.R - row0);
     const int t0 = row0 / a.G, toks = (row0 + rows - 1) / a.G - t0 + 1;
     // masks of the tile's tokens over the drafts, and each one's window
-    {
+    if (a.window || cw.k.lo + cw.end * kU > cw.k.n) {
       const int words = (a.T + 31) / 32;
       const int32_t* pos = a.pos + (int64_t)cw.b * a.T;
+#pragma unroll 4
       for (int i = warp; i < toks * words; i += 4) {
         const int tl = i / words, w = i - tl * words, t = t0 + tl, u = w * 32 + lane;
-        const int pt = pos[t];
+        const int uc = min(u, a.T - 1), pt = __ldg(pos + t), pu = u < a.T ? __ldg(pos + uc) : -1;
+        const bool may = a.mask ? __ldg(a.mask + cw.b * a.mask_b + (int64_t)t * a.T + uc) != 0 : u <= t;
         const int below = a.window ? max(pt, cw.k.n) - a.window : -1;
-        bool on = false;
-        if (pt >= 0 && u < a.T) {
-          const int pu = pos[u];
-          on = pu >= 0 && (!a.window || pu > below) &&
-               (a.mask ? a.mask[cw.b * a.mask_b + (int64_t)t * a.T + u] != 0 : u <= t);
-        }
-        const uint32_t m = __ballot_sync(0xffffffffu, on);
+        const uint32_t m = __ballot_sync(0xffffffffu, may && pt >= 0 && pu >= 0 && (!a.window || pu > below));
         if (lane == 0) {
           bits[tl * kWords + w] = m;
           if (w == 0) thr[tl] = pt >= 0 ? below : INT_MAX;
@@ -386,8 +382,8 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int col = k * 16 + half * 8;
-            qf[mt][k][e + 2 * half] =
-                on && col < a.c.dim ? __ldg(reinterpret_cast<const uint32_t*>(q + col)) : 0u;
+            const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(q + min(col, a.c.dim - 8)));
+            qf[mt][k][e + 2 * half] = on && col < a.c.dim ? v : 0u;
           }
       }
     int tl[MT][2];
@@ -546,8 +542,9 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
     const bool whole = cw.start == 0 && cw.end == cw.units;
     const int64_t slot = 2 * (int64_t)blockIdx.x + (cw.start == 0 ? 1 : 0);
     const int dim = a.c.dim;
-    for (int i = threadIdx.x; i < rows * (dim / 8); i += 128) {
-      const int row = i / (dim / 8), c = i - row * (dim / 8);
+    for (int i = threadIdx.x; i < kRows * (dim / 8); i += 128) {
+      const int row = whole ? i / (dim / 8) : i % kRows, c = whole ? i - row * (dim / 8) : i / kRows;
+      if (row >= rows) continue;
       float mx = -INFINITY, zz = 0.f;
       for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w * kRows + row].x);
       for (int w = 0; w < 4; ++w) {
@@ -557,9 +554,9 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
       const float4 v0 = *reinterpret_cast<const float4*>(merge + row * DP + c * 8);
       const float4 v1 = *reinterpret_cast<const float4*>(merge + row * DP + c * 8 + 4);
       if (!whole) {
-        float* po = a.part_o + (slot * kRows + row) * dim + c * 8;
-        *reinterpret_cast<float4*>(po) = v0;
-        *reinterpret_cast<float4*>(po + 4) = v1;
+        float4* po = a.part_o + (slot * (dim / 4) + 2 * c) * kRows + row;
+        po[0] = v0;
+        po[kRows] = v1;
         if (c == 0) a.part_ml[slot * kRows + row] = make_float2(mx, zz);
         continue;
       }
@@ -650,6 +647,57 @@ __device__ __forceinline__ uint32_t bit_range(int a, int b) {
   return below_b & ~below_a;
 }
 
+// Which drafts the rows of a warp's tokens may attend: a row of 256 bits (its
+// first ceil(T / 32) words) written by the lane of each row to `row`.  Lanes hold
+// consecutive rows, `tok` and its position `pt`; every lane calls.  The mask bytes
+// of kBatch tokens and two words are loaded at once.
+template <int kBatch>
+__device__ __forceinline__ void draft_bits(const TreeArgs& a, int b, int n, int tok, int pt, uint32_t* row) {
+  const int lane = threadIdx.x & 31;
+  const int t0 = __shfl_sync(0xffffffffu, tok, 0), t1 = __reduce_max_sync(0xffffffffu, tok);
+  const uint8_t* mask = a.mask ? a.mask + b * a.mask_b : nullptr;
+#pragma unroll 1
+  for (int i = 0; i < kMaxDrafts / 32; i += 2) {
+    if (i * 32 >= a.T) {
+      row[i] = row[i + 1] = 0;
+      continue;
+    }
+    int u[2], pu[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      u[h] = (i + h) * 32 + lane;
+      pu[h] = __ldg(a.pos + (int64_t)b * a.T + min(u[h], a.T - 1));
+      if (u[h] >= a.T) pu[h] = -1;
+    }
+#pragma unroll 1
+    for (int x = t0; x <= t1; x += kBatch) {
+      uint32_t on[kBatch][2];
+      if (mask) {  // loads without a condition, so that all are in flight together
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) on[j][h] = __ldg(mask + (int64_t)min(x + j, t1) * a.T + min(u[h], a.T - 1));
+      } else {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) on[j][h] = u[h] <= min(x + j, t1);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int t = min(x + j, t1);
+        const int px = __shfl_sync(0xffffffffu, pt, __ffs(__ballot_sync(0xffffffffu, tok == t)) - 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t v =
+              __ballot_sync(0xffffffffu, on[j][h] && pu[h] >= 0 && px >= 0 && (!a.window || pu[h] > max(px, n) - a.window));
+          if (tok == t) row[i + h] = v;
+        }
+      }
+    }
+  }
+}
+
 template <int DP, bool kPair>
 __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __grid_constant__ TreeArgs a,
                                                                      const __grid_constant__ CacheMaps maps) {
@@ -662,7 +710,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   __shared__ int abort_flag;
   __shared__ Range range;
   volatile int* abort = &abort_flag;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   const uint32_t sbase = ptx::smem_addr(smem);
   const uint32_t bar = sbase + Cfg::bars;
   auto full = [&](int s) { return bar + 8 * s; };
@@ -758,59 +806,65 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
       }
     } else if (warp >= 9) {
-      // ------------------------------------------------ MMA issue, one thread per pipeline
+      // ------------------------------------------------ MMA issue, one warp per pipeline
+      // The whole warp walks the loops and one elected thread issues: descriptors
+      // then stay in uniform registers (in a one-thread branch each product costs
+      // several moves to them, ~115 cycles).
       const int p = warp - 9;
-      if (lane == 0) {
-        const uint32_t idesc_s = ptx::idesc_bf16_f32(128, 128);
-        const uint32_t idesc_o = ptx::idesc_bf16_f32(128, DP) | (1u << 16);  // B with N contiguous
-        const uint32_t s_col = tmem + p * kSCol, o_col = tmem + kOCol + p * 128;
-        const uint32_t qs = sbase + Cfg::q + p * Cfg::kSlot;
-        int done = 0, pieces = 0;  // tiles and pieces of this pipeline so far
-        bool more = true;
-        while (more && ok) {
-          const int n = w.end - w.start;
-          const int first = kPair ? 0 : p, step = kPair ? 1 : 2;
-          if (first < n) {
-            ok = ptx::mbar_wait(qfull(p), pieces & 1, abort);
-            ++pieces;
-            for (int i = first; i < n && ok; i += step) {
-              const int ks = 2 * (base + i), vs = ks + 1;
-              const int ka = ks % Cfg::kSlots, va = vs % Cfg::kSlots;
-              ok = ptx::mbar_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
-              if (!ok) break;
-              ptx::tc_fence_after();
-              const uint32_t kt = sbase + ka * Cfg::kSlot;
+      const bool elected = ptx::elect_one();
+      constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) /* B with N contiguous */ |
+                                   (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
+      const uint32_t s_col = tmem + p * kSCol, o_col = tmem + kOCol + p * 128;
+      const uint64_t qd = ptx::sdesc_kmajor_sw128(sbase + Cfg::q + p * Cfg::kSlot);
+      const uint64_t kd0 = ptx::sdesc_kmajor_sw128(sbase), vd0 = sdesc_nmajor_sw128(sbase, 16384);
+      int done = 0, pieces = 0;  // tiles and pieces of this pipeline so far
+      bool more = true;
+      while (more && ok) {
+        const int n = w.end - w.start;
+        constexpr int step = kPair ? 1 : 2;
+        const int first = kPair ? 0 : p;
+        if (first < n) {
+          ok = warp_wait(qfull(p), pieces & 1, abort);
+          ++pieces;
+          for (int i = first; i < n && ok; i += step) {
+            const uint32_t ks = 2 * (base + i), vs = ks + 1;
+            const uint32_t ka = ks % Cfg::kSlots, va = vs % Cfg::kSlots;
+            ok = warp_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            if (elected) {
+              const uint64_t kd = kd0 + ka * (Cfg::kSlot >> 4);
 #pragma unroll
               for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-                ptx::mma_ss_bf16(s_col, ptx::sdesc_kmajor_sw128(qs + off), ptx::sdesc_kmajor_sw128(kt + off), idesc_s,
-                                 k > 0);
+                const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                ptx::mma_ss_bf16(s_col, qd + off, kd + off, idesc_s, k > 0);
               }
               ptx::tc_commit(sfull(p));
               ptx::tc_commit(empty(ka));
-              ok = ptx::mbar_wait(pready(p), done & 1, abort) &&
-                   ptx::mbar_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
-              if (!ok) break;
-              ptx::tc_fence_after();
-              const uint32_t vt = sbase + va * Cfg::kSlot;
+            }
+            ok = warp_wait(pready(p), done & 1, abort) && warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
+            if (!ok) break;
+            ptx::tc_fence_after();
+            if (elected) {
+              const uint64_t vd = vd0 + va * (Cfg::kSlot >> 4);
 #pragma unroll
-              for (int k = 0; k < 8; ++k)
-                ptx::mma_ts_bf16(o_col, s_col + k * 8, sdesc_nmajor_sw128(vt + k * 2048, 16384), idesc_o,
-                                 i > first || k > 0);
+              for (int k = 0; k < 8; ++k) ptx::mma_ts_bf16(o_col, s_col + k * 8, vd + k * 128, idesc_o, i > first || k > 0);
               ptx::tc_commit(empty(va));
               if (i + step >= n) ptx::tc_commit(odone(p));
-              ++done;
             }
+            __syncwarp();
+            ++done;
           }
-          base += n;
-          more = walk_next<kU>(a, r.p1, w);
         }
-        if (!ok) {
-          // products in flight end before tensor memory is given back
-          volatile int gone = 0;
-          ptx::tc_commit(drain(p));
-          ptx::mbar_wait(drain(p), 0, &gone);
-        }
+        base += n;
+        more = walk_next<kU>(a, r.p1, w);
+      }
+      if (!ok && elected) {
+        // products in flight end before tensor memory is given back
+        volatile int gone = 0;
+        ptx::tc_commit(drain(p));
+        ptx::mbar_wait(drain(p), 0, &gone);
       }
       __syncwarp();
     } else {
@@ -830,42 +884,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         const bool mine = t < rows, warp_on = (warp & 3) * 32 < rows;
         const int tok = mine ? (row0 + t) / a.G : 0, g = mine ? row0 + t - tok * a.G : 0;
         const int hq = w.h * a.G + g;
+        const int pt = mine ? a.pos[(int64_t)w.b * a.T + tok] : -1;
+        const float sink = mine && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
         int below = -1;  // keys up to here are outside the row's window (a row not in use is zeroed at the end)
         float m = -INFINITY, z = 0.f;
         if (first < n) {
-          // Q, and which keys this row may attend
+          // Q, and which keys this row may attend; the loads of both are in flight together
           uint8_t* qs = smem + Cfg::q + p * Cfg::kSlot;
           const __nv_bfloat16* q = a.q + w.b * a.qb + tok * a.qt + (int64_t)hq * a.qh;
+          uint4 v[DP / 8];
 #pragma unroll
-          for (int c = 0; c < DP / 8; ++c) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (mine && c * 8 < a.c.dim) v = __ldg(reinterpret_cast<const uint4*>(q + c * 8));
-            *reinterpret_cast<uint4*>(qs + (c >> 3) * 16384 + mma::tile_at<128>(t, c & 7)) = v;
-          }
+          for (int c = 0; c < DP / 8; ++c)
+            v[c] = __ldg(reinterpret_cast<const uint4*>(q + min(c * 8, a.c.dim - 8)));
+          if (a.window) below = max(pt, w.k.n) - a.window;
+          if (warp_on && w.k.lo + w.end * kU > w.k.n) draft_bits<8>(a, w.b, w.k.n, tok, pt, bits);
+#pragma unroll
+          for (int c = 0; c < DP / 8; ++c)
+            *reinterpret_cast<uint4*>(qs + mma::tile_at<128>(t, c)) = mine && c * 8 < a.c.dim ? v[c] : make_uint4(0, 0, 0, 0);
           ptx::fence_proxy_async_smem();
           ptx::mbar_arrive(qfull(p));
-          if (a.window) below = max(a.pos[(int64_t)w.b * a.T + tok], w.k.n) - a.window;
-          const int words = (a.T + 31) / 32;
-#pragma unroll 1
-          for (int i = 0; i < 8; ++i) bits[i] = 0;
-          if (warp_on) {
-            const int t0 = __shfl_sync(0xffffffffu, tok, 0);
-            const int t1 = __reduce_max_sync(0xffffffffu, tok);
-            for (int x = t0; x <= t1; ++x)
-              for (int i = 0; i < words; ++i) {
-                const int u = i * 32 + lane;
-                const int32_t* pos = a.pos + (int64_t)w.b * a.T;
-                const int px = pos[x];
-                bool on = false;
-                if (px >= 0 && u < a.T) {
-                  const int pu = pos[u];
-                  on = pu >= 0 && (!a.window || pu > max(px, w.k.n) - a.window) &&
-                       (a.mask ? a.mask[w.b * a.mask_b + (int64_t)x * a.T + u] != 0 : u <= x);
-                }
-                const uint32_t v = __ballot_sync(0xffffffffu, on);
-                if (mine && tok == x) bits[i] = v;
-              }
-          }
           for (int i = first; i < n; i += step) {
             ok = warp_wait(sfull(p), done & 1, abort);
             if (!ok) break;
@@ -980,8 +1017,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         const int64_t at = ((int64_t)w.b * a.T + tok) * a.Hkv * a.G + hq;
         float scale_o = 1.f;
         if (whole && mine) {
-          const bool used = a.pos[(int64_t)w.b * a.T + tok] >= 0;
-          const float sink = a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+          const bool used = pt >= 0;
           const float top = fmaxf(m, sink);
           const float ref = top == -INFINITY ? 0.f : top;
           const float f = m == -INFINITY ? 0.f : mma::exp2_fast(m - ref);
@@ -991,35 +1027,50 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         }
         if (!whole && mine && (kPair || p == 0)) a.part_ml[slot * kRows + row] = make_float2(m, z);
         if (warp_on) {
-          // columns of this group: all of its own tile, or one half of the shared one
-          constexpr int kHalf = kPair ? DP : DP / 2;
-          const int c0 = kPair ? 0 : p * kHalf;
+          // columns of this group: all of its own tile, or one half of the shared one.
+          // bf16 rows go through the piece's Q (no longer read) to be stored in lines.
+          constexpr int kCols = kPair ? DP : DP / 2;
+          const int c0 = kPair ? 0 : p * kCols;
+          uint8_t* stage = smem + Cfg::q + p * Cfg::kSlot;  // a warp's rows where its Q rows were
 #pragma unroll 1
-          for (int c = c0; c < c0 + kHalf; c += 16) {
-            uint32_t o0[16], o1[16];
-            ptx::tmem_ld_32x32b_x16(tmem + lanes + kOCol + (kPair ? p * 128 : 0) + c, o0);
-            if (!kPair) ptx::tmem_ld_32x32b_x16(tmem + lanes + kOCol + 128 + c, o1);
+          for (int c = c0; c < c0 + kCols; c += 32) {
+            float x[32], y[32];
+            ptx::tmem_ld_32x32b_x32(tmem + lanes + kOCol + (kPair ? p * 128 : 0) + c, reinterpret_cast<uint32_t*>(x));
+            if (!kPair) ptx::tmem_ld_32x32b_x32(tmem + lanes + kOCol + 128 + c, reinterpret_cast<uint32_t*>(y));
             ptx::tmem_wait_ld();
-            float x[16];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              x[e] = f0 == 0.f ? 0.f : __uint_as_float(o0[e]) * f0;
-              if (!kPair && f1 != 0.f) x[e] += __uint_as_float(o1[e]) * f1;
+            for (int e = 0; e < 32; ++e) {
+              x[e] = f0 == 0.f ? 0.f : x[e] * f0;
+              if (!kPair && f1 != 0.f) x[e] += y[e] * f1;
             }
+            if (whole) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if (!mine || c + j * 8 >= dim) continue;
-              if (whole) {
+              for (int j = 0; j < 4; ++j) {
                 uint32_t pk[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   pk[e] = scale_o == 0.f ? 0u : pack_bf16x2(x[j * 8 + 2 * e] * scale_o, x[j * 8 + 2 * e + 1] * scale_o);
-                *reinterpret_cast<uint4*>(a.out + at * dim + c + j * 8) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-              } else {
-                float* po = a.part_o + (slot * kRows + row) * dim + c + j * 8;
-                *reinterpret_cast<float4*>(po) = make_float4(x[j * 8], x[j * 8 + 1], x[j * 8 + 2], x[j * 8 + 3]);
-                *reinterpret_cast<float4*>(po + 4) = make_float4(x[j * 8 + 4], x[j * 8 + 5], x[j * 8 + 6], x[j * 8 + 7]);
+                const int chunk = (c - c0) / 8 + j;
+                *reinterpret_cast<uint4*>(stage + mma::tile_at<128>(t, chunk)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
               }
+            } else if (mine) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (c + j * 4 < dim)
+                  a.part_o[(slot * (dim / 4) + c / 4 + j) * kRows + row] =
+                      make_float4(x[j * 4], x[j * 4 + 1], x[j * 4 + 2], x[j * 4 + 3]);
+            }
+            __syncwarp();
+          }
+          if (whole) {
+            constexpr int kChunks = kCols / 8, kAtOnce = 32 / kChunks;
+#pragma unroll
+            for (int j = 0; j < 32 / kAtOnce; ++j) {
+              const int r = j * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+              const int64_t to = __shfl_sync(0xffffffffu, at, r);
+              const bool on = __shfl_sync(0xffffffffu, (int)mine, r);
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + mma::tile_at<128>((warp & 3) * 32 + r, chunk));
+              if (on && c0 + chunk * 8 < dim) *reinterpret_cast<uint4*>(a.out + to * dim + c0 + chunk * 8) = v;
             }
             __syncwarp();
           }
@@ -1082,9 +1133,11 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
   if (c0 == c1) return;
   const int dim = a.c.dim, row0 = tile * kRows, rows = min(kRows, a.R - row0);
   const int first = blockIdx.y * kJoinRows, last = min(rows, first + kJoinRows);
-  for (int i = first * (dim / 4) + threadIdx.x; i < last * (dim / 4); i += 128) {
-    const int row = i / (dim / 4), c = i - row * (dim / 4);
+  for (int i = threadIdx.x; i < kJoinRows * (dim / 4); i += 128) {
+    const int row = first + i % kJoinRows, c = i / kJoinRows;
+    if (row >= last) continue;
     float mx = -INFINITY;
+#pragma unroll 4
     for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, a.part_ml[(2 * (int64_t)x + (x == c0)) * kRows + row].x);
     const int t = (row0 + row) / a.G, hq = h * a.G + row0 + row - t * a.G;
     const bool used = a.pos[(int64_t)b * a.T + t] >= 0;
@@ -1093,13 +1146,13 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
     const float ref = top == -INFINITY ? 0.f : top;
     float den = a.sinks ? mma::exp2_fast(sink - ref) : 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int x = c0; x <= c1; ++x) {
-      const int64_t at = (2 * (int64_t)x + (x == c0)) * kRows + row;
-      const float2 mz = a.part_ml[at];
-      if (mz.x == -INFINITY) continue;
-      const float f = mma::exp2_fast(mz.x - ref);
+      const int64_t slot = 2 * (int64_t)x + (x == c0);
+      const float2 mz = a.part_ml[slot * kRows + row];
+      const float4 p = a.part_o[(slot * (dim / 4) + c) * kRows + row];
+      const float f = mz.x == -INFINITY ? 0.f : mma::exp2_fast(mz.x - ref);
       den += mz.y * f;
-      const float4 p = *reinterpret_cast<const float4*>(a.part_o + at * dim + c * 4);
       v.x += p.x * f;
       v.y += p.y * f;
       v.z += p.z * f;
@@ -1229,8 +1282,8 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
   const int grid = grid_for(rows);
-  a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * D);
+  a.part_o = static_cast<float4*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * (D / 4));
   a.min_chunk = rows <= 32 ? 4 : 2;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
