@@ -593,10 +593,11 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 }
 
 // ---------------------------------------------------------------- many rows
-// Row tiles of 128 on tcgen05: S = Q K^T (128 x 128 per tile of keys, both
+// Row tiles of 128 on tcgen05: S = Q K^T (128 x 64 per half tile of keys, both
 // operands in shared memory) into tensor memory, the weights P = 2^(x - m) back
-// into tensor memory as bf16, O += P V with P as the tensor-memory operand and V
-// as it lies in the cache (keys along K, the head contiguous).
+// into the same columns as bf16, O += P V with P as the tensor-memory operand and
+// V as it lies in the cache (keys along K, the head contiguous).  Two half tiles
+// of S alternate, so that the next one is ready when a softmax step ends.
 //
 // Two pipelines per CTA, each a group of four softmax warps (a thread per row)
 // and an MMA warp, so that one pipeline's products run while the other's
@@ -616,7 +617,7 @@ struct TilesCfg {
   static constexpr int bits = q + 2 * kSlot;             // [256 threads][8 words]
   static constexpr int ml = bits + 256 * 32;             // [2][128] float2
   static constexpr int bars = ml + 2 * 128 * 8;
-  static constexpr int total = bars + 256 + 1024;        // barriers; alignment of the base
+  static constexpr int total = bars + 320 + 1024;        // barriers; alignment of the base
 };
 constexpr int kTileThreads = 352;
 constexpr uint32_t kSCol = 128, kOCol = 256;             // pipeline p: S at p * kSCol, O at kOCol + p * 128
@@ -716,13 +717,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   auto full = [&](int s) { return bar + 8 * s; };
   auto empty = [&](int s) { return bar + 8 * (Cfg::kSlots + s); };
   constexpr int kB = 16 * Cfg::kSlots;
-  auto sfull = [&](int p) { return bar + kB + 8 * p; };
-  auto pready = [&](int p) { return bar + kB + 16 + 8 * p; };
-  auto qfull = [&](int p) { return bar + kB + 32 + 8 * p; };
-  auto odone = [&](int p) { return bar + kB + 48 + 8 * p; };
-  auto drain = [&](int p) { return bar + kB + 64 + 8 * p; };
-  const uint32_t meet = bar + kB + 80;
-  static_assert(kB + 88 <= 256, "barriers");
+  auto sfull = [&](int p, int half) { return bar + kB + 16 * p + 8 * half; };
+  auto pready = [&](int p, int half) { return bar + kB + 32 + 16 * p + 8 * half; };
+  auto qfull = [&](int p) { return bar + kB + 64 + 8 * p; };
+  auto pvdone = [&](int p) { return bar + kB + 80 + 8 * p; };
+  auto drain = [&](int p) { return bar + kB + 96 + 8 * p; };
+  const uint32_t meet = bar + kB + 112;
+  static_assert(kB + 120 <= 320, "barriers");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid < 128) {
@@ -738,10 +739,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       ptx::mbar_init(empty(i), kPair ? 2 : 1);
     }
     for (int p = 0; p < 2; ++p) {
-      ptx::mbar_init(sfull(p), 1);
-      ptx::mbar_init(pready(p), 128);
+      ptx::mbar_init(sfull(p, 0), 1);
+      ptx::mbar_init(sfull(p, 1), 1);
+      ptx::mbar_init(pready(p, 0), 128);  // one per half: a warp may be a half tile ahead of its group
+      ptx::mbar_init(pready(p, 1), 128);
       ptx::mbar_init(qfull(p), 128);
-      ptx::mbar_init(odone(p), 1);
+      ptx::mbar_init(pvdone(p), 1);
       ptx::mbar_init(drain(p), 1);
     }
     ptx::mbar_init(meet, 256);
@@ -812,49 +815,59 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       // several moves to them, ~115 cycles).
       const int p = warp - 9;
       const bool elected = ptx::elect_one();
-      constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
+      constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
       constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) /* B with N contiguous */ |
                                    (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
       const uint32_t s_col = tmem + p * kSCol, o_col = tmem + kOCol + p * 128;
       const uint64_t qd = ptx::sdesc_kmajor_sw128(sbase + Cfg::q + p * Cfg::kSlot);
       const uint64_t kd0 = ptx::sdesc_kmajor_sw128(sbase), vd0 = sdesc_nmajor_sw128(sbase, 16384);
-      int done = 0, pieces = 0;  // tiles and pieces of this pipeline so far
+      constexpr int step = kPair ? 1 : 2;
+      const int first = kPair ? 0 : p;
+      int halves = 0, pieces = 0;  // half tiles and pieces of this pipeline so far
       bool more = true;
       while (more && ok) {
-        const int n = w.end - w.start;
-        constexpr int step = kPair ? 1 : 2;
-        const int first = kPair ? 0 : p;
-        if (first < n) {
+        const int n = w.end - w.start, total = first < n ? 2 * ((n - first + step - 1) / step) : 0;
+        // S of half tile h of the piece, into half h & 1 of the S columns
+        auto scores = [&](int h) {
+          const uint32_t ks = 2 * (base + first + (h >> 1) * step), ka = ks % Cfg::kSlots;
+          if (!(h & 1)) {
+            ok = warp_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
+            if (!ok) return;
+            ptx::tc_fence_after();
+          }
+          if (elected) {
+            const uint64_t kd = kd0 + ka * (Cfg::kSlot >> 4) + (h & 1) * (8192 >> 4);
+#pragma unroll
+            for (int k = 0; k < DP / 16; ++k) {
+              const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+              ptx::mma_ss_bf16(s_col + (h & 1) * 64, qd + off, kd + off, idesc_s, k > 0);
+            }
+            ptx::tc_commit(sfull(p, h & 1));
+            if (h & 1) ptx::tc_commit(empty(ka));
+          }
+          __syncwarp();
+        };
+        if (total) {
           ok = warp_wait(qfull(p), pieces & 1, abort);
           ++pieces;
-          for (int i = first; i < n && ok; i += step) {
-            const uint32_t ks = 2 * (base + i), vs = ks + 1;
-            const uint32_t ka = ks % Cfg::kSlots, va = vs % Cfg::kSlots;
-            ok = warp_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
+          if (ok) scores(0);
+          if (ok) scores(1);
+          for (int h = 0; h < total && ok; ++h) {
+            const uint32_t vs = 2 * (base + first + (h >> 1) * step) + 1, va = vs % Cfg::kSlots;
+            ok = warp_wait(pready(p, h & 1), (halves >> 1) & 1, abort) && warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
             if (!ok) break;
+            ++halves;
             ptx::tc_fence_after();
             if (elected) {
-              const uint64_t kd = kd0 + ka * (Cfg::kSlot >> 4);
+              const uint64_t vd = vd0 + va * (Cfg::kSlot >> 4) + (h & 1) * (8192 >> 4);
 #pragma unroll
-              for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                ptx::mma_ss_bf16(s_col, qd + off, kd + off, idesc_s, k > 0);
-              }
-              ptx::tc_commit(sfull(p));
-              ptx::tc_commit(empty(ka));
-            }
-            ok = warp_wait(pready(p), done & 1, abort) && warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
-            if (!ok) break;
-            ptx::tc_fence_after();
-            if (elected) {
-              const uint64_t vd = vd0 + va * (Cfg::kSlot >> 4);
-#pragma unroll
-              for (int k = 0; k < 8; ++k) ptx::mma_ts_bf16(o_col, s_col + k * 8, vd + k * 128, idesc_o, i > first || k > 0);
-              ptx::tc_commit(empty(va));
-              if (i + step >= n) ptx::tc_commit(odone(p));
+              for (int k = 0; k < 4; ++k)
+                ptx::mma_ts_bf16(o_col, s_col + (h & 1) * 64 + k * 8, vd + k * 128, idesc_o, h > 0 || k > 0);
+              ptx::tc_commit(pvdone(p));
+              if (h & 1) ptx::tc_commit(empty(va));
             }
             __syncwarp();
-            ++done;
+            if (h + 2 < total) scores(h + 2);
           }
         }
         base += n;
@@ -874,11 +887,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       const uint32_t s_col = tmem + lanes + p * kSCol;
       uint32_t* bits = reinterpret_cast<uint32_t*>(smem + Cfg::bits) + tid * 8;
       float2* ml = reinterpret_cast<float2*>(smem + Cfg::ml);
-      int done = 0, pieces[2] = {0, 0}, meets = 0;
+      constexpr int step = kPair ? 1 : 2;
+      const int first = kPair ? 0 : p;
+      int halves = 0, meets = 0;  // half tiles of this pipeline so far
       bool more = true;
       while (more && ok) {
         const int n = w.end - w.start;
-        const int first = kPair ? 0 : p, step = kPair ? 1 : 2;
         const int row0 = w.tile * kRows + (kPair ? p * 128 : 0);
         const int rows = min(128, a.R - row0);  // may be negative: the second tile of a pair is empty
         const bool mine = t < rows, warp_on = (warp & 3) * 32 < rows;
@@ -903,33 +917,36 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
             *reinterpret_cast<uint4*>(qs + mma::tile_at<128>(t, c)) = mine && c * 8 < a.c.dim ? v[c] : make_uint4(0, 0, 0, 0);
           ptx::fence_proxy_async_smem();
           ptx::mbar_arrive(qfull(p));
-          for (int i = first; i < n; i += step) {
-            ok = warp_wait(sfull(p), done & 1, abort);
+          const int total = 2 * ((n - first + step - 1) / step);
+          int done = halves;
+          for (int h = 0; h < total; ++h, ++done) {
+            ok = warp_wait(sfull(p, h & 1), (done >> 1) & 1, abort);
             if (!ok) break;
-            ++done;
             ptx::tc_fence_after();
-            const int key0 = w.k.lo + (w.start + i) * kU;
+            const int i = first + (h >> 1) * step;
+            const int tile0 = w.k.lo + (w.start + i) * kU, key0 = tile0 + (h & 1) * 64;
+            const uint32_t sp = s_col + (h & 1) * 64;
             if (warp_on) {
-              const bool slow = key0 + kU > w.k.n || a.window || a.scale2 < 0.f;
-              float v[128];
-#pragma unroll
-              for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(s_col + c * 32, reinterpret_cast<uint32_t*>(v + c * 32));
+              const bool slow = key0 + 64 > w.k.n || a.window || a.scale2 < 0.f;
+              float v[64];
+              ptx::tmem_ld_32x32b_x32(sp, reinterpret_cast<uint32_t*>(v));
+              ptx::tmem_ld_32x32b_x32(sp + 32, reinterpret_cast<uint32_t*>(v + 32));
               ptx::tmem_wait_ld();
               if (slow) {
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
+                for (int c = 0; c < 2; ++c) {
                   const int k0 = key0 + c * 32;
                   const uint32_t see = bit_range(below + 1 - k0, w.k.n - k0) | bits_from(bits, k0 - w.k.n);
 #pragma unroll
                   for (int e = 0; e < 32; ++e) v[c * 32 + e] = see >> e & 1 ? v[c * 32 + e] * a.scale2 : -INFINITY;
                 }
               }
-              float top[4];
+              float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-              for (int e = 0; e < 4; ++e) top[e] = v[e];
+              for (int e = 4; e < 64; e += 8)
 #pragma unroll
-              for (int e = 4; e < 128; ++e) top[e & 3] = fmaxf(top[e & 3], v[e]);
-              float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                for (int x = 0; x < 4; ++x) top[x] = e + x + 4 < 64 ? mma::max3(top[x], v[e + x], v[e + x + 4]) : fmaxf(top[x], v[e + x]);
+              float mx = fmaxf(mma::max3(top[0], top[1], top[2]), top[3]);
               const float mul = slow ? 1.f : a.scale2;
               mx *= mul;
               const bool move = mx > m + kRescale || (m == -INFINITY && mx > -INFINITY);
@@ -939,23 +956,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                   z *= f;
                   m = mx;
                 }
-                if (i > first) {
+                if (h > 0) {
+                  ok = warp_wait(pvdone(p), (done - 1) & 1, abort);
+                  if (!ok) break;
+                  ptx::tc_fence_after();
                   const uint32_t o_col = tmem + lanes + kOCol + p * 128;
 #pragma unroll 1
-                  for (int c = 0; c < DP / 16; ++c) {
-                    uint32_t o[16];
-                    ptx::tmem_ld_32x32b_x16(o_col + c * 16, o);
+                  for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t o[32];
+                    ptx::tmem_ld_32x32b_x32(o_col + c * 32, o);
                     ptx::tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    ptx::tmem_st_32x32b_x16(o_col + c * 16, o);
+                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    ptx::tmem_st_32x32b_x32(o_col + c * 32, o);
                   }
                 }
               }
               const float ref = m == -INFINITY ? 0.f : m;
               float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
-              for (int c = 0; c < 4; ++c) {
+              for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -965,16 +985,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                   sum = mma::add2(sum, x);
                   pk[e] = pack_bf16x2(x.x, x.y);
                 }
-                ptx::tmem_st_32x32b_x16(s_col + c * 16, pk);
+                ptx::tmem_st_32x32b_x16(sp + c * 16, pk);
               }
               z += sum.x + sum.y;
             }
-            if (key0 < w.k.low || key0 + kU > w.k.n) {
+            if (!(h & 1) && (tile0 < w.k.low || tile0 + kU > w.k.n)) {
               // the tile's boxes bring all their slots: those that hold no key become zeros in V
               const int vs = 2 * (base + i) + 1, va = vs % Cfg::kSlots;
               ok = warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
               if (!ok) break;
-              if (!holds_key(a, w.b, w.k, key0 + t)) {
+              if (!holds_key(a, w.b, w.k, tile0 + t)) {
                 uint8_t* row = smem + va * Cfg::kSlot + t * 128;
 #pragma unroll
                 for (int c = 0; c < DP / 8; ++c)
@@ -984,16 +1004,15 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
             }
             if (warp_on) ptx::tmem_wait_st();
             ptx::tc_fence_before();
-            ptx::mbar_arrive(pready(p));
+            ptx::mbar_arrive(pready(p, h & 1));
           }
         }
         if (!ok) break;
         // ---- end of the piece: read the accumulators
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          if ((kPair && x != p) || (kPair ? 0 : x) >= n) continue;
-          ok = ok && warp_wait(odone(x), pieces[x] & 1, abort);
-          ++pieces[x];
+        if (first < n) {
+          halves += 2 * ((n - first + step - 1) / step);
+          // the last but one first: a parity alone does not tell the last from the one two before
+          ok = warp_wait(pvdone(p), halves & 1, abort) && warp_wait(pvdone(p), (halves - 1) & 1, abort);
         }
         if (!ok) break;
         ptx::tc_fence_after();
@@ -1001,10 +1020,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         if (!kPair) {
           // both pipelines hold the same rows: common maximum, sums together
           ml[p * 128 + t] = make_float2(m, z);
+          ptx::tc_fence_before();
           ptx::mbar_arrive(meet);
           ok = warp_wait(meet, meets & 1, abort);
           if (!ok) break;
           ++meets;
+          ptx::tc_fence_after();
           const float2 m0 = ml[t], m1 = ml[128 + t];
           m = fmaxf(m0.x, m1.x);
           f0 = m0.x == -INFINITY ? 0.f : mma::exp2_fast(m0.x - m);
