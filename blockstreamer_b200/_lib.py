@@ -136,7 +136,7 @@ def load(path: str | None = None) -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Call an int-returning entry point and raise on a non-zero status."""
-    lib = load()
+    lib = _lib or load()
     status = getattr(lib, name)(*args)
     if status != BS_OK:
         msg = lib.bs_last_error_string().decode(errors="replace")

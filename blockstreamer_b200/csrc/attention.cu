@@ -88,6 +88,7 @@ struct TreeArgs {
   float scale2;  // scale * log2(e)
   int window, T, G, R, tiles, Hkv, B;
   int box;          // slots of a TMA box, or 1
+  int setup;        // what starting an item costs, in units: it is counted as so many more
   __nv_bfloat16* out;
   float* lse;
   float4* part_o;   // [2 * grid][dim / 4][tile rows]: rows adjacent, as the writers' threads are
@@ -113,8 +114,10 @@ __device__ __forceinline__ bool holds_key(const TreeArgs& a, int b, const Keys& 
   return slot >= k.low && (slot < k.n || (slot < k.hi && __ldg(a.pos + (int64_t)b * a.T + slot - k.n) >= 0));
 }
 
-// Where the work of CTA `cta` of `grid` lies, units of kU keys: its range
-// [p0, p1) and the first item in it.  Every thread of a 128-thread CTA calls.
+// Where the work of CTA `cta` of `grid` lies: its range [p0, p1) of the units of
+// all items, item by item, and the sequence that holds unit p0.  An item has
+// `setup` units that stand for its start (Q, masks, epilogue), then one for each
+// kU keys.  The CTA's first 128 threads call.
 struct Range {
   int64_t p0, p1, chunk;
   int b;           // sequence of unit p0
@@ -123,30 +126,26 @@ struct Range {
 template <int kU>
 __device__ __forceinline__ int64_t units_of(const TreeArgs& a, int b) {
   const Keys k = keys_of(a, b);
-  return (k.hi - k.lo + kU - 1) / kU;
+  return a.setup + (k.hi - k.lo + kU - 1) / kU;
 }
 __device__ __forceinline__ void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 template <int kU>
 __device__ Range locate(const TreeArgs& a, int cta, int grid, int64_t* sums /* smem [6] */) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t per = (int64_t)a.Hkv * a.tiles;
+  Range r = {};
   int64_t total = 0;
-  for (int b = threadIdx.x; b < a.B; b += 128) total += units_of<kU>(a, b) * per;
+  if (a.B > 128) {
+    for (int b = threadIdx.x; b < a.B; b += 128) total += units_of<kU>(a, b) * per;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) sums[warp] = total;
-  sync128();
-  total = sums[0] + sums[1] + sums[2] + sums[3];
-  Range r;
-  r.chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
-  r.p0 = min(total, cta * r.chunk);
-  r.p1 = min(total, r.p0 + r.chunk);
-  r.b = 0;
-  r.before = 0;
-  if (r.p0 >= r.p1) return r;
-  // the sequence that holds unit p0: a scan of the sequences' units, 128 at a time
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) sums[warp] = total;
+    sync128();
+    total = sums[0] + sums[1] + sums[2] + sums[3];
+  }
+  // a scan of the sequences' units, 128 at a time (one step gives the total too)
   int64_t run = 0;
-  for (int base = 0; base < a.B && run <= r.p0; base += 128) {
+  for (int base = 0; base < a.B; base += 128) {
     const int b = base + threadIdx.x;
     const int64_t w = b < a.B ? units_of<kU>(a, b) * per : 0;
     int64_t incl = w;
@@ -161,12 +160,70 @@ __device__ Range locate(const TreeArgs& a, int cta, int grid, int64_t* sums /* s
     int64_t start = run + incl - w;
     for (int i = 0; i < warp; ++i) start += sums[i];
     run += sums[0] + sums[1] + sums[2] + sums[3];
+    if (base == 0) {
+      if (a.B <= 128) total = run;
+      r.chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
+      r.p0 = min(total, cta * r.chunk);
+      r.p1 = min(total, r.p0 + r.chunk);
+      if (r.p0 >= r.p1) return r;
+    }
     if (w > 0 && start <= r.p0 && r.p0 < start + w) sums[4] = b, sums[5] = start;
+    if (run > r.p0) break;
   }
   sync128();
   r.b = (int)sums[4];
   r.before = sums[5];
   return r;
+}
+
+// The pieces of a CTA's range, one per item that it touches; pieces without keys
+// are passed over.
+struct Walk {
+  int b, h, tile;
+  Keys k;
+  int u;               // the caller's next unit
+  int start, end;      // units of keys of this piece
+  int units;           // units of keys of the item
+  int len;             // of the piece, with the units that stand for the start
+  int64_t left;        // of the range, this piece included
+  __device__ __forceinline__ bool whole() const { return start == 0 && end == units; }
+};
+template <int kU>
+__device__ __forceinline__ bool walk_piece(const TreeArgs& a, Walk& w, int first) {
+  w.units = (w.k.hi - w.k.lo + kU - 1) / kU;
+  w.len = (int)min((int64_t)(w.units + a.setup - first), w.left);
+  w.start = max(0, first - a.setup);
+  w.end = max(0, first + w.len - a.setup);
+  return w.end > w.start;
+}
+// The next piece of the range; false at its end.
+template <int kU>
+__device__ __forceinline__ bool walk_next(const TreeArgs& a, Walk& w) {
+  while (true) {
+    w.left -= w.len;
+    if (w.left <= 0) return false;
+    if (++w.tile == a.tiles) {
+      w.tile = 0;
+      if (++w.h == a.Hkv) {
+        w.h = 0;
+        ++w.b;
+        w.k = keys_of(a, w.b);
+      }
+    }
+    if (walk_piece<kU>(a, w, 0)) return true;
+  }
+}
+template <int kU>
+__device__ __forceinline__ bool walk_begin(const TreeArgs& a, const Range& r, Walk& w) {
+  w.b = r.b;
+  w.k = keys_of(a, r.b);
+  const int64_t units = a.setup + (w.k.hi - w.k.lo + kU - 1) / kU;
+  const int64_t rel = r.p0 - r.before;
+  const int item = (int)(rel / units);
+  w.h = item / a.tiles;
+  w.tile = item - w.h * a.tiles;
+  w.left = r.p1 - r.p0;
+  return walk_piece<kU>(a, w, (int)(rel - item * units)) || walk_next<kU>(a, w);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -188,58 +245,14 @@ template <int DP, int MT>
 struct RowsSmem {
   static constexpr int kRows = 16 * MT;
   static constexpr int merge = 4 * RowsCfg<DP>::kWarpBytes;
-  static constexpr int ml = merge + kRows * DP * 4;            // [4 warps][rows] float2
+  static constexpr int kBufs = MT * DP == 64 ? 2 : 1;          // warps whose O is passed at once
+  static constexpr int ml = merge + kBufs * kRows * DP * 4;    // [4 warps][rows] float2
   static constexpr int bits = ml + 4 * kRows * 8;              // [rows][8] words
   static constexpr int thr = bits + kRows * (kMaxDrafts / 32) * 4;
   static constexpr int sums = (thr + kRows * 4 + 15) / 16 * 16;
   static constexpr int bars = sums + 64;                       // [4 warps][kStages]
   static constexpr int total = bars + 4 * RowsCfg<DP>::kStages * 8 + 1024;
 };
-
-// The units of a CTA's range as one warp meets them (it takes every fourth
-// unit of each item's piece).
-struct Walk {
-  int b, h, tile;
-  Keys k;
-  int u, end;      // next unit of this warp; end of the piece, in units of the item
-  int64_t pos;     // global index of the piece's first unit
-  int start;       // first unit of the piece
-  int units;       // units of the item
-};
-template <int kU>
-__device__ __forceinline__ void walk_piece(const TreeArgs& a, Walk& w, int64_t pos, int64_t p1, int first) {
-  w.units = (w.k.hi - w.k.lo + kU - 1) / kU;
-  w.pos = pos;
-  w.start = first;
-  w.end = (int)min((int64_t)w.units, first + (p1 - pos));
-}
-template <int kU>
-__device__ __forceinline__ void walk_begin(const TreeArgs& a, const Range& r, Walk& w) {
-  w.b = r.b;
-  w.k = keys_of(a, r.b);
-  const int units = (w.k.hi - w.k.lo + kU - 1) / kU;
-  const int64_t rel = r.p0 - r.before;
-  const int item = (int)(rel / units);
-  w.h = item / a.tiles;
-  w.tile = item - w.h * a.tiles;
-  walk_piece<kU>(a, w, r.p0, r.p1, (int)(rel - (int64_t)item * units));
-}
-// The next piece of the range; false at its end.
-template <int kU>
-__device__ __forceinline__ bool walk_next(const TreeArgs& a, int64_t p1, Walk& w) {
-  const int64_t pos = w.pos + (w.end - w.start);
-  if (pos >= p1) return false;
-  if (++w.tile == a.tiles) {
-    w.tile = 0;
-    if (++w.h == a.Hkv) {
-      w.h = 0;
-      ++w.b;
-      w.k = keys_of(a, w.b);
-    }
-  }
-  walk_piece<kU>(a, w, pos, p1, 0);
-  return true;
-}
 
 template <int DP, int MT, bool kTma>
 __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant__ TreeArgs a,
@@ -272,19 +285,19 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
   }
   __syncthreads();
   const Range r = locate<kU>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + Sm::sums));
-  if (r.p0 >= r.p1) return;
+  Walk lw, cw;
+  if (r.p0 >= r.p1 || !walk_begin<kU>(a, r, lw)) return;
+  cw = lw;
 
   // ---- loading.  Lane g holds the page and row of the next unit's g-th box (or,
   // without TMA, slot); pages are looked up one unit ahead.
   const int box = kTma ? min(a.box, kU) : 1, boxes = kU / box;
-  Walk lw;
-  walk_begin<kU>(a, r, lw);
   lw.u = lw.start + warp;
   bool more = true;
   int next_page = 0, next_row = -1;  // row < 0: no key there
   auto find = [&]() {
     while (more && lw.u >= lw.end) {
-      more = walk_next<kU>(a, r.p1, lw);
+      more = walk_next<kU>(a, lw);
       lw.u = lw.start + warp;
     }
     next_row = -1;
@@ -346,8 +359,6 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
   int stage = 0, phase = 0;
 
   // ---- pieces
-  Walk cw;
-  walk_begin<kU>(a, r, cw);
   while (true) {
     const int row0 = cw.tile * kRows, rows = min(kRows, a.R - row0);
     const int t0 = row0 / a.G, toks = (row0 + rows - 1) / a.G - t0 + 1;
@@ -498,11 +509,23 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
       }
     }
 
-    // ---- the warps' parts meet: common maximum, then their O in warp order
+    // ---- the warps' parts meet: common maximum, then O of warps 2, 3 to 0, 1 and of 1 to 0
+    // (what the rows' ends need is loaded meanwhile)
+    const bool whole = cw.whole();
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (cw.start == 0 ? 1 : 0);
+    const int dim = a.c.dim;
+    int64_t at[MT][2];
+    float sink[MT][2];
+    bool used[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        const int row = min(mt * 16 + lane / 4 + e * 8, rows - 1);
+        const int t = (row0 + row) / a.G, h = cw.h * a.G + row0 + row - t * a.G;
+        at[mt][e] = ((int64_t)cw.b * a.T + t) * a.Hkv * a.G + h;
+        used[mt][e] = __ldg(a.pos + (int64_t)cw.b * a.T + t) >= 0;
+        sink[mt][e] = a.sinks ? __ldg(a.sinks + h) * kLog2e : -INFINITY;
         z[mt][e] += __shfl_xor_sync(0xffffffffu, z[mt][e], 1);
         z[mt][e] += __shfl_xor_sync(0xffffffffu, z[mt][e], 2);
         if ((lane & 3) == 0) ml[warp * kRows + mt * 16 + lane / 4 + e * 8] = make_float2(m[mt][e], z[mt][e]);
@@ -513,71 +536,82 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = mt * 16 + lane / 4 + e * 8;
-        float mx = -INFINITY;
+        float mx = -INFINITY, zz = 0.f;
+#pragma unroll
         for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w * kRows + row].x);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float2 v = ml[w * kRows + row];
+          zz += v.x > -INFINITY ? v.y * mma::exp2_fast(v.x - mx) : 0.f;
+        }
         const float f = mx == -INFINITY ? 0.f : mma::exp2_fast(m[mt][e] - mx);
 #pragma unroll
         for (int d = 0; d < DP / 8; ++d) {
           o[mt][d][2 * e] *= f;
           o[mt][d][2 * e + 1] *= f;
         }
+        m[mt][e] = mx;
+        z[mt][e] = zz;
       }
-    for (int w = 0; w < 4; ++w) {
-      if (warp == w) {
+    // two buffers: 2, 3 -> 0, 1, then 1 -> 0; one (where two would cost the second CTA of an SM): 3, 2, 1 -> 0
+#pragma unroll 1
+    for (int step = Sm::kBufs == 2 ? 2 : 3; step; step = Sm::kBufs == 2 ? step / 2 : step - 1) {
+      const int to = warp - step, n = Sm::kBufs == 2 ? step : 1;
+      if (to >= 0 && to < n) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+          for (int d = 0; d < DP / 8; ++d)
+            *reinterpret_cast<float4*>(merge + (((to * MT + mt) * (DP / 8) + d) * 32 + lane) * 4) =
+                make_float4(o[mt][d][0], o[mt][d][1], o[mt][d][2], o[mt][d][3]);
+      }
+      __syncthreads();
+      if (warp < n) {
 #pragma unroll
-            for (int d = 0; d < DP / 8; ++d) {
-              float2* at = reinterpret_cast<float2*>(merge + (mt * 16 + lane / 4 + e * 8) * DP + d * 8 + (lane & 3) * 2);
-              float2 v = w ? *at : make_float2(0.f, 0.f);
-              v.x += o[mt][d][2 * e];
-              v.y += o[mt][d][2 * e + 1];
-              *at = v;
-            }
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d) {
+            const float4 v = *reinterpret_cast<const float4*>(merge + (((warp * MT + mt) * (DP / 8) + d) * 32 + lane) * 4);
+            o[mt][d][0] += v.x;
+            o[mt][d][1] += v.y;
+            o[mt][d][2] += v.z;
+            o[mt][d][3] += v.w;
+          }
       }
       __syncthreads();
     }
-    const bool whole = cw.start == 0 && cw.end == cw.units;
-    const int64_t slot = 2 * (int64_t)blockIdx.x + (cw.start == 0 ? 1 : 0);
-    const int dim = a.c.dim;
-    for (int i = threadIdx.x; i < kRows * (dim / 8); i += 128) {
-      const int row = whole ? i / (dim / 8) : i % kRows, c = whole ? i - row * (dim / 8) : i / kRows;
-      if (row >= rows) continue;
-      float mx = -INFINITY, zz = 0.f;
-      for (int w = 0; w < 4; ++w) mx = fmaxf(mx, ml[w * kRows + row].x);
-      for (int w = 0; w < 4; ++w) {
-        const float2 v = ml[w * kRows + row];
-        if (v.x > -INFINITY) zz += v.y * mma::exp2_fast(v.x - mx);
-      }
-      const float4 v0 = *reinterpret_cast<const float4*>(merge + row * DP + c * 8);
-      const float4 v1 = *reinterpret_cast<const float4*>(merge + row * DP + c * 8 + 4);
-      if (!whole) {
-        float4* po = a.part_o + (slot * (dim / 4) + 2 * c) * kRows + row;
-        po[0] = v0;
-        po[kRows] = v1;
-        if (c == 0) a.part_ml[slot * kRows + row] = make_float2(mx, zz);
-        continue;
-      }
-      const int t = (row0 + row) / a.G, h = cw.h * a.G + row0 + row - t * a.G;
-      const int64_t at = ((int64_t)cw.b * a.T + t) * a.Hkv * a.G + h;
-      const bool used = a.pos[(int64_t)cw.b * a.T + t] >= 0;
-      float sink = a.sinks ? a.sinks[h] * kLog2e : -INFINITY;
-      const float top = fmaxf(mx, sink);
-      const float ref = top == -INFINITY ? 0.f : top;
-      const float f = mx == -INFINITY ? 0.f : mma::exp2_fast(mx - ref);
-      const float den = zz * f + (a.sinks ? mma::exp2_fast(sink - ref) : 0.f);
-      const float g = used && mx > -INFINITY ? f / den : 0.f;
-      uint4 w;
-      w.x = pack_bf16x2(g == 0.f ? 0.f : v0.x * g, g == 0.f ? 0.f : v0.y * g);
-      w.y = pack_bf16x2(g == 0.f ? 0.f : v0.z * g, g == 0.f ? 0.f : v0.w * g);
-      w.z = pack_bf16x2(g == 0.f ? 0.f : v1.x * g, g == 0.f ? 0.f : v1.y * g);
-      w.w = pack_bf16x2(g == 0.f ? 0.f : v1.z * g, g == 0.f ? 0.f : v1.w * g);
-      *reinterpret_cast<uint4*>(a.out + at * dim + c * 8) = w;
-      if (c == 0 && a.lse) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
+    if (warp == 0) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = mt * 16 + lane / 4 + e * 8;
+          if (row >= rows) continue;
+          const float mx = m[mt][e];
+          if (!whole) {
+#pragma unroll
+            for (int d = 0; d < DP / 8; ++d)
+              if (d * 8 < dim)
+                *reinterpret_cast<float2*>(reinterpret_cast<float*>(
+                    a.part_o + (slot * (dim / 4) + 2 * d + ((lane & 3) >> 1)) * kRows + row) + (lane & 1) * 2) =
+                    make_float2(o[mt][d][2 * e], o[mt][d][2 * e + 1]);
+            if ((lane & 3) == 0) a.part_ml[slot * kRows + row] = make_float2(mx, z[mt][e]);
+            continue;
+          }
+          const float top = fmaxf(mx, sink[mt][e]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          const float f = mx == -INFINITY ? 0.f : mma::exp2_fast(mx - ref);
+          const float den = z[mt][e] * f + (a.sinks ? mma::exp2_fast(sink[mt][e] - ref) : 0.f);
+          const float g = used[mt][e] && mx > -INFINITY ? f / den : 0.f;
+#pragma unroll
+          for (int d = 0; d < DP / 8; ++d)
+            if (d * 8 < dim)
+              *reinterpret_cast<uint32_t*>(a.out + at[mt][e] * dim + d * 8 + (lane & 3) * 2) =
+                  g == 0.f ? 0u : pack_bf16x2(o[mt][d][2 * e] * g, o[mt][d][2 * e + 1] * g);
+          if ((lane & 3) == 0 && a.lse) a.lse[at[mt][e]] = used[mt][e] ? ref * kLn2 + logf(den) : -INFINITY;
+        }
     }
-    if (!walk_next<kU>(a, r.p1, cw)) break;
+    if (!walk_next<kU>(a, cw)) break;
     __syncthreads();
   }
   if constexpr (kTma) {
@@ -622,6 +656,7 @@ struct TilesCfg {
 constexpr int kTileThreads = 352;
 constexpr uint32_t kSCol = 128, kOCol = 256;             // pipeline p: S at p * kSCol, O at kOCol + p * 128
 constexpr float kRescale = 8.f;
+constexpr int kPolyOf = 8;  // one pair of exponentials in so many runs on the FMA pipe (none 136 us, 1/8 130, 1/4 132 at 2 x 131072 keys, 16 drafts)
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort));
@@ -722,8 +757,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   auto qfull = [&](int p) { return bar + kB + 64 + 8 * p; };
   auto pvdone = [&](int p) { return bar + kB + 80 + 8 * p; };
   auto drain = [&](int p) { return bar + kB + 96 + 8 * p; };
-  const uint32_t meet = bar + kB + 112;
-  static_assert(kB + 120 <= 320, "barriers");
+  auto odone = [&](int p) { return bar + kB + 112 + 8 * p; };
+  const uint32_t meet = bar + kB + 128;
+  static_assert(kB + 136 <= 320, "barriers");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid < 128) {
@@ -744,7 +780,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       ptx::mbar_init(pready(p, 0), 128);  // one per half: a warp may be a half tile ahead of its group
       ptx::mbar_init(pready(p, 1), 128);
       ptx::mbar_init(qfull(p), 128);
-      ptx::mbar_init(pvdone(p), 1);
+      ptx::mbar_init(pvdone(p), 1);  // each product; only waited for one behind, where its parity is unambiguous
+      ptx::mbar_init(odone(p), 1);   // the last of a piece
       ptx::mbar_init(drain(p), 1);
     }
     ptx::mbar_init(meet, 256);
@@ -760,12 +797,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
 
   if (r.p0 < r.p1) {
     Walk w;
-    walk_begin<kU>(a, r, w);
+    bool more = walk_begin<kU>(a, r, w);
     int base = 0;  // tiles of the pieces before this one
     if (warp == 8) {
       // ------------------------------------------------ loader: lane g fetches the g-th box of a tile
       const int boxes = kU / a.box;
-      int page = 0, row = -1, i = w.start, s = 0;
+      int page = 0, row = -1, i = more ? w.start : 0, s = 0;
       auto find = [&]() {
         row = -1;
         const int slot = w.k.lo + i * kU + lane * a.box;
@@ -775,8 +812,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           page = __ldg(a.c.table + w.b * a.c.table_stride + p);
         }
       };
-      bool more = true;
-      find();
+      if (more) find();
       while (more && ok) {
         if (row >= 0 && (unsigned)page >= (unsigned)a.c.pages) {
           record_status(a.c.status, BS_ERR_CAPACITY);
@@ -785,7 +821,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         // a box behind the last slot lies outside the descriptor's pages: zeros
         const int y = w.h, x = row >= 0 ? page : a.c.pages, z = max(row, 0);
         if (++i == w.end) {
-          more = walk_next<kU>(a, r.p1, w);
+          more = walk_next<kU>(a, w);
           i = w.start;
         }
         if (more) find();  // while the copies below are issued
@@ -824,7 +860,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       constexpr int step = kPair ? 1 : 2;
       const int first = kPair ? 0 : p;
       int halves = 0, pieces = 0;  // half tiles and pieces of this pipeline so far
-      bool more = true;
       while (more && ok) {
         const int n = w.end - w.start, total = first < n ? 2 * ((n - first + step - 1) / step) : 0;
         // S of half tile h of the piece, into half h & 1 of the S columns
@@ -864,6 +899,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
               for (int k = 0; k < 4; ++k)
                 ptx::mma_ts_bf16(o_col, s_col + (h & 1) * 64 + k * 8, vd + k * 128, idesc_o, h > 0 || k > 0);
               ptx::tc_commit(pvdone(p));
+              if (h + 1 == total) ptx::tc_commit(odone(p));
               if (h & 1) ptx::tc_commit(empty(va));
             }
             __syncwarp();
@@ -871,7 +907,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           }
         }
         base += n;
-        more = walk_next<kU>(a, r.p1, w);
+        more = walk_next<kU>(a, w);
       }
       if (!ok && elected) {
         // products in flight end before tensor memory is given back
@@ -889,8 +925,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       float2* ml = reinterpret_cast<float2*>(smem + Cfg::ml);
       constexpr int step = kPair ? 1 : 2;
       const int first = kPair ? 0 : p;
-      int halves = 0, meets = 0;  // half tiles of this pipeline so far
-      bool more = true;
+      int halves = 0, pieces = 0, meets = 0;  // half tiles and pieces of this pipeline so far
       while (more && ok) {
         const int n = w.end - w.start;
         const int row0 = w.tile * kRows + (kPair ? p * 128 : 0);
@@ -916,21 +951,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           for (int c = 0; c < DP / 8; ++c)
             *reinterpret_cast<uint4*>(qs + mma::tile_at<128>(t, c)) = mine && c * 8 < a.c.dim ? v[c] : make_uint4(0, 0, 0, 0);
           ptx::fence_proxy_async_smem();
+          __syncwarp();
           ptx::mbar_arrive(qfull(p));
           const int total = 2 * ((n - first + step - 1) / step);
           int done = halves;
-          for (int h = 0; h < total; ++h, ++done) {
+          float s[64];
+          // S of half tile h, asked for; tmem_wait_ld before it is used
+          auto fetch = [&](int h) {
             ok = warp_wait(sfull(p, h & 1), (done >> 1) & 1, abort);
-            if (!ok) break;
+            if (!ok || !warp_on) return;
             ptx::tc_fence_after();
+            ptx::tmem_ld_32x32b_x32(s_col + (h & 1) * 64, reinterpret_cast<uint32_t*>(s));
+            ptx::tmem_ld_32x32b_x32(s_col + (h & 1) * 64 + 32, reinterpret_cast<uint32_t*>(s + 32));
+          };
+          fetch(0);
+          for (int h = 0; h < total && ok; ++h) {
             const int i = first + (h >> 1) * step;
             const int tile0 = w.k.lo + (w.start + i) * kU, key0 = tile0 + (h & 1) * 64;
-            const uint32_t sp = s_col + (h & 1) * 64;
             if (warp_on) {
               const bool slow = key0 + 64 > w.k.n || a.window || a.scale2 < 0.f;
-              float v[64];
-              ptx::tmem_ld_32x32b_x32(sp, reinterpret_cast<uint32_t*>(v));
-              ptx::tmem_ld_32x32b_x32(sp + 32, reinterpret_cast<uint32_t*>(v + 32));
               ptx::tmem_wait_ld();
               if (slow) {
 #pragma unroll
@@ -938,17 +977,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                   const int k0 = key0 + c * 32;
                   const uint32_t see = bit_range(below + 1 - k0, w.k.n - k0) | bits_from(bits, k0 - w.k.n);
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) v[c * 32 + e] = see >> e & 1 ? v[c * 32 + e] * a.scale2 : -INFINITY;
+                  for (int e = 0; e < 32; ++e) s[c * 32 + e] = see >> e & 1 ? s[c * 32 + e] * a.scale2 : -INFINITY;
                 }
               }
-              float top[4] = {v[0], v[1], v[2], v[3]};
+              float top[22];  // a tree of three-way maxima: few steps that wait for one another
 #pragma unroll
-              for (int e = 4; e < 64; e += 8)
+              for (int e = 0; e < 21; ++e) top[e] = mma::max3(s[3 * e], s[3 * e + 1], s[3 * e + 2]);
+              top[21] = s[63];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) top[x] = e + x + 4 < 64 ? mma::max3(top[x], v[e + x], v[e + x + 4]) : fmaxf(top[x], v[e + x]);
-              float mx = fmaxf(mma::max3(top[0], top[1], top[2]), top[3]);
+              for (int e = 0; e < 7; ++e) top[e] = mma::max3(top[3 * e], top[3 * e + 1], top[3 * e + 2]);
+              top[0] = mma::max3(mma::max3(top[0], top[1], top[2]), mma::max3(top[3], top[4], top[5]), fmaxf(top[6], top[21]));
               const float mul = slow ? 1.f : a.scale2;
-              mx *= mul;
+              const float mx = top[0] * mul;
               const bool move = mx > m + kRescale || (m == -INFINITY && mx > -INFINITY);
               if (__any_sync(0xffffffffu, move)) {
                 const float f = move ? mma::exp2_fast(m - mx) : 1.f;  // 0 from -inf
@@ -957,6 +997,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                   m = mx;
                 }
                 if (h > 0) {
+                  // after the product before this one: S of this half came after the one before that,
+                  // so the parity is not mistaken for an older one's
                   ok = warp_wait(pvdone(p), (done - 1) & 1, abort);
                   if (!ok) break;
                   ptx::tc_fence_after();
@@ -973,21 +1015,26 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                 }
               }
               const float ref = m == -INFINITY ? 0.f : m;
-              float2 sum = make_float2(0.f, 0.f);
+              float2 sum[4] = {};
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                  float2 x = mma::fma2(make_float2(v[c * 32 + 2 * e], v[c * 32 + 2 * e + 1]), mul, -ref);
-                  x.x = mma::exp2_fast(x.x);
-                  x.y = mma::exp2_fast(x.y);
-                  sum = mma::add2(sum, x);
+                  float2 x = mma::fma2(make_float2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), mul, -ref);
+                  if (e % kPolyOf == kPolyOf - 1) {
+                    x = mma::exp2_poly(x);
+                  } else {
+                    x.x = mma::exp2_fast(x.x);
+                    x.y = mma::exp2_fast(x.y);
+                  }
+                  sum[e & 3] = mma::add2(sum[e & 3], x);
                   pk[e] = pack_bf16x2(x.x, x.y);
                 }
-                ptx::tmem_st_32x32b_x16(sp + c * 16, pk);
+                ptx::tmem_st_32x32b_x16(s_col + (h & 1) * 64 + c * 16, pk);
               }
-              z += sum.x + sum.y;
+              sum[0] = mma::add2(mma::add2(sum[0], sum[1]), mma::add2(sum[2], sum[3]));
+              z += sum[0].x + sum[0].y;
             }
             if (!(h & 1) && (tile0 < w.k.low || tile0 + kU > w.k.n)) {
               // the tile's boxes bring all their slots: those that hold no key become zeros in V
@@ -1001,7 +1048,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                   *reinterpret_cast<uint4*>(row + (c >> 3) * 16384 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
               }
               ptx::fence_proxy_async_smem();
+              __syncwarp();
             }
+            ++done;
+            if (h + 1 < total) fetch(h + 1);  // its latency and that of the stores pass together
+            if (!ok) break;
             if (warp_on) ptx::tmem_wait_st();
             ptx::tc_fence_before();
             ptx::mbar_arrive(pready(p, h & 1));
@@ -1011,8 +1062,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         // ---- end of the piece: read the accumulators
         if (first < n) {
           halves += 2 * ((n - first + step - 1) / step);
-          // the last but one first: a parity alone does not tell the last from the one two before
-          ok = warp_wait(pvdone(p), halves & 1, abort) && warp_wait(pvdone(p), (halves - 1) & 1, abort);
+          ok = warp_wait(odone(p), pieces & 1, abort);
+          ++pieces;
         }
         if (!ok) break;
         ptx::tc_fence_after();
@@ -1032,7 +1083,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           f1 = m1.x == -INFINITY ? 0.f : mma::exp2_fast(m1.x - m);
           z = m0.y * f0 + m1.y * f1;
         }
-        const bool whole = w.start == 0 && w.end == w.units;
+        const bool whole = w.whole();
         const int64_t slot = 2 * (int64_t)blockIdx.x + (w.start == 0 ? 1 : 0);
         const int dim = a.c.dim, row = (kPair ? p * 128 : 0) + t;
         const int64_t at = ((int64_t)w.b * a.T + tok) * a.Hkv * a.G + hq;
@@ -1105,7 +1156,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           ++meets;
         }
         base += n;
-        more = walk_next<kU>(a, r.p1, w);
+        more = walk_next<kU>(a, w);
       }
     }
   }
@@ -1125,15 +1176,14 @@ constexpr int kJoinRows = 8;
 template <int kU, int kRows>
 __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ TreeArgs a, int grid) {
   __shared__ int64_t sums[8];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int per = a.Hkv * a.tiles;
   const int b = blockIdx.x / per, item = blockIdx.x - b * per;
   const int h = item / a.tiles, tile = item - h * a.tiles;
-  // units before this sequence, and in all
+  // units before this sequence, and in all (the lengths are inputs of the first
+  // launch too, so nothing of this waits for it)
   int64_t before = 0, total = 0;
   for (int i = threadIdx.x; i < a.B; i += 128) {
-    const Keys k = keys_of(a, i);
-    const int64_t w = (int64_t)((k.hi - k.lo + kU - 1) / kU) * per;
+    const int64_t w = units_of<kU>(a, i) * per;
     total += w;
     if (i < b) before += w;
   }
@@ -1146,25 +1196,26 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
   __syncthreads();
   before = sums[0] + sums[1] + sums[2] + sums[3];
   total = sums[4] + sums[5] + sums[6] + sums[7];
-  const Keys k = keys_of(a, b);
-  const int64_t units = (k.hi - k.lo + kU - 1) / kU;
+  const int64_t units = units_of<kU>(a, b);
   const int64_t chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
   const int64_t s = before + item * units, e = s + units;
-  const int c0 = (int)(s / chunk), c1 = (int)((e - 1) / chunk);
+  const int c0 = (int)((s + a.setup) / chunk), c1 = (int)((e - 1) / chunk);
   if (c0 == c1) return;
   const int dim = a.c.dim, row0 = tile * kRows, rows = min(kRows, a.R - row0);
   const int first = blockIdx.y * kJoinRows, last = min(rows, first + kJoinRows);
-  for (int i = threadIdx.x; i < kJoinRows * (dim / 4); i += 128) {
-    const int row = first + i % kJoinRows, c = i / kJoinRows;
-    if (row >= last) continue;
-    float mx = -INFINITY;
+  const int row = first + threadIdx.x % kJoinRows;  // each thread: one row, every 16th group of four columns
+  if (row >= last) return;
+  const int t = (row0 + row) / a.G, hq = h * a.G + row0 + row - t * a.G;
+  const bool used = a.pos[(int64_t)b * a.T + t] >= 0;
+  const float sink = a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float mx = -INFINITY;
 #pragma unroll 4
-    for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, a.part_ml[(2 * (int64_t)x + (x == c0)) * kRows + row].x);
-    const int t = (row0 + row) / a.G, hq = h * a.G + row0 + row - t * a.G;
-    const bool used = a.pos[(int64_t)b * a.T + t] >= 0;
-    const float sink = a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
-    const float top = fmaxf(mx, sink);
-    const float ref = top == -INFINITY ? 0.f : top;
+  for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, a.part_ml[(2 * (int64_t)x + (x == c0)) * kRows + row].x);
+  const float top = fmaxf(mx, sink);
+  const float ref = top == -INFINITY ? 0.f : top;
+  const int64_t at = ((int64_t)b * a.T + t) * a.Hkv * a.G + hq;
+  for (int c = threadIdx.x / kJoinRows; c < dim / 4; c += 128 / kJoinRows) {
     float den = a.sinks ? mma::exp2_fast(sink - ref) : 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
@@ -1179,10 +1230,8 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
       v.z += p.z * f;
       v.w += p.w * f;
     }
-    const int64_t at = ((int64_t)b * a.T + t) * a.Hkv * a.G + hq;
-    const bool any = used && mx > -INFINITY;
     uint2 w = make_uint2(0u, 0u);
-    if (any) w = make_uint2(pack_bf16x2(v.x / den, v.y / den), pack_bf16x2(v.z / den, v.w / den));
+    if (used && mx > -INFINITY) w = make_uint2(pack_bf16x2(v.x / den, v.y / den), pack_bf16x2(v.z / den, v.w / den));
     *reinterpret_cast<uint2*>(a.out + at * dim + c * 4) = w;
     if (c == 0 && a.lse) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
   }
@@ -1306,6 +1355,7 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.part_o = static_cast<float4*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * (D / 4));
   a.min_chunk = rows <= 32 ? 4 : 2;
+  a.setup = rows <= 32 ? 8 : 3;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   CacheMaps maps = {};

@@ -95,14 +95,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 // a * b + c and a + b on two values at once.
-__device__ __forceinline__ float2 fma2(float2 a, float b, float c) {
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float c) {
   float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %4};\n\tmov.b64 z, {%5, %5};\n\t"
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %6};\n\t"
       "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b), "f"(c));
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c));
   return r;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float b, float c) { return fma2(a, make_float2(b, b), c); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;
   asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
@@ -110,6 +111,25 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "=f"(r.x), "=f"(r.y)
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
+}
+// 2^x on the FMA pipe, for x in [-126, 126] (smaller x give 2^-126): x = n + f
+// with n the nearest integer, a quartic for 2^f on [-1/2, 1/2] fitted here to the
+// least largest relative error (2.6e-6), and n added to the exponent.  The
+// special-function unit gives 16 exponentials per clock and SM; a share of them
+// computed here shortens a softmax step, and the weights are rounded to bf16.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+  x.x = fmaxf(x.x, -126.f);
+  x.y = fmaxf(x.y, -126.f);
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are n
+  const float2 t = add2(x, make_float2(kRound, kRound));
+  const float2 n = add2(t, make_float2(-kRound, -kRound));
+  const float2 f = add2(x, make_float2(-n.x, -n.y));
+  float2 y = fma2(f, make_float2(0.009570102207362652f, 0.009570102207362652f), 0.05591785907745361f);
+  y = fma2(y, f, 0.240247443318367f);
+  y = fma2(y, f, 0.6931217908859253f);
+  y = fma2(y, f, 0.9999992847442627f);
+  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(y.x)),
+                     __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(y.y)));
 }
 // 16-byte asynchronous copy; zero bytes are read and zeros written when !on.
 __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool on) {

@@ -425,39 +425,70 @@ def mxfp4_matmul_backward(grad_out: torch.Tensor, blocks: torch.Tensor, scales: 
 
 
 # ---------------------------------------------------------------- attention half of the decoder layer
+# These run at every layer of a decoding step, where the host's time counts:
+# arguments are passed as plain integers (the signatures convert them), and the
+# device context is entered only when another device is current.
+def _ptr(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(name: str, index: int, *args) -> None:
+    """``_lib.call`` on the current stream of device ``index`` (appended to the arguments)."""
+    if torch.cuda.current_device() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _device_index(name: str, first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """Index of the CUDA device that all the tensors are on."""
+    index = first.get_device()
+    if index < 0:
+        raise ValueError(f"{name}: blockstreamer_b200 runs on CUDA tensors only (got {first.device})")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name}: tensors on {first.device} and {t.device}; blockstreamer_b200 runs on CUDA "
+                             "tensors only, of one device")
+    return index
+
+
 def _heads(name: str, t: torch.Tensor | None):
     """bs_heads of a [B, T, heads, D] or [T, heads, D] tensor (views are fine, D contiguous)."""
     if t is None:
-        return _lib.Heads(None, 0, 0, 0)
+        return _NO_HEADS
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] > 1:
         raise ValueError(f"{name}: the last dimension must be contiguous")
     return _lib.Heads(t.data_ptr(), st[0] if len(st) == 4 else 0, st[-3], st[-2])
 
 
+_NO_HEADS = _lib.Heads(None, 0, 0, 0)
+
+
 def _kv_cache(name: str, k_cache: torch.Tensor, v_cache: torch.Tensor | None, page_table: torch.Tensor,
               cache_lens: torch.Tensor):
-    if k_cache.dim() != 4 or (v_cache is not None and v_cache.shape != k_cache.shape):
+    shape, v = k_cache.shape, k_cache if v_cache is None else v_cache
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError(f"{name}: the caches must be [pages, page_size, heads, D] of one shape")
-    v = k_cache if v_cache is None else v_cache
     if k_cache.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
         raise ValueError(f"{name}: the caches must be bf16")
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or (page_table.shape[1] > 1
-                                                                    and page_table.stride(1) != 1):
+    table, rows = page_table.shape, page_table.stride()
+    if len(table) != 2 or page_table.dtype != torch.int32 or (table[1] > 1 and rows[1] != 1):
         raise ValueError(f"{name}: page_table must be int32 [B, pages of a sequence] with contiguous rows")
-    B = page_table.shape[0]
+    B = table[0]
     if cache_lens.shape != (B,) or cache_lens.dtype != torch.int32 or not cache_lens.is_contiguous():
         raise ValueError(f"{name}: cache_lens must be contiguous int32 [{B}]")
-    P, S, H, D = k_cache.shape
-    ks, vs = k_cache.stride(), v.stride()
-    if D > 1 and (ks[3] != 1 or vs[3] != 1):
+    kp, ks, kh, kd = k_cache.stride()
+    vp, vs, vh, vd = v.stride()
+    if shape[3] > 1 and (kd != 1 or vd != 1):
         raise ValueError(f"{name}: the caches' last dimension must be contiguous")
-    return _lib.KVCache(k_cache.data_ptr(), v.data_ptr(), P, S, H, D, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                        page_table.data_ptr(), page_table.shape[1], page_table.stride(0), cache_lens.data_ptr(), B)
+    return _lib.KVCache(k_cache.data_ptr(), v.data_ptr(), *shape, kp, ks, kh, vp, vs, vh, page_table.data_ptr(),
+                        table[1], rows[0], cache_lens.data_ptr(), B)
 
 
 def _positions(name: str, positions: torch.Tensor, shape, dtypes=(torch.int32, torch.int64)) -> torch.Tensor:
-    if tuple(positions.shape) != tuple(shape) or positions.dtype not in dtypes:
+    if positions.shape != shape or positions.dtype not in dtypes:
         raise ValueError(f"{name}: positions must be {' or '.join(str(d) for d in dtypes)} {tuple(shape)}, got "
                          f"{positions.dtype} {tuple(positions.shape)}")
     return _contig(f"{name}: positions", positions)
@@ -481,7 +512,7 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions
     without its last two dimensions; a negative one gives zeros.  ``inverse``
     turns back, which is the gradient.  Returns (q', k') contiguous (k' None
     without k)."""
-    _cuda("rope", q, k, table, positions)
+    index = _device_index("rope", q, k, table, positions)
     if q.dim() not in (3, 4) or (k is not None and (k.dim() != q.dim() or k.shape[:-2] != q.shape[:-2]
                                                     or k.shape[-1] != q.shape[-1] or k.dtype != q.dtype)):
         raise ValueError("rope: q and k must be [B, T, heads, D] or [T, heads, D], alike but for the heads")
@@ -491,12 +522,11 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions
     rot = _rope_table("rope", table, D)
     positions = _positions("rope", positions, q.shape[:-2])
     B, T = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = None if k is None else torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    with torch.cuda.device(q.device):
-        _lib.call("bs_rope", _heads("rope", q), _heads("rope", k), _heads("rope", qo), _heads("rope", ko),
-                  _DT[q.dtype], B, T, q.shape[-2], 0 if k is None else k.shape[-2], D, _p(table), table.shape[0],
-                  rot, _p(positions), _DT[positions.dtype], int(interleaved), int(inverse), _stream(q))
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ko = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
+    _launch("bs_rope", index, _heads("rope", q), _heads("rope", k), _heads("rope", qo), _heads("rope", ko),
+            _DT[q.dtype], B, T, q.shape[-2], 0 if k is None else k.shape[-2], D, _ptr(table), table.shape[0], rot,
+            _ptr(positions), _DT[positions.dtype], interleaved, inverse)
     return qo, ko
 
 
@@ -506,7 +536,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.
     """The serving form of ``rope`` (bs_rope_append): returns the turned q
     [B, T, Hq, D] and writes the turned k and v [B, T, Hkv, D] into the cache at
     slots cache_lens[b] + t.  Rows of negative position write nothing."""
-    _cuda("rope_append", q, k, v, table, positions, k_cache, v_cache, page_table, cache_lens)
+    index = _device_index("rope_append", q, k, v, table, positions, k_cache, v_cache, page_table, cache_lens)
     cache = _kv_cache("rope_append", k_cache, v_cache, page_table, cache_lens)
     if q.dim() != 4 or q.dtype != torch.bfloat16 or k.dtype != q.dtype or v.dtype != q.dtype:
         raise ValueError("rope_append: q, k and v must be bf16 [B, T, heads, D]")
@@ -516,11 +546,10 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.
                          f"cache of {cache.batch} sequences, {cache.heads} heads of {cache.dim}")
     rot = _rope_table("rope_append", table, D)
     positions = _positions("rope_append", positions, (B, T))
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.call("bs_rope_append", _heads("rope_append", q), _heads("rope_append", k), _heads("rope_append", v),
-                  _heads("rope_append", qo), cache, T, Hq, _p(table), table.shape[0], rot, _p(positions),
-                  _DT[positions.dtype], int(interleaved), _stream(q))
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+    _launch("bs_rope_append", index, _heads("rope_append", q), _heads("rope_append", k), _heads("rope_append", v),
+            _heads("rope_append", qo), cache, T, Hq, _ptr(table), table.shape[0], rot, _ptr(positions),
+            _DT[positions.dtype], interleaved)
     return qo
 
 
@@ -535,7 +564,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     attends, itself included (None: a chain); ``sinks`` [Hq] f32; ``window`` 0
     for none; ``scale`` defaults to D**-0.5.  Returns (out [B, T, Hq, D] bf16,
     lse [B, T, Hq] f32)."""
-    _cuda("tree_attention", q, k_cache, v_cache, page_table, cache_lens, positions, tree_mask, sinks)
+    index = _device_index("tree_attention", q, k_cache, v_cache, page_table, cache_lens, positions, tree_mask, sinks)
     cache = _kv_cache("tree_attention", k_cache, v_cache, page_table, cache_lens)
     if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != cache.batch or q.shape[3] != cache.dim:
         raise ValueError(f"tree_attention: q must be bf16 [{cache.batch}, T, Hq, {cache.dim}], got {q.dtype} "
@@ -552,14 +581,13 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
             raise ValueError("tree_attention: every sequence's tree_mask must be contiguous")
     if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (Hq,) or not sinks.is_contiguous()):
         raise ValueError(f"tree_attention: sinks must be contiguous f32 [{Hq}]")
-    out = torch.empty((B, T, Hq, D), dtype=q.dtype, device=q.device)
-    lse = torch.empty((B, T, Hq), dtype=torch.float32, device=q.device)
-    ws_bytes = _lib.load().bs_tree_attention_workspace_bytes(B, T, Hq, cache.heads, D)
-    ws = torch.empty(max(ws_bytes, 16), dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.call("bs_tree_attention", _heads("tree_attention", q), cache, T, Hq, _p(positions), _p(tree_mask),
-                  mask_stride, _p(sinks), window, D ** -0.5 if scale is None else scale, _p(out), _p(lse), _p(ws),
-                  ws_bytes, _stream(q))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = q.new_empty((B, T, Hq), dtype=torch.float32)
+    ws_bytes = (_lib._lib or _lib.load()).bs_tree_attention_workspace_bytes(B, T, Hq, cache.heads, D)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8)
+    _launch("bs_tree_attention", index, _heads("tree_attention", q), cache, T, Hq, _ptr(positions), _ptr(tree_mask),
+            mask_stride, _ptr(sinks), window, D ** -0.5 if scale is None else scale, _ptr(out), _ptr(lse), _ptr(ws),
+            ws_bytes)
     return out, lse
 
 
@@ -569,13 +597,12 @@ def tree_commit(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.
     accepted[b, i] to cache_lens[b] + i (bs_tree_commit).  ``accepted`` [B, A]
     int32 holds ascending draft indices, then negative ones; ``drafted`` is the
     step's T.  cache_lens is left for the caller to advance."""
-    _cuda("tree_commit", k_cache, v_cache, page_table, cache_lens, accepted)
+    index = _device_index("tree_commit", k_cache, v_cache, page_table, cache_lens, accepted)
     cache = _kv_cache("tree_commit", k_cache, v_cache, page_table, cache_lens)
     if accepted.dim() != 2 or accepted.dtype != torch.int32 or accepted.shape[0] != cache.batch:
         raise ValueError(f"tree_commit: accepted must be int32 [{cache.batch}, A]")
     accepted = _contig("tree_commit: accepted", accepted)
-    with torch.cuda.device(k_cache.device):
-        _lib.call("bs_tree_commit", cache, drafted, _p(accepted), accepted.shape[1], _stream(k_cache))
+    _launch("bs_tree_commit", index, cache, drafted, _ptr(accepted), accepted.shape[1])
 
 
 def kv_scores_add(scores: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, k_cache: torch.Tensor,
@@ -587,7 +614,7 @@ def kv_scores_add(scores: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, k_ca
     cache_lens[b] + i and attended every slot up to its own.  q and ``lse`` are
     those of ``tree_attention``; entries of ``accepted`` [B, A] int32 outside
     [0, T) are skipped.  ``out`` may be ``scores``."""
-    _cuda("kv_scores_add", scores, q, lse, k_cache, page_table, cache_lens, accepted, out)
+    index = _device_index("kv_scores_add", scores, q, lse, k_cache, page_table, cache_lens, accepted, out)
     cache = _kv_cache("kv_scores_add", k_cache, None, page_table, cache_lens)
     if q.dim() != 4 or q.dtype != torch.bfloat16 or q.shape[0] != cache.batch or q.shape[3] != cache.dim:
         raise ValueError(f"kv_scores_add: q must be bf16 [{cache.batch}, T, Hq, {cache.dim}], got {q.dtype} "
@@ -606,10 +633,9 @@ def kv_scores_add(scores: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, k_ca
         out = torch.empty_like(scores)
     elif out.shape != scores.shape or out.dtype != scores.dtype or not out.is_contiguous():
         raise ValueError("kv_scores_add: out must be contiguous and of the shape of scores")
-    with torch.cuda.device(q.device):
-        _lib.call("bs_kv_scores_add", _heads("kv_scores_add", q), cache, T, Hq, _p(lse), _p(accepted),
-                  T if accepted is None else accepted.shape[1], D ** -0.5 if scale is None else scale, _p(scores),
-                  _p(out), scores.shape[2], _stream(q))
+    _launch("bs_kv_scores_add", index, _heads("kv_scores_add", q), cache, T, Hq, _ptr(lse), _ptr(accepted),
+            T if accepted is None else accepted.shape[1], D ** -0.5 if scale is None else scale, _ptr(scores),
+            _ptr(out), scores.shape[2])
     return out
 
 
@@ -622,7 +648,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Ten
     ``out_page_table`` [B, width].  Returns (kept [B, Hkv, budget] int32 slots
     then -1, new lengths [B] int32, scores of the new slots [B, Hkv, width *
     page_size] f32)."""
-    _cuda("kv_evict", k_cache, v_cache, page_table, cache_lens, scores, out_page_table)
+    index = _device_index("kv_evict", k_cache, v_cache, page_table, cache_lens, scores, out_page_table)
     cache = _kv_cache("kv_evict", k_cache, v_cache, page_table, cache_lens)
     B, Hkv = cache.batch, cache.heads
     if scores.dtype != torch.float32 or scores.dim() != 3 or tuple(scores.shape[:2]) != (B, Hkv):
@@ -631,11 +657,10 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Ten
         raise ValueError(f"kv_evict: out_page_table must be int32 [{B}, width]")
     scores = _contig("kv_evict: scores", scores)
     out_page_table = _contig("kv_evict: out_page_table", out_page_table)
-    dev, width = k_cache.device, out_page_table.shape[1]
-    kept = torch.empty((B, Hkv, max(budget, 0)), dtype=torch.int32, device=dev)
-    lens = torch.empty((B,), dtype=torch.int32, device=dev)
-    new = torch.empty((B, Hkv, width * cache.page_size), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        _lib.call("bs_kv_evict", cache, _p(scores), scores.shape[2], budget, keep_first, keep_last,
-                  _p(out_page_table), width, _p(kept), _p(lens), _p(new), _stream(k_cache))
+    width = out_page_table.shape[1]
+    kept = page_table.new_empty((B, Hkv, max(budget, 0)))
+    lens = torch.empty_like(cache_lens)
+    new = scores.new_empty((B, Hkv, width * cache.page_size))
+    _launch("bs_kv_evict", index, cache, _ptr(scores), scores.shape[2], budget, keep_first, keep_last,
+            _ptr(out_page_table), width, _ptr(kept), _ptr(lens), _ptr(new))
     return kept, lens, new
