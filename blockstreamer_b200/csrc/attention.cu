@@ -653,7 +653,10 @@ struct TilesCfg {
   static constexpr int bars = ml + 2 * 128 * 8;
   static constexpr int total = bars + 320 + 1024;        // barriers; alignment of the base
 };
-constexpr int kTileThreads = 352;
+constexpr int kTileThreads = 384;
+// Registers of a thread: 168 at launch; the softmax warps' rows of S want more, and
+// the other four warps give it (256 * 200 + 128 * 104 = 384 * 168).
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr uint32_t kSCol = 128, kOCol = 256;             // pipeline p: S at p * kSCol, O at kOCol + p * 128
 constexpr float kRescale = 8.f;
 constexpr int kPolyOf = 8;  // one pair of exponentials in so many runs on the FMA pipe (none 136 us, 1/8 130, 1/4 132 at 2 x 131072 keys, 16 drafts)
@@ -796,11 +799,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   bool ok = true;
 
   if (r.p0 < r.p1) {
-    Walk w;
-    bool more = walk_begin<kU>(a, r, w);
     int base = 0;  // tiles of the pieces before this one
     if (warp == 8) {
       // ------------------------------------------------ loader: lane g fetches the g-th box of a tile
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      Walk w;
+      bool more = walk_begin<kU>(a, r, w);
       const int boxes = kU / a.box;
       int page = 0, row = -1, i = more ? w.start : 0, s = 0;
       auto find = [&]() {
@@ -844,11 +848,14 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         volatile int gone = 0;
         for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
       }
-    } else if (warp >= 9) {
+    } else if (warp == 9 || warp == 10) {
       // ------------------------------------------------ MMA issue, one warp per pipeline
       // The whole warp walks the loops and one elected thread issues: descriptors
       // then stay in uniform registers (in a one-thread branch each product costs
       // several moves to them, ~115 cycles).
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      Walk w;
+      bool more = walk_begin<kU>(a, r, w);
       const int p = warp - 9;
       const bool elected = ptx::elect_one();
       constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
@@ -916,8 +923,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         ptx::mbar_wait(drain(p), 0, &gone);
       }
       __syncwarp();
-    } else {
+    } else if (warp < 8) {
       // ------------------------------------------------ softmax, a thread per row
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+      Walk w;
+      bool more = walk_begin<kU>(a, r, w);
       const int p = warp >> 2, t = tid & 127;
       const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // lane offset in a tensor-memory address
       const uint32_t s_col = tmem + lanes + p * kSCol;
@@ -1158,6 +1168,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         base += n;
         more = walk_next<kU>(a, w);
       }
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     }
   }
   __syncwarp();
