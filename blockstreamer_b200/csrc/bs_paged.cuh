@@ -62,6 +62,149 @@ struct CacheMaps {
 int cache_box_rows(const bs_kv_cache* c, int most);
 int cache_maps(const bs_kv_cache* c, int rows, bool need_v, CacheMaps* out);
 
+// What the split of a call's keys over CTAs goes by: items are (sequence, kv
+// head, row tile), in that order.
+struct SplitArgs {
+  PagedCache c;
+  const int32_t* pos;    // positions of the drafted tokens [B, T] (attention only)
+  int B, Hkv, tiles;
+  int T;                 // slots behind the committed ones
+  int window;
+  int box;               // slots of a TMA box, or 1
+  int setup;             // what starting an item costs, in units: it is counted as so many more
+  int min_chunk;         // units of a CTA at least
+};
+
+// The keys of a sequence: n committed; slots [low, hi) may be attended; units
+// start at lo, low rounded down to where a TMA box may start.
+struct Keys {
+  int n, low, lo, hi;
+};
+__device__ __forceinline__ Keys keys_of(const SplitArgs& a, int b) {
+  Keys k;
+  k.n = a.c.len(b, a.T);
+  k.hi = k.n + a.T;
+  k.low = a.window ? max(0, k.n - a.window + 1) : 0;
+  k.lo = k.low & -a.box;
+  return k;
+}
+// Whether a slot holds a key that some row may attend (others may hold anything).
+__device__ __forceinline__ bool holds_key(const SplitArgs& a, int b, const Keys& k, int slot) {
+  return slot >= k.low && (slot < k.n || (slot < k.hi && __ldg(a.pos + (int64_t)b * a.T + slot - k.n) >= 0));
+}
+
+// Where the work of CTA `cta` of `grid` lies: its range [p0, p1) of the units of
+// all items, item by item, and the sequence that holds unit p0.  An item has
+// `setup` units that stand for its start (Q, masks, epilogue), then one for each
+// kU keys.  The CTA's first 128 threads call.
+struct Range {
+  int64_t p0, p1, chunk;
+  int b;           // sequence of unit p0
+  int64_t before;  // units of the sequences before b
+};
+template <int kU>
+__device__ __forceinline__ int64_t units_of(const SplitArgs& a, int b) {
+  const Keys k = keys_of(a, b);
+  return a.setup + (k.hi - k.lo + kU - 1) / kU;
+}
+__device__ __forceinline__ void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+template <int kU>
+__device__ Range locate(const SplitArgs& a, int cta, int grid, int64_t* sums /* smem [6] */) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t per = (int64_t)a.Hkv * a.tiles;
+  Range r = {};
+  int64_t total = 0;
+  if (a.B > 128) {
+    for (int b = threadIdx.x; b < a.B; b += 128) total += units_of<kU>(a, b) * per;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    if (lane == 0) sums[warp] = total;
+    sync128();
+    total = sums[0] + sums[1] + sums[2] + sums[3];
+  }
+  // a scan of the sequences' units, 128 at a time (one step gives the total too)
+  int64_t run = 0;
+  for (int base = 0; base < a.B; base += 128) {
+    const int b = base + threadIdx.x;
+    const int64_t w = b < a.B ? units_of<kU>(a, b) * per : 0;
+    int64_t incl = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
+    }
+    sync128();
+    if (lane == 31) sums[warp] = incl;
+    sync128();
+    int64_t start = run + incl - w;
+    for (int i = 0; i < warp; ++i) start += sums[i];
+    run += sums[0] + sums[1] + sums[2] + sums[3];
+    if (base == 0) {
+      if (a.B <= 128) total = run;
+      r.chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
+      r.p0 = min(total, cta * r.chunk);
+      r.p1 = min(total, r.p0 + r.chunk);
+      if (r.p0 >= r.p1) return r;
+    }
+    if (w > 0 && start <= r.p0 && r.p0 < start + w) sums[4] = b, sums[5] = start;
+    if (run > r.p0) break;
+  }
+  sync128();
+  r.b = (int)sums[4];
+  r.before = sums[5];
+  return r;
+}
+
+// The pieces of a CTA's range, one per item that it touches; pieces without keys
+// are passed over.
+struct Walk {
+  int b, h, tile;
+  Keys k;
+  int u;               // the caller's next unit
+  int start, end;      // units of keys of this piece
+  int units;           // units of keys of the item
+  int len;             // of the piece, with the units that stand for the start
+  int64_t left;        // of the range, this piece included
+  __device__ __forceinline__ bool whole() const { return start == 0 && end == units; }
+};
+template <int kU>
+__device__ __forceinline__ bool walk_piece(const SplitArgs& a, Walk& w, int first) {
+  w.units = (w.k.hi - w.k.lo + kU - 1) / kU;
+  w.len = (int)min((int64_t)(w.units + a.setup - first), w.left);
+  w.start = max(0, first - a.setup);
+  w.end = max(0, first + w.len - a.setup);
+  return w.end > w.start;
+}
+// The next piece of the range; false at its end.
+template <int kU>
+__device__ __forceinline__ bool walk_next(const SplitArgs& a, Walk& w) {
+  while (true) {
+    w.left -= w.len;
+    if (w.left <= 0) return false;
+    if (++w.tile == a.tiles) {
+      w.tile = 0;
+      if (++w.h == a.Hkv) {
+        w.h = 0;
+        ++w.b;
+        w.k = keys_of(a, w.b);
+      }
+    }
+    if (walk_piece<kU>(a, w, 0)) return true;
+  }
+}
+template <int kU>
+__device__ __forceinline__ bool walk_begin(const SplitArgs& a, const Range& r, Walk& w) {
+  w.b = r.b;
+  w.k = keys_of(a, r.b);
+  const int64_t units = a.setup + (w.k.hi - w.k.lo + kU - 1) / kU;
+  const int64_t rel = r.p0 - r.before;
+  const int item = (int)(rel / units);
+  w.h = item / a.tiles;
+  w.tile = item - w.h * a.tiles;
+  w.left = r.p1 - r.p0;
+  return walk_piece<kU>(a, w, (int)(rel - item * units)) || walk_next<kU>(a, w);
+}
+
 namespace mma {
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t r[4]) {

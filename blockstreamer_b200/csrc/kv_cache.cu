@@ -46,13 +46,13 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
 }
 
 // ---------------------------------------------------------------- scores
-// One CTA per kKeys slots of a (sequence, kv head).  K is the 16-row operand of
-// the tensor-core product, the accepted rows its columns, so that a key's sum
-// over the rows stays in one lane group; no atomics, one store per slot.
-// HBM-bound: 2 dim + 8 bytes per slot and kv head.  All K of the CTA is asked for
-// at once (TMA boxes where pages allow, else 16-byte copies), then the queries.
-struct ScoreArgs {
-  PagedCache c;
+// K is the 16-row operand of the tensor-core product and the accepted rows its
+// columns, so that a key's sum over the rows stays in one lane group: no atomics,
+// one store per slot.  HBM-bound: 2 dim + 8 bytes per slot and kv head.  The
+// slots of all (sequence, kv head) items are cut into equal ranges, one per CTA;
+// each warp streams its own units of 32 or 64 keys through its own ring (TMA boxes where
+// the pages allow, else 16-byte copies), the rows' queries are in shared memory.
+struct ScoreArgs : SplitArgs {  // T: accepted entries; slots lens + i belong to them
   const __nv_bfloat16* q;
   int64_t qb, qt, qh;
   const float* lse;
@@ -60,191 +60,255 @@ struct ScoreArgs {
   const float* scores;
   float* out;
   float scale2;
-  int T, A, i0, rows, G, Hq, capacity, box;  // accepted entries i0 .. i0 + rows / G
+  int tokens, i0, rows, G, Hq, capacity;  // this launch: accepted entries i0 .. i0 + rows / G
 };
 
 template <int DP>
 struct ScoreCfg {
-  static constexpr int kUnits = DP == 64 ? 4 : 2;   // units of 32 keys per warp
-  static constexpr int kKeys = 4 * 32 * kUnits;
-  static constexpr int kTile = 32 * DP * 2;
-  static constexpr int q = 4 * kUnits * kTile;      // then [rows] q, [rows] float2, barriers
-  static int smem(int rows) { return q + rows * (DP * 2 + 8) + 4 * kUnits * 8 + 1024; }
+  static constexpr int kU = DP == 64 ? 64 : 32;
+  static constexpr int kStages = 3;
+  static constexpr int kTile = kU * DP * 2;
+  static constexpr int kWarpBytes = kTile * kStages;
+  static constexpr int bars = 4 * kWarpBytes;            // [4 warps][kStages]
+  static constexpr int sums = bars + 4 * kStages * 8;
+  static constexpr int q = (sums + 64 + 127) / 128 * 128;  // [rows] q, [rows] float2
+  static int smem(int rows) { return q + rows * (DP * 2 + 8) + 1024; }
 };
 
 template <int DP, bool kTma>
 __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ ScoreArgs a,
                                                         const __grid_constant__ CacheMaps maps) {
   using Cfg = ScoreCfg<DP>;
-  constexpr int KS = DP / 16, kLanesRow = DP / 8, kUnits = Cfg::kUnits;
+  constexpr int kU = Cfg::kU, KS = DP / 16, MT = kU / 16, kMine = kU / 32;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   __shared__ int abort_flag;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.y / a.c.heads, h = blockIdx.y - b * a.c.heads;
-  const int n = a.c.len(b, a.A);
   const int rows8 = (a.rows + 7) / 8 * 8;
-  const uint32_t kbase = ptx::smem_addr(smem) + warp * kUnits * Cfg::kTile;
+  const uint32_t base = ptx::smem_addr(smem) + warp * Cfg::kWarpBytes;
+  const uint32_t bar = ptx::smem_addr(smem) + Cfg::bars + warp * Cfg::kStages * 8;
   uint8_t* qs = smem + Cfg::q;
   float2* info = reinterpret_cast<float2*>(qs + rows8 * DP * 2);  // (lse log2(e), last slot seen)
-  const uint32_t bar = ptx::smem_addr(info + rows8) + warp * kUnits * 8;
-  const int first = blockIdx.x * Cfg::kKeys + warp * 32 * kUnits;
-  const int top = min(a.capacity, n + a.A);
   auto qat = [&](int r, int c) { return (uint32_t)((c >> 3) * (rows8 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)); };
 
-  // the scores to add to: slot of lane in each unit
-  const int mine = lane / 4 + (lane & 3) * 8;
-  const int64_t base = (int64_t)blockIdx.y * a.capacity;
-  float before[kUnits];
-#pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int slot = first + u * 32 + mine;
-    before[u] = slot < a.capacity ? a.scores[base + slot] : 0.f;
-  }
-  if (blockIdx.x * Cfg::kKeys < top) {
-    if constexpr (kTma) {
-      const int boxes = 32 / a.box, u = lane / boxes, x = lane - u * boxes;
-      const int slot = first + u * 32 + x * a.box;
-      const bool on = u < kUnits && first + u * 32 < top;
-      int page = a.c.pages, row = 0;  // a box behind the last slot lies outside the descriptor's pages: zeros
-      if (on && slot < top) {
-        int p;
-        a.c.div.split(slot, p, row);
-        page = a.c.page_of(b, p);
-      }
-      if (threadIdx.x == 0) abort_flag = 0;
-      if (lane < kUnits) ptx::mbar_init(bar + 8 * lane, 1);
+  if constexpr (kTma) {
+    if (threadIdx.x == 0) abort_flag = 0;
+    if (lane == 0) {
+      for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_init(bar + 8 * s, 1);
       ptx::fence_mbar_init();
-      __syncwarp();
-      if (lane < kUnits && first + lane * 32 < top) ptx::mbar_arrive_expect_tx(bar + 8 * lane, Cfg::kTile);
-      __syncwarp();
-      if (on) {
+    }
+  } else if (a.c.dim < DP) {
+    for (int i = threadIdx.x; i < 4 * Cfg::kWarpBytes / 16; i += 128)
+      reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  const Range r = locate<kU>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + Cfg::sums));
+  Walk lw, cw;
+  bool more = r.p0 < r.p1 && walk_begin<kU>(a, r, lw);
+  const bool any = more;
+  cw = lw;
+
+  // ---- loading: lane g holds where the next unit's g-th box (or slot) lies
+  const int box = kTma ? a.box : 1, boxes = kU / box;
+  if (any) lw.u = lw.start + warp;
+  int next_page[kMine] = {}, next_row[kMine];  // row < 0: no key there
+  auto find = [&]() {
+    while (more && lw.u >= lw.end) {
+      more = walk_next<kU>(a, lw);
+      lw.u = lw.start + warp;
+    }
 #pragma unroll
-        for (int c = 0; c < DP / 64; ++c)
-          ptx::tma_load_4d(kbase + u * Cfg::kTile + c * 4096 + x * a.box * 128, &maps.k, bar + 8 * u, c * 64, h, row, page);
-      }
-    } else {
-      if (a.c.dim < DP) {
-        for (int i = threadIdx.x; i < Cfg::q / 16; i += 128) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-      }
-#pragma unroll
-      for (int u = 0; u < kUnits; ++u) {
-        const int slot = first + u * 32 + lane;
-        int page = 0, row = -1;
-        if (slot < top) {
-          int p;
-          a.c.div.split(slot, p, row);
-          page = a.c.page_of(b, p);
-        }
-        const int c = lane % kLanesRow;
-        const __nv_bfloat16* kb = a.c.k + h * a.c.kh + c * 8;
-#pragma unroll
-        for (int i = 0; i < kLanesRow; ++i) {
-          const int r = lane / kLanesRow + i * (32 / kLanesRow);
-          const int p = __shfl_sync(0xffffffffu, page, r), x = __shfl_sync(0xffffffffu, row, r);
-          if (c * 8 < a.c.dim)
-            mma::cp_async_16_or_zero(kbase + u * Cfg::kTile + mma::tile_at<32>(r, c),
-                                     x >= 0 ? kb + p * a.c.kp + x * a.c.ks : kb, x >= 0);
-        }
+    for (int e = 0; e < kMine; ++e) {
+      next_row[e] = -1;
+      const int g = lane + 32 * e, slot = lw.u * kU + g * box;
+      if (more && g < boxes && slot < lw.k.hi) {
+        int p;
+        a.c.div.split(slot, p, next_row[e]);
+        next_page[e] = __ldg(a.c.table + lw.b * a.c.table_stride + p);
       }
     }
+  };
+  auto load = [&](int stage) {
+    if (more) {
+      const uint32_t kd = base + stage * Cfg::kTile;
+#pragma unroll
+      for (int e = 0; e < kMine; ++e)
+        if (next_row[e] >= 0 && (unsigned)next_page[e] >= (unsigned)a.c.pages) {
+          record_status(a.c.status, BS_ERR_CAPACITY);
+          next_page[e] = next_page[e] < 0 ? 0 : a.c.pages - 1;
+        }
+      if constexpr (kTma) {  // at most kU / 8 <= 32 boxes: the first of a lane's places
+        if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * stage, Cfg::kTile);
+        __syncwarp();
+        if (lane < boxes) {
+          // a box behind the last slot lies outside the descriptor's pages: zeros
+          const int page = next_row[0] >= 0 ? next_page[0] : a.c.pages, row = max(next_row[0], 0);
+#pragma unroll
+          for (int x = 0; x < DP / 64; ++x)
+            ptx::tma_load_4d(kd + x * (kU * 128) + lane * box * 128, &maps.k, bar + 8 * stage, x * 64, lw.h, row, page);
+        }
+      } else {
+        constexpr int kLanesRow = DP / 8;
+        const int c = lane % kLanesRow;
+        const __nv_bfloat16* kb = a.c.k + lw.h * a.c.kh + c * 8;
+#pragma unroll
+        for (int i = 0; i < kU * kLanesRow / 32; ++i) {
+          const int row = lane / kLanesRow + i * (32 / kLanesRow);
+          const int e = i * (32 / kLanesRow) / 32;  // the same for all lanes
+          const int p = __shfl_sync(0xffffffffu, next_page[e], row & 31), x = __shfl_sync(0xffffffffu, next_row[e], row & 31);
+          if (c * 8 < a.c.dim)
+            mma::cp_async_16_or_zero(kd + mma::tile_at<kU>(row, c), x >= 0 ? kb + p * a.c.kp + x * a.c.ks : kb, x >= 0);
+        }
+      }
+      lw.u += 4;
+      find();
+    }
+    if constexpr (!kTma) ptx::cp_async_commit();
+  };
+  find();
+#pragma unroll
+  for (int s = 0; s < Cfg::kStages - 1; ++s) load(s);
+  int stage = 0, phase = 0;
+  const uint32_t qaddr = ptx::smem_addr(qs);
+  const int mine = lane / 4 + (lane & 3) * 8;  // the slots of a unit that this lane stores: mine, mine + 32
+
+  // ---- behind an item's last unit scores are only copied, by all CTAs alike, in
+  // segments of 1024 slots, while the first keys are on their way
+  if (a.out != a.scores) {
+    const int segs = (a.capacity + 1023) / 1024;
+    for (int64_t i = blockIdx.x; i < (int64_t)a.B * a.Hkv * segs; i += gridDim.x) {
+      const int64_t item = i / segs;
+      const int seg = (int)(i - item * segs), b = (int)(item / a.Hkv);
+      const int from = max(seg * 1024, (a.c.len(b, a.T) + a.T + kU - 1) / kU * kU), to = min(a.capacity, seg * 1024 + 1024);
+      const float* src = a.scores + item * a.capacity;
+      float* dst = a.out + item * a.capacity;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = src[min(from + (int)threadIdx.x + j * 128, a.capacity - 1)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (from + (int)threadIdx.x + j * 128 < to) dst[from + threadIdx.x + j * 128] = v[j];
+    }
+  }
+
+  while (any) {
+    const int64_t row0 = ((int64_t)cw.b * a.Hkv + cw.h) * a.capacity;
     for (int i = threadIdx.x; i < rows8 * (DP / 8); i += 128) {
       const int r = i / (DP / 8), c = i - r * (DP / 8), e = a.i0 + r / a.G;
       uint4 v = make_uint4(0, 0, 0, 0);
       float2 f = make_float2(INFINITY, __int_as_float(-1));
       if (r < a.rows) {
-        const int u = a.accepted ? a.accepted[(int64_t)b * a.A + e] : e;
-        if ((unsigned)u < (unsigned)a.T) {
-          const int hq = h * a.G + r % a.G;
+        const int u = a.accepted ? a.accepted[(int64_t)cw.b * a.T + e] : e;
+        if ((unsigned)u < (unsigned)a.tokens) {
+          const int hq = cw.h * a.G + r % a.G;
           if (c * 8 < a.c.dim)
-            v = __ldg(reinterpret_cast<const uint4*>(a.q + b * a.qb + u * a.qt + hq * a.qh + c * 8));
-          const float l = a.lse[((int64_t)b * a.T + u) * a.Hq + hq];
-          if (l != -INFINITY) f = make_float2(l * kLog2e, __int_as_float(n + e));
+            v = __ldg(reinterpret_cast<const uint4*>(a.q + cw.b * a.qb + u * a.qt + hq * a.qh + c * 8));
+          const float l = a.lse[((int64_t)cw.b * a.tokens + u) * a.Hq + hq];
+          if (l != -INFINITY) f = make_float2(l * kLog2e, __int_as_float(cw.k.n + e));
         }
       }
       *reinterpret_cast<uint4*>(qs + qat(r, c)) = v;
       if (c == 0) info[r] = f;
     }
-    if constexpr (!kTma) ptx::cp_async_wait_all();
     __syncthreads();
-  }
-  const uint32_t qaddr = ptx::smem_addr(qs);
+    // the scores to add to are asked for one unit ahead
+    const int top = a.out != a.scores ? a.capacity : min(a.capacity, cw.k.hi);
+    float next[kMine];
+    auto ask = [&](int u) {
 #pragma unroll
-  for (int u = 0; u < kUnits; ++u) {
-    const int slot0 = first + u * 32;
-    float sum[4] = {0.f, 0.f, 0.f, 0.f};  // slots slot0 + lane / 4 + 8 i
-    if (slot0 < top) {
-      if constexpr (kTma) {
-        ptx::mbar_wait(bar + 8 * u, 0, &abort_flag);  // a wait that ran out is reported at the end
-        __syncwarp();
-      }
-      uint32_t kf[2][KS][4];
+      for (int e = 0; e < kMine; ++e) next[e] = __ldg(a.scores + row0 + min(u * kU + mine + 32 * e, a.capacity - 1));
+    };
+    ask(cw.start + warp);
+    for (int u = cw.start + warp; u < cw.end; u += 4) {
+      const int slot0 = u * kU;
+      float before[kMine];
 #pragma unroll
-      for (int mt = 0; mt < 2; ++mt)
+      for (int e = 0; e < kMine; ++e) before[e] = next[e];
+      ask(u + 4);
+      const uint32_t kt = base + stage * Cfg::kTile;
+      if constexpr (kTma)
+        ptx::mbar_wait(bar + 8 * stage, phase, &abort_flag);  // a wait that ran out is reported at the end
+      else
+        ptx::cp_async_wait<Cfg::kStages - 2>();
+      __syncwarp();
+      load((stage + Cfg::kStages - 1) % Cfg::kStages);
+      if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
+      uint32_t kf[MT][KS][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          mma::ldsm_x4(kbase + u * Cfg::kTile + mma::tile_at<32>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), kf[mt][k]);
+          mma::ldsm_x4(kt + mma::tile_at<kU>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), kf[mt][k]);
+      float sum[2 * MT] = {};  // slots slot0 + lane / 4 + 8 i
       for (int r = 0; r < rows8; r += 8) {
-        float s[2][4] = {};
+        float s[MT][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
           uint32_t f[4];
           mma::ldsm_x4(qaddr + qat(r + (lane & 7), 2 * k + (lane >> 3)), f);
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
+          for (int mt = 0; mt < MT; ++mt) {
             mma::bf16_16816(s[mt], kf[mt][k], f[0], f[1]);
             mma::bf16_16816(s[mt], kf[mt][k + 1], f[2], f[3]);
           }
         }
         const float2 f0 = info[r + (lane & 3) * 2], f1 = info[r + (lane & 3) * 2 + 1];
 #pragma unroll
-        for (int mt = 0; mt < 2; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = e & 1 ? f1 : f0;
-            const int slot = slot0 + mt * 16 + lane / 4 + (e >> 1) * 8;
+            const int key = slot0 + mt * 16 + lane / 4 + (e >> 1) * 8;
             const float p = mma::exp2_fast(s[mt][e] * a.scale2 - f.x);
-            sum[mt * 2 + (e >> 1)] += slot <= __float_as_int(f.y) ? p : 0.f;
+            sum[mt * 2 + (e >> 1)] += key <= __float_as_int(f.y) ? p : 0.f;
           }
       }
-    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
-      sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+      for (int i = 0; i < 2 * MT; ++i) {
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
+        sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 2);
+      }
+      const int sel = lane & 3;
+#pragma unroll
+      for (int e = 0; e < kMine; ++e) {
+        const float* t = sum + 4 * e;
+        const float add = sel == 0 ? t[0] : sel == 1 ? t[1] : sel == 2 ? t[2] : t[3];
+        if (slot0 + mine + 32 * e < top) a.out[row0 + slot0 + mine + 32 * e] = before[e] + add;
+      }
     }
-    const int sel = lane & 3, slot = slot0 + mine;
-    const float add = sel == 0 ? sum[0] : sel == 1 ? sum[1] : sel == 2 ? sum[2] : sum[3];
-    if (slot < a.capacity && (slot < top || a.out != a.scores)) a.out[base + slot] = before[u] + add;
+    if (!walk_next<kU>(a, cw)) break;
+    __syncthreads();
   }
   if constexpr (kTma) {
-    if (first < top && *(volatile int*)&abort_flag) {
+    if (*(volatile int*)&abort_flag) {
       if (lane == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
       // copies in flight end before the CTA's memory is given back
       volatile int gone = 0;
-      for (int u = 0; u < kUnits && first + u * 32 < top; ++u) ptx::mbar_wait(bar + 8 * u, 0, &gone);
+      for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_wait(bar + 8 * s, phase ^ 1, &gone);
     }
+  } else {
+    ptx::cp_async_wait_all();
   }
 }
 
 template <int DP, bool kTma>
-int scores_launch(ScoreArgs a, const CacheMaps& maps, int64_t Hkv, int64_t B, cudaStream_t st) {
+int scores_launch(ScoreArgs a, const CacheMaps& maps, cudaStream_t st) {
   using Cfg = ScoreCfg<DP>;
   static bool set[64] = {};
   int dev = 0;
   BS_CUDA(cudaGetDevice(&dev));
-  constexpr int kMost = 128 * 1024;
+  constexpr int kMost = 200 * 1024;
   if (dev >= 64 || !set[dev]) {
     BS_CUDA(cudaFuncSetAttribute(kv_scores_kernel<DP, kTma>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost));
     if (dev < 64) set[dev] = true;
   }
   // as many accepted entries at a time as their queries fit beside the keys
   const int step = std::max(1, (kMost - Cfg::smem(0)) / (DP * 2 + 8) / 8 * 8 / a.G);
-  const dim3 grid((unsigned)cdiv(a.capacity, (int64_t)Cfg::kKeys), (unsigned)(B * Hkv));
-  for (a.i0 = 0; a.i0 < a.A; a.i0 += step) {
-    a.rows = std::min(step, a.A - a.i0) * a.G;
-    kv_scores_kernel<DP, kTma><<<grid, 128, Cfg::smem((a.rows + 7) / 8 * 8), st>>>(a, maps);
+  for (a.i0 = 0; a.i0 < a.T; a.i0 += step) {
+    a.rows = std::min(step, a.T - a.i0) * a.G;
+    const int smem = Cfg::smem((a.rows + 7) / 8 * 8);
+    const int grid = sm_count() * (smem <= 113 * 1024 ? 2 : 1);
+    kv_scores_kernel<DP, kTma><<<grid, 128, smem, st>>>(a, maps);
     BS_LAUNCHED();
     a.scores = a.out;
   }
@@ -292,18 +356,44 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   const int n = min(a.c.len(b, 0), a.capacity);
   const int want = min(n, a.budget);
   const float* scores = a.scores + (int64_t)item * a.capacity;
-  // this CTA's slots [s0, s1), a multiple of 4 each
+  // this CTA's slots [s0, s1)
   const int per = ((n + cluster - 1) / cluster + 3) / 4 * 4;
   const int s0 = min(n, rank * per), s1 = min(n, s0 + per), mine = s1 - s0;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // each warp takes a contiguous run of slots, 32 at a time
+  const int run = ((mine + kSel / 32 - 1) / (kSel / 32) + 31) / 32 * 32;
+  const int w0 = min(mine, warp * run), steps = (min(mine, w0 + run) - w0 + 31) / 32;
   const bool fits = per <= a.held;
-  auto key_at = [&](int i) -> uint32_t {
-    const int s = s0 + i;
-    return s < a.first || s >= n - a.last ? 0xffffffffu : score_key(scores[s]);
+  auto key_of = [&](int s, float x) -> uint32_t { return s < a.first || s >= n - a.last ? 0xffffffffu : score_key(x); };
+  if (fits) {
+    // eight loads of a lane in flight; the loops stay short, since each is run once
+    // and its instructions come from memory too
+    for (int j = 0; j < steps; j += 8) {
+      float x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = __ldg(scores + min(s0 + w0 + (j + e) * 32 + lane, a.capacity - 1));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int i = w0 + (j + e) * 32 + lane;
+        if (j + e < steps) held[i] = key_of(s0 + i, x[e]);
+      }
+    }
+    __syncwarp();
+  }
+  // f(slot of this lane or -1, its key) for every step of the warp
+  auto walk = [&](auto&& f) {
+    const int last = min(mine, w0 + run);
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) {
+      const int i = w0 + j * 32 + lane, c = min(i, last - 1);
+      const uint32_t k = fits ? held[c] : key_of(s0 + c, scores[s0 + c]);
+      f(i < last ? s0 + i : -1, i < last ? k : 0u);
+    }
   };
-  auto key = [&](int i) -> uint32_t { return fits ? held[i] : key_at(i); };
-  if (fits)
-    for (int i = threadIdx.x; i < mine; i += kSel) held[i] = key_at(i);
 
+  const uint32_t below = (1u << lane) - 1u;
+  uint32_t* match = held + a.held;
+  int matches = 0;
   uint32_t prefix = 0, mask = 0;
   int need = want;  // slots still to choose among those whose key matches prefix
   if (want < n) {
@@ -312,39 +402,50 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
       uint32_t* hs = hist[pass & 1];
       for (int i = threadIdx.x; i < 256; i += kSel) hs[i] = 0;
       __syncthreads();
-      for (int i = threadIdx.x; i < mine; i += kSel) {
-        const uint32_t k = key(i);
-        if ((k & mask) == prefix) atomicAdd(&hs[k >> shift & 255], 1u);
+      if (pass == 0) {
+        // sign and exponent: few digits, so a warp counts equal ones together
+        walk([&](int slot, uint32_t k) {
+          const uint32_t same = __match_any_sync(0xffffffffu, slot >= 0 ? k >> 24 : 256u);
+          if (slot >= 0 && lane == __ffs(same) - 1) atomicAdd(&hs[k >> 24], (uint32_t)__popc(same));
+        });
+      } else if (fits) {
+        // the keys that still match, put together by each warp after the first digit
+        if (pass == 1) {
+          walk([&](int slot, uint32_t k) {
+            const bool on = slot >= 0 && (k & mask) == prefix;
+            const uint32_t m = __ballot_sync(0xffffffffu, on);
+            if (on) match[w0 + matches + __popc(m & below)] = k;
+            matches += __popc(m);
+          });
+          __syncwarp();
+        }
+        for (int j = lane; j < matches; j += 32) {
+          const uint32_t k = match[w0 + j];
+          if ((k & mask) == prefix) atomicAdd(&hs[k >> shift & 255], 1u);
+        }
+      } else {
+        walk([&](int slot, uint32_t k) {
+          if (slot >= 0 && (k & mask) == prefix) atomicAdd(&hs[k >> shift & 255], 1u);
+        });
       }
       ptx::cluster_sync();
-      // the digit whose bin holds the need-th highest key: warp 0, eight bins a lane from the top
-      if (threadIdx.x < 32) {
-        uint32_t bin[8], sum = 0;
+      // every CTA finds the digit whose bin holds the need-th highest key: a thread
+      // per bin from the top, a scan, and the one thread whose bin it is
+      uint32_t bin = 0;
+      if (threadIdx.x < 256)
+        for (int r = 0; r < cluster; ++r) bin += dsmem_u32(ptx::smem_addr(&hs[255 - threadIdx.x]), r);
+      uint32_t incl = bin;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int d = 255 - (threadIdx.x * 8 + j);
-          uint32_t v = 0;
-          for (int r = 0; r < cluster; ++r) v += dsmem_u32(ptx::smem_addr(&hs[d]), r);
-          bin[j] = v;
-          sum += v;
-        }
-        uint32_t incl = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
-          if ((int)threadIdx.x >= o) incl += v;
-        }
-        uint32_t above = incl - sum;
-        if (above < (uint32_t)need && (uint32_t)need <= incl) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            if (above < (uint32_t)need && (uint32_t)need <= above + bin[j]) {
-              found[0] = 255 - (threadIdx.x * 8 + j);
-              found[1] = need - above;
-            }
-            above += bin[j];
-          }
-        }
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31 && warp < 8) warps[0][warp] = incl;
+      __syncthreads();
+      if (threadIdx.x < 256) {
+        uint32_t above = incl - bin;
+        for (int w = 0; w < warp; ++w) above += warps[0][w];
+        if (above < (uint32_t)need && (uint32_t)need <= above + bin) found[0] = 255 - threadIdx.x, found[1] = need - above;
       }
       __syncthreads();
       prefix |= found[0] << shift;
@@ -355,51 +456,41 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   }
   // key == prefix: the first `need` in slot order are kept; key > prefix: all
   const bool all = want == n;
-  const int run = (mine + kSel - 1) / kSel;
-  const int i0 = min(mine, (int)threadIdx.x * run), i1 = min(mine, i0 + run);
   uint32_t gt = 0, eq = 0;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = all ? 0u : key(i);
-    gt += all || k > prefix;
-    eq += !all && k == prefix;
-  }
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t ig = gt, ie = eq;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t x = __shfl_up_sync(0xffffffffu, ig, o), y = __shfl_up_sync(0xffffffffu, ie, o);
-    if (lane >= o) ig += x, ie += y;
-  }
-  if (lane == 31) warps[0][warp] = ig, warps[1][warp] = ie;
+  walk([&](int slot, uint32_t k) {
+    gt += __popc(__ballot_sync(0xffffffffu, slot >= 0 && (all || k > prefix)));
+    eq += __popc(__ballot_sync(0xffffffffu, slot >= 0 && !all && k == prefix));
+  });
   __syncthreads();
-  if (threadIdx.x == 0) {
-    uint32_t x = 0, y = 0;
-    for (int w = 0; w < kSel / 32; ++w) {
-      const uint32_t u = warps[0][w], v = warps[1][w];
-      warps[0][w] = x, warps[1][w] = y;
-      x += u, y += v;
-    }
-    totals[0] = x, totals[1] = y;
+  if (lane == 0) warps[0][warp] = gt, warps[1][warp] = eq;
+  __syncthreads();
+  uint32_t bg = 0, be = 0, tg = 0, te = 0;
+#pragma unroll
+  for (int w = 0; w < kSel / 32; ++w) {
+    const uint32_t u = warps[0][w], v = warps[1][w];
+    if (w < warp) bg += u, be += v;
+    tg += u, te += v;
   }
+  if (threadIdx.x == 0) totals[0] = tg, totals[1] = te;
   ptx::cluster_sync();
-  uint32_t bg = warps[0][warp] + ig - gt, be = warps[1][warp] + ie - eq;
   for (int r = 0; r < rank; ++r) {
     bg += dsmem_u32(ptx::smem_addr(&totals[0]), r);
     be += dsmem_u32(ptx::smem_addr(&totals[1]), r);
   }
   int32_t* kept = a.kept + (int64_t)item * a.budget;
   float* out = a.out_scores + (int64_t)item * a.out_capacity;
-  for (int i = i0; i < i1; ++i) {
-    const uint32_t k = all ? 0u : key(i);
-    const bool more = all || k > prefix, same = !all && k == prefix;
-    if (more || (same && be < (uint32_t)need)) {
-      const uint32_t at = bg + min(be, (uint32_t)need);
-      kept[at] = s0 + i;
-      if (at < (uint32_t)a.out_capacity) out[at] = scores[s0 + i];
+  walk([&](int slot, uint32_t k) {
+    const bool more = slot >= 0 && (all || k > prefix), same = slot >= 0 && !all && k == prefix;
+    const uint32_t mg = __ballot_sync(0xffffffffu, more), me = __ballot_sync(0xffffffffu, same);
+    const uint32_t eq0 = be + __popc(me & below);
+    if (more || (same && eq0 < (uint32_t)need)) {
+      const uint32_t at = bg + __popc(mg & below) + min(eq0, (uint32_t)need);
+      kept[at] = slot;
+      if (at < (uint32_t)a.out_capacity) out[at] = scores[slot];
     }
-    bg += more;
-    be += same;
-  }
+    bg += __popc(mg);
+    be += __popc(me);
+  });
   // behind the kept slots: -1 and zero scores
   for (int i = want + rank * kSel + threadIdx.x; i < a.budget; i += cluster * kSel) kept[i] = -1;
   for (int i = want + rank * kSel + threadIdx.x; i < a.out_capacity; i += cluster * kSel) out[i] = 0.f;
@@ -490,7 +581,7 @@ extern "C" int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int
   BS_TRY(paged_cache(fn, cache, A, false, &a.c));
   BS_ARG(Hq > 0 && Hq % cache->heads == 0 && Hq <= 65535, "%s: query heads must be a multiple of the cache's heads", fn);
   BS_ARG(capacity > 0 && capacity <= a.c.capacity, "%s: scores for more slots than the page table has", fn);
-  BS_ARG(cache->batch * cache->heads <= 65535, "%s: more than 65535 (sequence, kv head) pairs", fn);
+  BS_ARG(cache->batch * cache->heads < INT32_MAX, "%s: sizes too large", fn);
   BS_ALIGNED16(q->ptr, "q");
   BS_REQUIRE(q->stride_b % 8 == 0 && q->stride_t % 8 == 0 && q->stride_h % 8 == 0, BS_ERR_MISALIGNED,
              "%s: q strides must be multiples of 8 elements", fn);
@@ -503,19 +594,22 @@ extern "C" int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int
   a.scores = scores;
   a.out = scores_out;
   a.scale2 = scale * kLog2e;
-  a.T = (int)T, a.A = (int)A, a.Hq = (int)Hq, a.capacity = (int)capacity;
+  a.tokens = (int)T, a.Hq = (int)Hq, a.capacity = (int)capacity;
+  a.B = (int)cache->batch, a.Hkv = (int)cache->heads, a.tiles = 1;
+  a.T = (int)A;
+  a.setup = 4;
+  a.min_chunk = 4;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const int64_t D = cache->dim;
   CacheMaps maps = {};
-  a.box = cache_box_rows(cache, 32);
+  a.box = cache_box_rows(cache, D <= 64 ? ScoreCfg<64>::kU : ScoreCfg<128>::kU);
   if (a.box >= 8) {
     BS_TRY(cache_maps(cache, a.box, false, &maps));
-    return D <= 64 ? scores_launch<64, true>(a, maps, cache->heads, cache->batch, st)
-                   : scores_launch<128, true>(a, maps, cache->heads, cache->batch, st);
+    return D <= 64 ? scores_launch<64, true>(a, maps, st) : scores_launch<128, true>(a, maps, st);
   }
-  return D <= 64 ? scores_launch<64, false>(a, maps, cache->heads, cache->batch, st)
-                 : scores_launch<128, false>(a, maps, cache->heads, cache->batch, st);
+  a.box = 1;
+  return D <= 64 ? scores_launch<64, false>(a, maps, st) : scores_launch<128, false>(a, maps, st);
 }
 
 extern "C" int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_t capacity, int64_t budget,
@@ -543,17 +637,17 @@ extern "C" int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_
   a.out_width = (int)out_width, a.out_capacity = (int)(out_width * cache->page_size);
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // CTAs per (sequence, kv head): about 8192 scores each, up to eight
+  // CTAs per (sequence, kv head): 8192 scores each, up to eight CTAs
   int cluster = 1;
   while (cluster < 8 && (int64_t)cluster * 8192 < capacity) cluster *= 2;
   const int64_t per = cdiv(cdiv(capacity, (int64_t)cluster), (int64_t)4) * 4;
-  constexpr int kHeldMost = 48 * 1024;  // keys; longer ranges are read again for every digit
-  a.held = (int)std::min<int64_t>(per, kHeldMost);
+  constexpr int kHeldMost = 24 * 1024;  // keys, twice; longer ranges are read again for every digit
+  a.held = (int)(std::min<int64_t>(per, kHeldMost) + 31) / 32 * 32;
   static bool set[64] = {};
   int dev = 0;
   BS_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !set[dev]) {
-    BS_CUDA(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMost * 4));
+    BS_CUDA(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMost * 8));
     if (dev < 64) set[dev] = true;
   }
   cudaLaunchConfig_t cfg = {};
@@ -561,7 +655,7 @@ extern "C" int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_
   const unsigned items = (unsigned)(cache->batch * cache->heads);
   cfg.gridDim = dim3(items * cluster);
   cfg.blockDim = dim3(kSel);
-  cfg.dynamicSmemBytes = (size_t)a.held * 4;
+  cfg.dynamicSmemBytes = (size_t)a.held * 8;
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;

@@ -73,7 +73,7 @@ __device__ __forceinline__ __nv_bfloat16 rounded<__nv_bfloat16>(float x) { retur
 // neighbouring pairs) and, beyond rot, copied chunks.
 template <typename T, int V, bool INTER, bool APPEND>
 __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeArgs<T> a) {
-  constexpr int kPairs = INTER ? V / 2 : V;
+  constexpr int kPairs = INTER ? V / 2 : V, kBatch = 3;
   const int turned = INTER ? a.rot / V : a.rot / 2 / V;
   const int units = turned + (a.D - a.rot) / V;
   const int wide = min(units, a.group);
@@ -117,42 +117,51 @@ __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeA
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) cs[2 * i + 1] *= a.sign;
       }
-#pragma unroll 2
-      for (int h = h0; h < a.Hq + a.Hk; h += heads_at_once) {
-        const bool isq = h < a.Hq;
-        const T* src = isq ? a.q.at(b, t, h) : a.k.at(b, t, h - a.Hq);
-        T* dst;
-        if constexpr (APPEND) {
-          if (!isq && !write) continue;
-          dst = isq ? a.qo.at(b, t, h)
-                    : reinterpret_cast<T*>(a.cache.k) + koff + (int64_t)(h - a.Hq) * a.cache.kh;
-        } else {
-          dst = isq ? a.qo.at(b, t, h) : a.ko.at(b, t, h - a.Hq);
-        }
-        Chunk<T, V> x, y;
+      // kBatch heads at a time: their loads are in flight together
+      for (int hb = h0; hb < a.Hq + a.Hk; hb += kBatch * heads_at_once) {
+        Chunk<T, V> x[kBatch], y[INTER ? 1 : kBatch];
         const bool two = turn && !INTER;
-        if (used) {
-          x.load(src + c);
-          if (two) y.load(src + c + a.rot / 2);
-          if (turn) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int h = min(hb + j * heads_at_once, a.Hq + a.Hk - 1);
+          const T* src = (h < a.Hq ? a.q.at(b, t, h) : a.k.at(b, t, h - a.Hq)) + c;
+          x[j].load(src);
+          if constexpr (!INTER) y[j].load(two ? src + a.rot / 2 : src);
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int h = hb + j * heads_at_once;
+          if (h >= a.Hq + a.Hk) continue;
+          const bool isq = h < a.Hq;
+          T* dst;
+          if constexpr (APPEND) {
+            if (!isq && !write) continue;
+            dst = isq ? a.qo.at(b, t, h)
+                      : reinterpret_cast<T*>(a.cache.k) + koff + (int64_t)(h - a.Hq) * a.cache.kh;
+          } else {
+            dst = isq ? a.qo.at(b, t, h) : a.ko.at(b, t, h - a.Hq);
+          }
+          Chunk<T, V>& u0 = x[j];
+          Chunk<T, V>& u1 = y[INTER ? 0 : j];
+          if (!used) {
+            u0.zero();
+            if (two) u1.zero();
+          } else if (turn) {
 #pragma unroll
             for (int i = 0; i < kPairs; ++i) {
-              const float p = val(INTER ? x.x[2 * i] : x.x[i]);
-              const float r = val(INTER ? x.x[2 * i + 1] : y.x[i]);
+              const float p = val(INTER ? u0.x[2 * i] : u0.x[i]);
+              const float r = val(INTER ? u0.x[2 * i + 1] : u1.x[i]);
               const T e = rounded<T>(p * cs[2 * i] - r * cs[2 * i + 1]);
               const T f = rounded<T>(r * cs[2 * i] + p * cs[2 * i + 1]);
               if constexpr (INTER)
-                x.x[2 * i] = e, x.x[2 * i + 1] = f;
+                u0.x[2 * i] = e, u0.x[2 * i + 1] = f;
               else
-                x.x[i] = e, y.x[i] = f;
+                u0.x[i] = e, u1.x[i] = f;
             }
           }
-        } else {
-          x.zero();
-          y.zero();
+          u0.store(dst + c);
+          if (two) u1.store(dst + c + a.rot / 2);
         }
-        x.store(dst + c);
-        if (two) y.store(dst + c + a.rot / 2);
       }
     }
     if constexpr (APPEND) {
