@@ -172,22 +172,25 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
   const uint32_t qaddr = ptx::smem_addr(qs);
   const int mine = lane / 4 + (lane & 3) * 8;  // the slots of a unit that this lane stores: mine, mine + 32
 
-  // ---- behind an item's last unit scores are only copied, by all CTAs alike, in
-  // segments of 1024 slots, while the first keys are on their way
+  // ---- behind an item's last unit scores are only copied: an equal share of the
+  // whole array for each CTA, while the first keys are on their way
   if (a.out != a.scores) {
-    const int segs = (a.capacity + 1023) / 1024;
-    for (int64_t i = blockIdx.x; i < (int64_t)a.B * a.Hkv * segs; i += gridDim.x) {
-      const int64_t item = i / segs;
-      const int seg = (int)(i - item * segs), b = (int)(item / a.Hkv);
-      const int from = max(seg * 1024, (a.c.len(b, a.T) + a.T + kU - 1) / kU * kU), to = min(a.capacity, seg * 1024 + 1024);
-      const float* src = a.scores + item * a.capacity;
-      float* dst = a.out + item * a.capacity;
-      float v[8];
+    const int64_t all = (int64_t)a.B * a.Hkv * a.capacity, share = (all + gridDim.x - 1) / gridDim.x;
+    const int64_t end = min(all, (blockIdx.x + 1) * share);
+    for (int64_t from = blockIdx.x * share; from < end;) {
+      const int64_t item = from / a.capacity, first = item * a.capacity;
+      const int64_t to = min(end, first + a.capacity);
+      const int n = a.c.len(item / a.Hkv, a.T) + a.T;
+      const int64_t begin = max(from, first + min(a.capacity, (n + kU - 1) / kU * kU));
+      for (int64_t i = begin + threadIdx.x; i < to; i += 16 * 128) {
+        float v[16];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = src[min(from + (int)threadIdx.x + j * 128, a.capacity - 1)];
+        for (int j = 0; j < 16; ++j) v[j] = a.scores[min(i + j * 128, all - 1)];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (from + (int)threadIdx.x + j * 128 < to) dst[from + threadIdx.x + j * 128] = v[j];
+        for (int j = 0; j < 16; ++j)
+          if (i + j * 128 < to) a.out[i + j * 128] = v[j];
+      }
+      from = to;
     }
   }
 
@@ -597,7 +600,7 @@ extern "C" int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int
   a.tokens = (int)T, a.Hq = (int)Hq, a.capacity = (int)capacity;
   a.B = (int)cache->batch, a.Hkv = (int)cache->heads, a.tiles = 1;
   a.T = (int)A;
-  a.setup = 4;
+  a.setup = 8;
   a.min_chunk = 4;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
