@@ -16,6 +16,8 @@
 // SMs for ragged batches or single sequences).  An item inside one range is
 // finished there; the pieces of the others go to the workspace and a second
 // launch (programmatic, so that its start overlaps) joins them.
+#include <type_traits>
+
 #include "bs_paged.cuh"
 
 namespace bs {
@@ -498,9 +500,10 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 // V as it lies in the cache (keys along K, the head contiguous).  Two half tiles
 // of S alternate, so that the next one is ready when a softmax step ends.
 //
-// Two pipelines per CTA, each a group of four softmax warps (a thread per row)
-// and an MMA warp, so that one pipeline's products run while the other's
-// exponentials do.  With more than 128 rows to a kv head (kPair) they take two
+// Two pipelines per CTA, each two groups of four softmax warps (a thread per row;
+// the groups take alternate half tiles) and an MMA warp.  Four softmax warps to a
+// scheduler hide each other's latencies: with one group per pipeline a scheduler
+// issued in 45% of its cycles.  With more than 128 rows to a kv head (kPair) they take two
 // row tiles and share every K and V tile; with fewer they take alternate tiles
 // of keys for the same rows and meet at the end of an item, where both read both
 // accumulators (same lanes of tensor memory).  One more warp fetches K and V by
@@ -512,17 +515,17 @@ template <int DP>
 struct TilesCfg {
   static constexpr int kSlot = 128 * DP * 2;             // a K or V tile, [DP / 64] panels of 128 rows x 128 bytes
   static constexpr int kSlots = DP == 64 ? 10 : 4;
+  // tensor memory of pipeline p: S half tiles at p * kSCol, 64 columns each; O at kOCol + p * DP
+  static constexpr int kBufs = DP == 64 ? 3 : 2;
+  static constexpr uint32_t kSCol = 64 * kBufs, kOCol = 2 * kSCol;
   static constexpr int q = kSlots * kSlot;               // two Q tiles
-  static constexpr int bits = q + 2 * kSlot;             // [256 threads][8 words]
-  static constexpr int ml = bits + 256 * 32;             // [2][128] float2
-  static constexpr int bars = ml + 2 * 128 * 8;
-  static constexpr int total = bars + 320 + 1024;        // barriers; alignment of the base
+  static constexpr int bits = q + 2 * kSlot;             // [512 threads][8 words]
+  static constexpr int ml = bits + 512 * 32;             // [4 groups][128] float2
+  static constexpr int mref = ml + 4 * 128 * 8;          // [2 pipelines][128] float
+  static constexpr int bars = mref + 2 * 128 * 4;
+  static constexpr int total = bars + 512 + 1024;        // barriers; alignment of the base
 };
-constexpr int kTileThreads = 384;
-// Registers of a thread: 168 at launch; the softmax warps' rows of S want more, and
-// the other four warps give it (256 * 200 + 128 * 104 = 384 * 168).
-constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
-constexpr uint32_t kSCol = 128, kOCol = 256;             // pipeline p: S at p * kSCol, O at kOCol + p * 128
+constexpr int kTileThreads = 672;
 constexpr float kRescale = 8.f;
 constexpr int kPolyOf = 8;  // one pair of exponentials in so many runs on the FMA pipe (none 136 us, 1/8 130, 1/4 132 at 2 x 131072 keys, 16 drafts)
 
@@ -620,20 +623,21 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   auto full = [&](int s) { return bar + 8 * s; };
   auto empty = [&](int s) { return bar + 8 * (Cfg::kSlots + s); };
   constexpr int kB = 16 * Cfg::kSlots;
-  auto sfull = [&](int p, int half) { return bar + kB + 16 * p + 8 * half; };
-  auto pready = [&](int p, int half) { return bar + kB + 32 + 16 * p + 8 * half; };
-  auto qfull = [&](int p) { return bar + kB + 64 + 8 * p; };
-  auto pvdone = [&](int p) { return bar + kB + 80 + 8 * p; };
-  auto drain = [&](int p) { return bar + kB + 96 + 8 * p; };
-  auto odone = [&](int p) { return bar + kB + 112 + 8 * p; };
-  const uint32_t meet = bar + kB + 128;
-  static_assert(kB + 136 <= 320, "barriers");
+  auto sfull = [&](int p, int buf) { return bar + kB + 24 * p + 8 * buf; };
+  auto pready = [&](int p, int buf) { return bar + kB + 48 + 24 * p + 8 * buf; };
+  auto pvdone = [&](int p, int buf) { return bar + kB + 96 + 24 * p + 8 * buf; };
+  auto qfull = [&](int p) { return bar + kB + 144 + 8 * p; };
+  auto odone = [&](int p) { return bar + kB + 160 + 8 * p; };
+  auto meet = [&](int p) { return bar + kB + 176 + 8 * p; };
+  auto drain = [&](int i) { return bar + kB + 192 + 8 * i; };
+  auto turn = [&](int p, int w, int half) { return bar + kB + 224 + 64 * p + 16 * w + 8 * half; };
+  static_assert(kB + 352 <= 512, "barriers");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   if (tid < 128) {
     const Range r = locate<kU>(a, blockIdx.x, gridDim.x, sums);
     if (tid == 0) range = r;
-  } else if (warp == 10) {
+  } else if (warp == 18) {
     ptx::tmem_alloc(ptx::smem_addr(&tmem_at), 512);
     ptx::tmem_relinquish();
   } else if (tid == 128) {
@@ -643,16 +647,19 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       ptx::mbar_init(empty(i), kPair ? 2 : 1);
     }
     for (int p = 0; p < 2; ++p) {
-      ptx::mbar_init(sfull(p, 0), 1);
-      ptx::mbar_init(sfull(p, 1), 1);
-      ptx::mbar_init(pready(p, 0), 128);  // one per half: a warp may be a half tile ahead of its group
-      ptx::mbar_init(pready(p, 1), 128);
-      ptx::mbar_init(qfull(p), 128);
-      ptx::mbar_init(pvdone(p), 1);  // each product; only waited for one behind, where its parity is unambiguous
-      ptx::mbar_init(odone(p), 1);   // the last of a piece
+      for (int i = 0; i < Cfg::kBufs; ++i) {
+        ptx::mbar_init(sfull(p, i), 1);
+        ptx::mbar_init(pready(p, i), 128);
+        ptx::mbar_init(pvdone(p, i), 1);
+      }
+      ptx::mbar_init(qfull(p), 256);
+      ptx::mbar_init(meet(p), kPair ? 256 : 512);
+      for (int w = 0; w < 4; ++w)
+        for (int half = 0; half < 2; ++half) ptx::mbar_init(turn(p, w, half), 1);
+      ptx::mbar_init(odone(p), 1);      // the last product of a piece
       ptx::mbar_init(drain(p), 1);
+      ptx::mbar_init(drain(2 + p), 1);
     }
-    ptx::mbar_init(meet, 256);
     ptx::fence_mbar_init();
   }
   __syncwarp();
@@ -660,14 +667,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   __syncthreads();
   ptx::tc_fence_after();
   const Range r = range;
-  const uint32_t tmem = tmem_at;
+  const uint32_t tmem = 0;  // all columns: they start at 0
   bool ok = true;
 
   if (r.p0 < r.p1) {
     int base = 0;  // tiles of the pieces before this one
-    if (warp == 8) {
+    if (warp == 16) {
       // ------------------------------------------------ loader: lane g fetches the g-th box of a tile
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
       Walk w;
       bool more = walk_begin<kU>(a, r, w);
       const int boxes = kU / a.box;
@@ -713,94 +719,103 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         volatile int gone = 0;
         for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
       }
-    } else if (warp == 9 || warp == 10) {
-      // ------------------------------------------------ MMA issue, one warp per pipeline
-      // The whole warp walks the loops and one elected thread issues: descriptors
-      // then stay in uniform registers (in a one-thread branch each product costs
-      // several moves to them, ~115 cycles).
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-      Walk w;
-      bool more = walk_begin<kU>(a, r, w);
-      const int p = warp - 9;
-      const bool elected = ptx::elect_one();
-      constexpr uint32_t idesc_s = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
-      constexpr uint32_t idesc_o = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) /* B with N contiguous */ |
-                                   (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
-      const uint32_t s_col = tmem + p * kSCol, o_col = tmem + kOCol + p * 128;
-      const uint64_t qd = ptx::sdesc_kmajor_sw128(sbase + Cfg::q + p * Cfg::kSlot);
-      const uint64_t kd0 = ptx::sdesc_kmajor_sw128(sbase), vd0 = sdesc_nmajor_sw128(sbase, 16384);
+    } else if (warp >= 17) {
+      // ------------------------------------------------ MMA issue: S and PV of each pipeline have a
+      // warp each.  One thread gets about one product or commit out per 95 cycles whatever its
+      // size (32 to 64 cycles of the tensor pipe here), so four threads issue.  The whole warp
+      // walks the loops and one elected thread issues.
+      const int p = (warp - 17) & 1;
       constexpr int step = kPair ? 1 : 2;
       const int first = kPair ? 0 : p;
-      int halves = 0, pieces = 0;  // half tiles and pieces of this pipeline so far
-      while (more && ok) {
-        const int n = w.end - w.start, total = first < n ? 2 * ((n - first + step - 1) / step) : 0;
-        // S of half tile h of the piece, into half h & 1 of the S columns
-        auto scores = [&](int h) {
-          const uint32_t ks = 2 * (base + first + (h >> 1) * step), ka = ks % Cfg::kSlots;
-          if (!(h & 1)) {
-            ok = warp_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
-            if (!ok) return;
-            ptx::tc_fence_after();
+      constexpr int kBufs = Cfg::kBufs;
+      const uint32_t s_col = p * Cfg::kSCol, o_col = Cfg::kOCol + p * DP;
+      const bool elected = ptx::elect_one();
+      Walk w;
+      bool more = walk_begin<kU>(a, r, w);
+      int halves = 0, pieces = 0, tiles = 0;  // half tiles and pieces of this pipeline, tiles of the CTA so far
+      if (warp < 19) {
+        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((64u >> 3) << 17) | ((128u >> 4) << 24);
+        const uint64_t qd = ptx::sdesc_kmajor_sw128(sbase + Cfg::q + p * Cfg::kSlot), kd0 = ptx::sdesc_kmajor_sw128(sbase);
+        while (more && ok) {
+          const int n = w.end - w.start, total = first < n ? 2 * ((n - first + step - 1) / step) : 0;
+          if (total) {
+            ok = warp_wait(qfull(p), pieces & 1, abort);
+            ++pieces;
           }
-          if (elected) {
-            const uint64_t kd = kd0 + ka * (Cfg::kSlot >> 4) + (h & 1) * (8192 >> 4);
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-              const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-              ptx::mma_ss_bf16(s_col + (h & 1) * 64, qd + off, kd + off, idesc_s, k > 0);
-            }
-            ptx::tc_commit(sfull(p, h & 1));
-            if (h & 1) ptx::tc_commit(empty(ka));
-          }
-          __syncwarp();
-        };
-        if (total) {
-          ok = warp_wait(qfull(p), pieces & 1, abort);
-          ++pieces;
-          if (ok) scores(0);
-          if (ok) scores(1);
-          for (int h = 0; h < total && ok; ++h) {
-            const uint32_t vs = 2 * (base + first + (h >> 1) * step) + 1, va = vs % Cfg::kSlots;
-            ok = warp_wait(pready(p, h & 1), (halves >> 1) & 1, abort) && warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
+          for (int h = 0; h < total && ok; ++h, ++halves) {
+            const uint32_t ks = 2 * (tiles + first + (h >> 1) * step), ka = ks % Cfg::kSlots;
+            if (!(h & 1)) ok = warp_wait(full(ka), (ks / Cfg::kSlots) & 1, abort);
+            // the product that last read the weights in these columns has ended
+            const uint32_t buf = (uint32_t)halves % kBufs, use = (uint32_t)halves / kBufs;
+            if (use) ok = ok && warp_wait(pvdone(p, buf), (use - 1) & 1, abort);
             if (!ok) break;
-            ++halves;
+            ptx::tc_fence_after();
+            if (elected) {
+              const uint64_t kd = kd0 + ka * (Cfg::kSlot >> 4) + (h & 1) * (8192 >> 4);
+#pragma unroll
+              for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                ptx::mma_ss_bf16(s_col + buf * 64, qd + off, kd + off, idesc, k > 0);
+              }
+              ptx::tc_commit(sfull(p, buf));
+              if (h & 1) ptx::tc_commit(empty(ka));
+            }
+            __syncwarp();
+          }
+          tiles += n;
+          more = walk_next<kU>(a, w);
+        }
+      } else {
+        constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) /* B with N contiguous */ |
+                                   (((uint32_t)DP >> 3) << 17) | ((128u >> 4) << 24);
+        const uint64_t vd0 = sdesc_nmajor_sw128(sbase, 16384);
+        while (more && ok) {
+          const int n = w.end - w.start, total = first < n ? 2 * ((n - first + step - 1) / step) : 0;
+          for (int h = 0; h < total && ok; ++h, ++halves) {
+            const uint32_t vs = 2 * (tiles + first + (h >> 1) * step) + 1, va = vs % Cfg::kSlots;
+            const uint32_t buf = (uint32_t)halves % kBufs, use = (uint32_t)halves / kBufs;
+            ok = warp_wait(pready(p, buf), use & 1, abort);
+            ok = ok && warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
+            if (!ok) break;
             ptx::tc_fence_after();
             if (elected) {
               const uint64_t vd = vd0 + va * (Cfg::kSlot >> 4) + (h & 1) * (8192 >> 4);
 #pragma unroll
               for (int k = 0; k < 4; ++k)
-                ptx::mma_ts_bf16(o_col, s_col + (h & 1) * 64 + k * 8, vd + k * 128, idesc_o, h > 0 || k > 0);
-              ptx::tc_commit(pvdone(p));
+                ptx::mma_ts_bf16(o_col, s_col + buf * 64 + k * 8, vd + k * 128, idesc, h > 0 || k > 0);
+              ptx::tc_commit(pvdone(p, buf));
               if (h + 1 == total) ptx::tc_commit(odone(p));
               if (h & 1) ptx::tc_commit(empty(va));
             }
             __syncwarp();
-            if (h + 2 < total) scores(h + 2);
           }
+          tiles += n;
+          more = walk_next<kU>(a, w);
         }
-        base += n;
-        more = walk_next<kU>(a, w);
       }
       if (!ok && elected) {
         // products in flight end before tensor memory is given back
         volatile int gone = 0;
-        ptx::tc_commit(drain(p));
-        ptx::mbar_wait(drain(p), 0, &gone);
+        ptx::tc_commit(drain(warp - 17));
+        ptx::mbar_wait(drain(warp - 17), 0, &gone);
       }
       __syncwarp();
-    } else if (warp < 8) {
-      // ------------------------------------------------ softmax, a thread per row
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    } else if (warp < 16) {
+      // ------------------------------------------------ softmax, a thread per row; group `hp` of
+      // pipeline p takes its even or odd half tiles
       Walk w;
       bool more = walk_begin<kU>(a, r, w);
-      const int p = warp >> 2, t = tid & 127;
+      const int p = warp >> 3, hp = (warp >> 2) & 1, t = tid & 127;
       const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // lane offset in a tensor-memory address
-      const uint32_t s_col = tmem + lanes + p * kSCol;
+      constexpr int kBufs = Cfg::kBufs;
       uint32_t* bits = reinterpret_cast<uint32_t*>(smem + Cfg::bits) + tid * 8;
-      float2* ml = reinterpret_cast<float2*>(smem + Cfg::ml);
+      float2* ml = reinterpret_cast<float2*>(smem + Cfg::ml) + t;
+      float* mref = reinterpret_cast<float*>(smem + Cfg::mref) + p * 128 + t;
+      const uint32_t my_turn = turn(p, warp & 3, hp), other_turn = turn(p, warp & 3, hp ^ 1);
       constexpr int step = kPair ? 1 : 2;
       const int first = kPair ? 0 : p;
       int halves = 0, pieces = 0, meets = 0;  // half tiles and pieces of this pipeline so far
+      int turns = 0;                          // references that this warp has settled
       while (more && ok) {
         const int n = w.end - w.start;
         const int row0 = w.tile * kRows + (kPair ? p * 128 : 0);
@@ -809,109 +824,120 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         const int tok = mine ? (row0 + t) / a.G : 0, g = mine ? row0 + t - tok * a.G : 0;
         const int hq = w.h * a.G + g;
         const int pt = mine ? a.pos[(int64_t)w.b * a.T + tok] : -1;
-        const float sink = mine && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
         int below = -1;  // keys up to here are outside the row's window (a row not in use is zeroed at the end)
-        float m = -INFINITY, z = 0.f;
+        float m = -INFINITY, z = 0.f;  // z of this group's halves, relative to the reference m that it last saw
         if (first < n) {
-          // Q, and which keys this row may attend; the loads of both are in flight together
+          // half of the row of Q, and which keys the row may attend; the loads of both are in flight together
           uint8_t* qs = smem + Cfg::q + p * Cfg::kSlot;
+          constexpr int kMine = DP / 16;
+          const int c0 = hp * kMine;
           const __nv_bfloat16* q = a.q + w.b * a.qb + tok * a.qt + (int64_t)hq * a.qh;
-          uint4 v[DP / 8];
+          uint4 v[kMine];
 #pragma unroll
-          for (int c = 0; c < DP / 8; ++c)
-            v[c] = __ldg(reinterpret_cast<const uint4*>(q + min(c * 8, a.c.dim - 8)));
+          for (int c = 0; c < kMine; ++c) v[c] = __ldg(reinterpret_cast<const uint4*>(q + min((c0 + c) * 8, a.c.dim - 8)));
           if (a.window) below = max(pt, w.k.n) - a.window;
           if (warp_on && w.k.lo + w.end * kU > w.k.n) draft_bits<8>(a, w.b, w.k.n, tok, pt, bits);
 #pragma unroll
-          for (int c = 0; c < DP / 8; ++c)
-            *reinterpret_cast<uint4*>(qs + mma::tile_at<128>(t, c)) = mine && c * 8 < a.c.dim ? v[c] : make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < kMine; ++c)
+            *reinterpret_cast<uint4*>(qs + mma::tile_at<128>(t, c0 + c)) =
+                mine && (c0 + c) * 8 < a.c.dim ? v[c] : make_uint4(0, 0, 0, 0);
           ptx::fence_proxy_async_smem();
           __syncwarp();
           ptx::mbar_arrive(qfull(p));
           const int total = 2 * ((n - first + step - 1) / step);
-          int done = halves;
-          float s[64];
-          // S of half tile h, asked for; tmem_wait_ld before it is used
-          auto fetch = [&](int h) {
-            ok = warp_wait(sfull(p, h & 1), (done >> 1) & 1, abort);
-            if (!ok || !warp_on) return;
+          for (int h = hp; h < total && ok; h += 2) {
+            const int i = first + (h >> 1) * step, done = halves + h;
+            const int tile0 = w.k.lo + (w.start + i) * kU, key0 = tile0 + hp * 64;
+            const uint32_t buf = (uint32_t)done % kBufs, use = (uint32_t)done / kBufs;
+            const uint32_t s_col = tmem + lanes + p * Cfg::kSCol + buf * 64;
+            ok = warp_wait(sfull(p, buf), use & 1, abort);
+            if (!ok) break;
             ptx::tc_fence_after();
-            ptx::tmem_ld_32x32b_x32(s_col + (h & 1) * 64, reinterpret_cast<uint32_t*>(s));
-            ptx::tmem_ld_32x32b_x32(s_col + (h & 1) * 64 + 32, reinterpret_cast<uint32_t*>(s + 32));
-          };
-          fetch(0);
-          for (int h = 0; h < total && ok; ++h) {
-            const int i = first + (h >> 1) * step;
-            const int tile0 = w.k.lo + (w.start + i) * kU, key0 = tile0 + (h & 1) * 64;
             if (warp_on) {
               const bool slow = key0 + 64 > w.k.n || a.window || a.scale2 < 0.f;
-              ptx::tmem_wait_ld();
-              if (slow) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
+              const float mul = slow ? 1.f : a.scale2;
+              float s[32];
+              // 32 columns of S (read again for the weights: tensor memory is nearer than
+              // the registers that holding all would take)
+              auto fetch = [&](int c) {
+                ptx::tmem_ld_32x32b_x32(s_col + c * 32, reinterpret_cast<uint32_t*>(s));
+                ptx::tmem_wait_ld();
+                if (slow) {
                   const int k0 = key0 + c * 32;
                   const uint32_t see = bit_range(below + 1 - k0, w.k.n - k0) | bits_from(bits, k0 - w.k.n);
 #pragma unroll
-                  for (int e = 0; e < 32; ++e) s[c * 32 + e] = see >> e & 1 ? s[c * 32 + e] * a.scale2 : -INFINITY;
+                  for (int e = 0; e < 32; ++e) s[e] = see >> e & 1 ? s[e] * a.scale2 : -INFINITY;
                 }
-              }
-              float top[22];  // a tree of three-way maxima: few steps that wait for one another
-#pragma unroll
-              for (int e = 0; e < 21; ++e) top[e] = mma::max3(s[3 * e], s[3 * e + 1], s[3 * e + 2]);
-              top[21] = s[63];
-#pragma unroll
-              for (int e = 0; e < 7; ++e) top[e] = mma::max3(top[3 * e], top[3 * e + 1], top[3 * e + 2]);
-              top[0] = mma::max3(mma::max3(top[0], top[1], top[2]), mma::max3(top[3], top[4], top[5]), fmaxf(top[6], top[21]));
-              const float mul = slow ? 1.f : a.scale2;
-              const float mx = top[0] * mul;
-              const bool move = mx > m + kRescale || (m == -INFINITY && mx > -INFINITY);
-              if (__any_sync(0xffffffffu, move)) {
-                const float f = move ? mma::exp2_fast(m - mx) : 1.f;  // 0 from -inf
-                if (move) {
-                  z *= f;
-                  m = mx;
-                }
-                if (h > 0) {
-                  // after the product before this one: S of this half came after the one before that,
-                  // so the parity is not mistaken for an older one's
-                  ok = warp_wait(pvdone(p), (done - 1) & 1, abort);
-                  if (!ok) break;
-                  ptx::tc_fence_after();
-                  const uint32_t o_col = tmem + lanes + kOCol + p * 128;
-#pragma unroll 1
-                  for (int c = 0; c < DP / 32; ++c) {
-                    uint32_t o[32];
-                    ptx::tmem_ld_32x32b_x32(o_col + c * 32, o);
-                    ptx::tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                    ptx::tmem_st_32x32b_x32(o_col + c * 32, o);
-                  }
-                }
-              }
-              const float ref = m == -INFINITY ? 0.f : m;
-              float2 sum[4] = {};
+              };
+              float mx = -INFINITY;
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
+                fetch(c);
+                float top[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top[e] = fmaxf(mma::max3(s[e], s[e + 8], s[e + 16]), s[e + 24]);
+                mx = fmaxf(mx, mma::max3(mma::max3(top[0], top[1], top[2]), mma::max3(top[3], top[4], top[5]),
+                                         fmaxf(top[6], top[7])));
+              }
+              mx *= mul;
+              // the groups of a pipeline settle the row's reference half tile by half tile, in turn
+              float ref = -INFINITY;
+              if (h > 0) {
+                ok = warp_wait(other_turn, (turns + hp + 1) & 1, abort);
+                if (!ok) break;
+                ref = *mref;
+              }
+              const bool move = mx > ref + kRescale || (ref == -INFINITY && mx > -INFINITY);
+              const float f = move ? mma::exp2_fast(ref - mx) : 1.f;  // 0 from -inf
+              if (move) ref = mx;
+              if (move || h == 0) *mref = ref;
+              __syncwarp();
+              if (lane == 0) ptx::mbar_arrive(my_turn);
+              ++turns;
+              if (h > 0 && __any_sync(0xffffffffu, move)) {
+                const uint32_t last = done - 1;  // the product before this one
+                ok = warp_wait(pvdone(p, last % kBufs), (last / kBufs) & 1, abort);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                const uint32_t o_col = tmem + lanes + Cfg::kOCol + p * DP;
+#pragma unroll 1
+                for (int c = 0; c < DP / 16; ++c) {
+                  uint32_t o[16];
+                  ptx::tmem_ld_32x32b_x16(o_col + c * 16, o);
+                  ptx::tmem_wait_ld();
+#pragma unroll
+                  for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  ptx::tmem_st_32x32b_x16(o_col + c * 16, o);
+                }
+              }
+              if (ref != m) {
+                z *= mma::exp2_fast(m - ref);  // z is 0 where m is -inf
+                m = ref;
+              }
+              ref = ref == -INFINITY ? 0.f : ref;
+              float2 sum[2] = {};
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                fetch(c);
                 uint32_t pk[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                  float2 x = mma::fma2(make_float2(s[c * 32 + 2 * e], s[c * 32 + 2 * e + 1]), mul, -ref);
+                  float2 x = mma::fma2(make_float2(s[2 * e], s[2 * e + 1]), mul, -ref);
                   if (e % kPolyOf == kPolyOf - 1) {
                     x = mma::exp2_poly(x);
                   } else {
                     x.x = mma::exp2_fast(x.x);
                     x.y = mma::exp2_fast(x.y);
                   }
-                  sum[e & 3] = mma::add2(sum[e & 3], x);
+                  sum[e & 1] = mma::add2(sum[e & 1], x);
                   pk[e] = pack_bf16x2(x.x, x.y);
                 }
-                ptx::tmem_st_32x32b_x16(s_col + (h & 1) * 64 + c * 16, pk);
+                ptx::tmem_st_32x32b_x16(s_col + c * 16, pk);
               }
-              sum[0] = mma::add2(mma::add2(sum[0], sum[1]), mma::add2(sum[2], sum[3]));
+              sum[0] = mma::add2(sum[0], sum[1]);
               z += sum[0].x + sum[0].y;
             }
-            if (!(h & 1) && (tile0 < w.k.low || tile0 + kU > w.k.n)) {
+            if (hp == 0 && (tile0 < w.k.low || tile0 + kU > w.k.n)) {
               // the tile's boxes bring all their slots: those that hold no key become zeros in V
               const int vs = 2 * (base + i) + 1, va = vs % Cfg::kSlots;
               ok = warp_wait(full(va), (vs / Cfg::kSlots) & 1, abort);
@@ -925,98 +951,107 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
               ptx::fence_proxy_async_smem();
               __syncwarp();
             }
-            ++done;
-            if (h + 1 < total) fetch(h + 1);  // its latency and that of the stores pass together
-            if (!ok) break;
             if (warp_on) ptx::tmem_wait_st();
             ptx::tc_fence_before();
-            ptx::mbar_arrive(pready(p, h & 1));
+            ptx::mbar_arrive(pready(p, buf));
           }
+          halves += total;
         }
         if (!ok) break;
         // ---- end of the piece: read the accumulators
         if (first < n) {
-          halves += 2 * ((n - first + step - 1) / step);
           ok = warp_wait(odone(p), pieces & 1, abort);
           ++pieces;
         }
         if (!ok) break;
+        // the groups' sums: of this pipeline, or of both where they hold the same rows
+        ml[(2 * p + hp) * 128] = make_float2(m, z);
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(meet(kPair ? p : 0));
+        ok = warp_wait(meet(kPair ? p : 0), meets & 1, abort);
+        if (!ok) break;
+        ++meets;
         ptx::tc_fence_after();
+        auto both = [&](int x) {
+          const float2 u = ml[2 * x * 128], v = ml[(2 * x + 1) * 128];
+          const float top = fmaxf(u.x, v.x);
+          const float zz = (u.x == -INFINITY ? 0.f : u.y * mma::exp2_fast(u.x - top)) +
+                           (v.x == -INFINITY ? 0.f : v.y * mma::exp2_fast(v.x - top));
+          return make_float2(top, zz);
+        };
         float f0 = 1.f, f1 = 0.f;
-        if (!kPair) {
-          // both pipelines hold the same rows: common maximum, sums together
-          ml[p * 128 + t] = make_float2(m, z);
-          ptx::tc_fence_before();
-          ptx::mbar_arrive(meet);
-          ok = warp_wait(meet, meets & 1, abort);
-          if (!ok) break;
-          ++meets;
-          ptx::tc_fence_after();
-          const float2 m0 = ml[t], m1 = ml[128 + t];
-          m = fmaxf(m0.x, m1.x);
-          f0 = m0.x == -INFINITY ? 0.f : mma::exp2_fast(m0.x - m);
-          f1 = m1.x == -INFINITY ? 0.f : mma::exp2_fast(m1.x - m);
-          z = m0.y * f0 + m1.y * f1;
+        if (kPair) {
+          const float2 u = both(p);
+          m = u.x, z = u.y;
+        } else {
+          const float2 u = both(0), v = both(1);
+          m = fmaxf(u.x, v.x);
+          f0 = u.x == -INFINITY ? 0.f : mma::exp2_fast(u.x - m);
+          f1 = v.x == -INFINITY ? 0.f : mma::exp2_fast(v.x - m);
+          z = u.y * f0 + v.y * f1;
         }
         const bool whole = w.whole();
         const int64_t slot = 2 * (int64_t)blockIdx.x + (w.start == 0 ? 1 : 0);
         const int dim = a.c.dim, row = (kPair ? p * 128 : 0) + t;
         const int64_t at = ((int64_t)w.b * a.T + tok) * a.Hkv * a.G + hq;
+        const bool speaks = mine && hp == 0 && (kPair || p == 0);  // for the row
         float scale_o = 1.f;
         if (whole && mine) {
           const bool used = pt >= 0;
+          const float sink = a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
           const float top = fmaxf(m, sink);
           const float ref = top == -INFINITY ? 0.f : top;
           const float f = m == -INFINITY ? 0.f : mma::exp2_fast(m - ref);
           const float den = z * f + (a.sinks ? mma::exp2_fast(sink - ref) : 0.f);
           scale_o = used && m > -INFINITY ? f / den : 0.f;
-          if (a.lse && (kPair || p == 0)) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
+          if (a.lse && speaks) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
         }
-        if (!whole && mine && (kPair || p == 0)) a.part_ml[slot * kRows + row] = make_float2(m, z);
+        if (!whole && speaks) a.part_ml[slot * kRows + row] = make_float2(m, z);
         if (warp_on) {
-          // columns of this group: all of its own tile, or one half of the shared one.
-          // bf16 rows go through the piece's Q (no longer read) to be stored in lines.
-          constexpr int kCols = kPair ? DP : DP / 2;
-          const int c0 = kPair ? 0 : p * kCols;
-          uint8_t* stage = smem + Cfg::q + p * Cfg::kSlot;  // a warp's rows where its Q rows were
+          // columns of this group: half of its tile's, or a quarter of the shared tile's.
+          // bf16 rows go through this thread's part of Q (no longer read) to be stored in lines.
+          constexpr int kCols = kPair ? DP / 2 : DP / 4;
+          const int c0 = kPair ? hp * kCols : (2 * p + hp) * kCols;
+          uint8_t* stage = smem + Cfg::q + p * Cfg::kSlot;
+          const int chunk0 = hp * (DP / 16);
 #pragma unroll 1
-          for (int c = c0; c < c0 + kCols; c += 32) {
-            float x[32], y[32];
-            ptx::tmem_ld_32x32b_x32(tmem + lanes + kOCol + (kPair ? p * 128 : 0) + c, reinterpret_cast<uint32_t*>(x));
-            if (!kPair) ptx::tmem_ld_32x32b_x32(tmem + lanes + kOCol + 128 + c, reinterpret_cast<uint32_t*>(y));
+          for (int c = 0; c < kCols; c += 16) {
+            float x[16], y[16];
+            ptx::tmem_ld_32x32b_x16(tmem + lanes + Cfg::kOCol + (kPair ? p * DP : 0) + c0 + c, reinterpret_cast<uint32_t*>(x));
+            if (!kPair) ptx::tmem_ld_32x32b_x16(tmem + lanes + Cfg::kOCol + DP + c0 + c, reinterpret_cast<uint32_t*>(y));
             ptx::tmem_wait_ld();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
+            for (int e = 0; e < 16; ++e) {
               x[e] = f0 == 0.f ? 0.f : x[e] * f0;
               if (!kPair && f1 != 0.f) x[e] += y[e] * f1;
             }
             if (whole) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
+              for (int j = 0; j < 2; ++j) {
                 uint32_t pk[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                   pk[e] = scale_o == 0.f ? 0u : pack_bf16x2(x[j * 8 + 2 * e] * scale_o, x[j * 8 + 2 * e + 1] * scale_o);
-                const int chunk = (c - c0) / 8 + j;
-                *reinterpret_cast<uint4*>(stage + mma::tile_at<128>(t, chunk)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+                *reinterpret_cast<uint4*>(stage + mma::tile_at<128>(t, chunk0 + c / 8 + j)) =
+                    make_uint4(pk[0], pk[1], pk[2], pk[3]);
               }
             } else if (mine) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j)
-                if (c + j * 4 < dim)
-                  a.part_o[(slot * (dim / 4) + c / 4 + j) * kRows + row] =
+              for (int j = 0; j < 4; ++j)
+                if (c0 + c + j * 4 < dim)
+                  a.part_o[(slot * (dim / 4) + (c0 + c) / 4 + j) * kRows + row] =
                       make_float4(x[j * 4], x[j * 4 + 1], x[j * 4 + 2], x[j * 4 + 3]);
             }
             __syncwarp();
           }
           if (whole) {
             constexpr int kChunks = kCols / 8, kAtOnce = 32 / kChunks;
-#pragma unroll
+#pragma unroll 2
             for (int j = 0; j < 32 / kAtOnce; ++j) {
-              const int r = j * kAtOnce + lane / kChunks, chunk = lane % kChunks;
-              const int64_t to = __shfl_sync(0xffffffffu, at, r);
-              const bool on = __shfl_sync(0xffffffffu, (int)mine, r);
-              const uint4 v = *reinterpret_cast<const uint4*>(stage + mma::tile_at<128>((warp & 3) * 32 + r, chunk));
+              const int x = j * kAtOnce + lane / kChunks, chunk = lane % kChunks;
+              const int64_t to = __shfl_sync(0xffffffffu, at, x);
+              const bool on = __shfl_sync(0xffffffffu, (int)mine, x);
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + mma::tile_at<128>((warp & 3) * 32 + x, chunk0 + chunk));
               if (on && c0 + chunk * 8 < dim) *reinterpret_cast<uint4*>(a.out + to * dim + c0 + chunk * 8) = v;
             }
             __syncwarp();
@@ -1024,26 +1059,25 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         }
         ptx::tc_fence_before();
         if (!kPair) {
-          // the other pipeline's accumulator has been read before it is written again
-          ptx::mbar_arrive(meet);
-          ok = warp_wait(meet, meets & 1, abort);
+          // the other pipeline's accumulator has been read before it is written again (a pair's
+          // is only read by the two groups whose next Q its next product waits for)
+          ptx::mbar_arrive(meet(0));
+          ok = warp_wait(meet(0), meets & 1, abort);
           if (!ok) break;
           ++meets;
         }
         base += n;
         more = walk_next<kU>(a, w);
       }
-    } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     }
   }
   __syncwarp();
   if (!ok && lane == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == 10) {
+  if (warp == 18) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem, 512);
+    ptx::tmem_dealloc(tmem_at, 512);
   }
 }
 
@@ -1232,7 +1266,7 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.part_o = static_cast<float4*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * (D / 4));
   a.min_chunk = rows <= 32 ? 4 : 2;
-  a.setup = rows <= 32 ? 8 : 3;
+  a.setup = rows <= 32 ? 8 : 6;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   CacheMaps maps = {};
