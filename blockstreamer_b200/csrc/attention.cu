@@ -525,7 +525,10 @@ struct TilesCfg {
   static constexpr int bars = mref + 2 * 128 * 4;
   static constexpr int total = bars + 512 + 1024;        // barriers; alignment of the base
 };
-constexpr int kTileThreads = 672;
+constexpr int kTileThreads = 768;  // 16 softmax warps, loader, four issuing warps, three idle
+// Registers of a thread: 80 at launch; the softmax warps want more, and the other
+// eight warps give it (512 * 96 + 256 * 48 = 768 * 80).
+constexpr int kSoftmaxRegs = 96, kOtherRegs = 48;
 constexpr float kRescale = 8.f;
 constexpr int kPolyOf = 8;  // one pair of exponentials in so many runs on the FMA pipe (none 136 us, 1/8 130, 1/4 132 at 2 x 131072 keys, 16 drafts)
 
@@ -674,6 +677,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
     int base = 0;  // tiles of the pieces before this one
     if (warp == 16) {
       // ------------------------------------------------ loader: lane g fetches the g-th box of a tile
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
       Walk w;
       bool more = walk_begin<kU>(a, r, w);
       const int boxes = kU / a.box;
@@ -719,11 +723,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         volatile int gone = 0;
         for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
       }
-    } else if (warp >= 17) {
+    } else if (warp >= 17 && warp < 21) {
       // ------------------------------------------------ MMA issue: S and PV of each pipeline have a
       // warp each.  One thread gets about one product or commit out per 95 cycles whatever its
       // size (32 to 64 cycles of the tensor pipe here), so four threads issue.  The whole warp
       // walks the loops and one elected thread issues.
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
       const int p = (warp - 17) & 1;
       constexpr int step = kPair ? 1 : 2;
       const int first = kPair ? 0 : p;
@@ -803,6 +808,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
     } else if (warp < 16) {
       // ------------------------------------------------ softmax, a thread per row; group `hp` of
       // pipeline p takes its even or odd half tiles
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
       Walk w;
       bool more = walk_begin<kU>(a, r, w);
       const int p = warp >> 3, hp = (warp >> 2) & 1, t = tid & 127;
@@ -1069,6 +1075,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         base += n;
         more = walk_next<kU>(a, w);
       }
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     }
   }
   __syncwarp();
