@@ -1274,7 +1274,7 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.part_o = static_cast<float4*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * (D / 4));
   a.min_chunk = rows <= 32 ? 4 : 2;
-  a.setup = rows <= 32 ? 8 : 6;
+  a.setup = rows <= 32 ? 16 : 8;
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   CacheMaps maps = {};

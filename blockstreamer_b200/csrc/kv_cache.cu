@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   const uint32_t below = (1u << lane) - 1u;
   uint32_t* match = held + a.held;
   int matches = 0;
+  uint32_t gt = 0, eq = 0;  // this warp's keys above the chosen one, and equal to it
   uint32_t prefix = 0, mask = 0;
   int need = want;  // slots still to choose among those whose key matches prefix
   if (want < n) {
@@ -412,19 +413,26 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
           if (slot >= 0 && lane == __ffs(same) - 1) atomicAdd(&hs[k >> 24], (uint32_t)__popc(same));
         });
       } else if (fits) {
-        // the keys that still match, put together by each warp after the first digit
+        // the keys that still match, put together by each warp after the first digit;
+        // those above it are counted on the way
         if (pass == 1) {
           walk([&](int slot, uint32_t k) {
             const bool on = slot >= 0 && (k & mask) == prefix;
             const uint32_t m = __ballot_sync(0xffffffffu, on);
+            gt += __popc(__ballot_sync(0xffffffffu, slot >= 0 && (k & mask) > prefix));
             if (on) match[w0 + matches + __popc(m & below)] = k;
             matches += __popc(m);
           });
           __syncwarp();
         }
-        for (int j = lane; j < matches; j += 32) {
-          const uint32_t k = match[w0 + j];
-          if ((k & mask) == prefix) atomicAdd(&hs[k >> shift & 255], 1u);
+        const uint32_t digit = shift == 16 ? 0u : 255u << (shift + 8);  // the last digit found
+        for (int j = 0; j < matches; j += 32) {
+          const uint32_t k = match[w0 + min(j + lane, matches - 1)];
+          const bool on = j + lane < matches, now = on && (k & mask) == prefix;
+          // among keys that matched before the last digit, those above it
+          if (pass > 1)
+            gt += __popc(__ballot_sync(0xffffffffu, on && ((k ^ prefix) & (mask & ~digit)) == 0 && (k & digit) > (prefix & digit)));
+          if (now) atomicAdd(&hs[k >> shift & 255], 1u);
         }
       } else {
         walk([&](int slot, uint32_t k) {
@@ -459,11 +467,21 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   }
   // key == prefix: the first `need` in slot order are kept; key > prefix: all
   const bool all = want == n;
-  uint32_t gt = 0, eq = 0;
-  walk([&](int slot, uint32_t k) {
-    gt += __popc(__ballot_sync(0xffffffffu, slot >= 0 && (all || k > prefix)));
-    eq += __popc(__ballot_sync(0xffffffffu, slot >= 0 && !all && k == prefix));
-  });
+  if (all) {
+    gt = max(0, min(mine, w0 + run) - w0);
+  } else if (fits) {
+    for (int j = 0; j < matches; j += 32) {
+      const uint32_t k = match[w0 + min(j + lane, matches - 1)];
+      const bool near = j + lane < matches && ((k ^ prefix) & 0xffffff00u) == 0;  // all but the last digit
+      gt += __popc(__ballot_sync(0xffffffffu, near && k > prefix));
+      eq += __popc(__ballot_sync(0xffffffffu, near && k == prefix));
+    }
+  } else {
+    walk([&](int slot, uint32_t k) {
+      gt += __popc(__ballot_sync(0xffffffffu, slot >= 0 && k > prefix));
+      eq += __popc(__ballot_sync(0xffffffffu, slot >= 0 && k == prefix));
+    });
+  }
   __syncthreads();
   if (lane == 0) warps[0][warp] = gt, warps[1][warp] = eq;
   __syncthreads();
@@ -489,7 +507,9 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
     if (more || (same && eq0 < (uint32_t)need)) {
       const uint32_t at = bg + __popc(mg & below) + min(eq0, (uint32_t)need);
       kept[at] = slot;
-      if (at < (uint32_t)a.out_capacity) out[at] = scores[slot];
+      // the key gives the score back, but for protected slots and NaN
+      if (at < (uint32_t)a.out_capacity)
+        out[at] = k == 0xffffffffu || k == 0u ? scores[slot] : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
     }
     bg += __popc(mg);
     be += __popc(me);
