@@ -2,8 +2,11 @@
 
 ``rotary_frequencies`` / ``rotary_table`` make the cos/sin table that the rotary
 kernels read, with transformers' scalings for long contexts (yarn, linear);
-``apply_rotary`` is the differentiable form for training.  The kernels
-themselves are in ``kernels``.
+``apply_rotary`` is the differentiable form for training.  ``PagedKVCache``
+holds a batch of sequences and runs the steps of speculative decoding on them
+(append, tree attention, commit, scores, eviction); ``B200GptOssAttention`` is
+the layer around it, with transformers' parameter names.  The kernels themselves
+are in ``kernels``.
 
 Mirrors transformers models/gpt_oss/modeling_gpt_oss.py (GptOssRotaryEmbedding,
 apply_rotary_pos_emb, GptOssAttention), which the reference runs unchanged.
@@ -14,7 +17,7 @@ from __future__ import annotations
 import math
 
 import torch
-from torch import Tensor
+from torch import Tensor, nn
 
 from . import kernels
 
@@ -78,24 +81,143 @@ class _Rotary(torch.autograd.Function):
         return kernels.rope(q, k, table, positions, interleaved)
 
     @staticmethod
-    def backward(ctx, dq: Tensor | None, dk: Tensor | None):
+    def backward(ctx, dq: Tensor, dk: Tensor | None):
+        # gradients that did not arrive are zeros here (autograd makes them); dk is None without k
         table, positions = ctx.saved_tensors
-        if dq is None or dk is None:
-            one = dq if dq is not None else dk
-            if one is None:
-                return None, None, None, None, None
-            g, _ = kernels.rope(_last_contiguous(one), None, table, positions, ctx.interleaved, inverse=True)
-            return (g if dq is not None else None), (g if dk is not None else None), None, None, None
-        gq, gk = kernels.rope(_last_contiguous(dq), _last_contiguous(dk), table, positions, ctx.interleaved,
-                              inverse=True)
+        dq = dq if dq.stride(-1) == 1 else dq.contiguous()
+        if dk is not None and dk.stride(-1) != 1:
+            dk = dk.contiguous()
+        gq, gk = kernels._rope(dq.get_device(), dq, dk, table, positions, ctx.interleaved, True)
         return gq, gk, None, None, None
-
-
-def _last_contiguous(t: Tensor) -> Tensor:
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def apply_rotary(q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interleaved: bool = False):
     """Rotary positions of q and k with gradients (``kernels.rope`` both ways).
     No gradient flows to the table."""
     return _Rotary.apply(q, k, table, positions, interleaved)
+
+
+class PagedKVCache:
+    """Keys and values of ``batch`` sequences in ``pages`` pages of ``page_size`` slots.
+
+    Pages are [page, head, slot, dim] in memory, so that a head's slots of a page
+    lie together.  The host keeps the lengths and hands out the pages; what the
+    kernels read (``page_table``, ``lens``) is on the device.  ``scores`` (with
+    ``track_scores``) accumulates the attention weight of every cached key."""
+
+    def __init__(self, batch: int, pages: int, page_size: int, heads: int, dim: int, max_len: int, device="cuda",
+                 track_scores: bool = False) -> None:
+        shape = (pages, heads, page_size, dim)
+        self.k = torch.zeros(shape, dtype=torch.bfloat16, device=device).transpose(1, 2)
+        self.v = torch.zeros(shape, dtype=torch.bfloat16, device=device).transpose(1, 2)
+        self.page_size, self.max_len = page_size, max_len
+        self.width = -(-max_len // page_size)
+        self.page_table = torch.zeros(batch, self.width, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.scores = None
+        if track_scores:
+            self.scores = torch.zeros(batch, heads, self.width * page_size, dtype=torch.float32, device=device)
+        self.lengths = [0] * batch                      # the host's copy of lens
+        self._free = list(range(pages - 1, -1, -1))
+        self._held: list[list[int]] = [[] for _ in range(batch)]
+
+    def _upload(self) -> None:
+        rows = [h + [0] * (self.width - len(h)) for h in self._held]
+        self.page_table.copy_(torch.tensor(rows, dtype=torch.int32))
+        self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+
+    def reserve(self, tokens: int) -> None:
+        """Pages for ``tokens`` more slots of every sequence."""
+        need = [-(-(n + tokens) // self.page_size) - len(h) for n, h in zip(self.lengths, self._held)]
+        if any(n + tokens > self.max_len for n in self.lengths):
+            raise ValueError(f"a sequence would pass max_len = {self.max_len}")
+        if sum(max(0, x) for x in need) > len(self._free):
+            raise RuntimeError(f"{sum(max(0, x) for x in need)} pages wanted, {len(self._free)} free")
+        if max(need, default=0) > 0:
+            for held, x in zip(self._held, need):
+                held.extend(self._free.pop() for _ in range(max(0, x)))
+            self._upload()
+
+    def append(self, q: Tensor, k: Tensor, v: Tensor, table: Tensor, positions: Tensor,
+               interleaved: bool = False) -> Tensor:
+        """Turns q and k, writes k and v behind the committed keys; returns the turned q."""
+        self.reserve(q.shape[1])
+        return kernels.rope_append(q, k, v, table, positions, self.k, self.v, self.page_table, self.lens, interleaved)
+
+    def attend(self, q: Tensor, positions: Tensor, tree_mask: Tensor | None = None, sinks: Tensor | None = None,
+               window: int = 0):
+        """(out, lse) of the drafted tokens whose keys ``append`` wrote."""
+        return kernels.tree_attention(q, self.k, self.v, self.page_table, self.lens, positions, tree_mask, sinks,
+                                      window)
+
+    def commit(self, accepted: list[list[int]], drafted: int, q: Tensor | None = None, lse: Tensor | None = None) -> None:
+        """Keeps the accepted drafts (ascending indices per sequence) and, given the
+        step's turned ``q`` and its ``lse``, adds their attention to the scores."""
+        most = max((len(x) for x in accepted), default=0)
+        if most:
+            rows = [x + [-1] * (most - len(x)) for x in accepted]
+            acc = torch.tensor(rows, dtype=torch.int32, device=self.k.device)
+            kernels.tree_commit(self.k, self.v, self.page_table, self.lens, acc, drafted)
+            if self.scores is not None and q is not None and lse is not None:
+                kernels.kv_scores_add(self.scores, q, lse, self.k, self.page_table, self.lens, acc, out=self.scores)
+        self.lengths = [n + len(x) for n, x in zip(self.lengths, accepted)]
+        self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
+
+    def evict(self, budget: int, keep_first: int = 4, keep_last: int = 0) -> Tensor:
+        """Cuts every sequence to its ``budget`` best keys per head; returns the kept
+        slots.  Only for layers without a window: slots are no longer positions."""
+        if self.scores is None:
+            raise ValueError("PagedKVCache.evict needs track_scores=True")
+        new = [-(-min(n, budget) // self.page_size) for n in self.lengths]
+        if sum(new) > len(self._free):
+            raise RuntimeError(f"eviction needs {sum(new)} free pages, {len(self._free)} are")
+        taken = [[self._free.pop() for _ in range(x)] for x in new]
+        width = max(1, max(new, default=0))
+        out = torch.tensor([t + [0] * (width - len(t)) for t in taken], dtype=torch.int32, device=self.k.device)
+        budget = min(budget, width * self.page_size)
+        kept, _, scores = kernels.kv_evict(self.k, self.v, self.page_table, self.lens, self.scores, budget, out,
+                                           min(keep_first, budget), min(keep_last, budget - min(keep_first, budget)))
+        self.scores.zero_()
+        self.scores[..., : scores.shape[-1]] = scores
+        for held in self._held:
+            self._free.extend(held)
+        self._held = taken
+        self.lengths = [min(n, budget) for n in self.lengths]
+        self._upload()
+        return kept
+
+
+class B200GptOssAttention(nn.Module):
+    """GptOssAttention (modeling_gpt_oss.py) over a ``PagedKVCache``: drafted tokens
+    (or one token) of every sequence against the cached ones.
+
+    Parameters ``q_proj``, ``k_proj``, ``v_proj``, ``o_proj`` (weight and bias) and
+    ``sinks`` have transformers' names and shapes, on ``meta`` until bound."""
+
+    def __init__(self, config, layer_idx: int = 0, dtype: torch.dtype = torch.bfloat16) -> None:
+        super().__init__()
+        self.heads, self.kv_heads = config.num_attention_heads, config.num_key_value_heads
+        self.head_dim = getattr(config, "head_dim", None) or config.hidden_size // self.heads
+        types = getattr(config, "layer_types", None)
+        kind = types[layer_idx] if types else "full_attention"
+        self.window = config.sliding_window if kind == "sliding_attention" else 0
+        bias = getattr(config, "attention_bias", True)
+        H, D = config.hidden_size, self.head_dim
+        with torch.device("meta"):
+            self.q_proj = nn.Linear(H, self.heads * D, bias=bias, dtype=dtype)
+            self.k_proj = nn.Linear(H, self.kv_heads * D, bias=bias, dtype=dtype)
+            self.v_proj = nn.Linear(H, self.kv_heads * D, bias=bias, dtype=dtype)
+            self.o_proj = nn.Linear(self.heads * D, H, bias=bias, dtype=dtype)
+            self.sinks = nn.Parameter(torch.empty(self.heads, dtype=dtype))
+
+    def forward(self, hidden_states: Tensor, positions: Tensor, cache: PagedKVCache, table: Tensor,
+                tree_mask: Tensor | None = None):
+        """hidden_states [B, T, H], positions [B, T] int32 (negative: unused) ->
+        (output [B, T, H], turned q, lse); the last two go to ``cache.commit``."""
+        B, T, _ = hidden_states.shape
+        q = self.q_proj(hidden_states).view(B, T, self.heads, self.head_dim)
+        k = self.k_proj(hidden_states).view(B, T, self.kv_heads, self.head_dim)
+        v = self.v_proj(hidden_states).view(B, T, self.kv_heads, self.head_dim)
+        q = cache.append(q, k, v, table, positions)
+        out, lse = cache.attend(q, positions, tree_mask, self.sinks.float(), self.window)
+        return self.o_proj(out.view(B, T, -1)), q, lse

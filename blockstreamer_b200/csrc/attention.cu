@@ -1119,15 +1119,16 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
   const int64_t chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
   const int64_t s = before + item * units, e = s + units;
   const int c0 = (int)((s + a.setup) / chunk), c1 = (int)((e - 1) / chunk);
-  if (c0 == c1) return;
   const int dim = a.c.dim, row0 = tile * kRows, rows = min(kRows, a.R - row0);
   const int first = blockIdx.y * kJoinRows, last = min(rows, first + kJoinRows);
   const int row = first + threadIdx.x % kJoinRows;  // each thread: one row, every 16th group of four columns
-  if (row >= last) return;
-  const int t = (row0 + row) / a.G, hq = h * a.G + row0 + row - t * a.G;
-  const bool used = a.pos[(int64_t)b * a.T + t] >= 0;
-  const float sink = a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+  const bool joins = c0 != c1 && row < last;
+  const int t = (row0 + min(row, rows - 1)) / a.G, hq = h * a.G + row0 + min(row, rows - 1) - t * a.G;
+  const bool used = joins && a.pos[(int64_t)b * a.T + t] >= 0;
+  const float sink = joins && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+  // every thread waits, so that this launch does not end before the first
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!joins) return;
   float mx = -INFINITY;
 #pragma unroll 4
   for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, a.part_ml[(2 * (int64_t)x + (x == c0)) * kRows + row].x);

@@ -518,15 +518,25 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions
         raise ValueError("rope: q and k must be [B, T, heads, D] or [T, heads, D], alike but for the heads")
     if q.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("rope: q and k must be bf16 or f32")
-    D = q.shape[-1]
-    rot = _rope_table("rope", table, D)
-    positions = _positions("rope", positions, q.shape[:-2])
-    B, T = (q.shape[0], q.shape[1]) if q.dim() == 4 else (1, q.shape[0])
+    _rope_table("rope", table, q.shape[-1])
+    return _rope(index, q, k, table, _positions("rope", positions, q.shape[:-2]), interleaved, inverse)
+
+
+def _rope(index: int, q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor,
+          interleaved: bool, inverse: bool):
+    """``rope`` of arguments that have been checked (its gradient has the forward's)."""
+    shape = q.shape
     qo = torch.empty_like(q, memory_format=torch.contiguous_format)
-    ko = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
-    _launch("bs_rope", index, _heads("rope", q), _heads("rope", k), _heads("rope", qo), _heads("rope", ko),
-            _DT[q.dtype], B, T, q.shape[-2], 0 if k is None else k.shape[-2], D, _ptr(table), table.shape[0], rot,
-            _ptr(positions), _DT[positions.dtype], interleaved, inverse)
+    if k is None:
+        ko, hk, Hk = None, _NO_HEADS, 0
+        hko = hk
+    else:
+        ko, Hk = torch.empty_like(k, memory_format=torch.contiguous_format), k.shape[-2]
+        hk, hko = _heads("rope", k), _heads("rope", ko)
+    B, T = (shape[0], shape[1]) if len(shape) == 4 else (1, shape[0])
+    _launch("bs_rope", index, _heads("rope", q), hk, _heads("rope", qo), hko, _DT[q.dtype], B, T, shape[-2], Hk,
+            shape[-1], table.data_ptr(), table.shape[0], 2 * table.shape[1], positions.data_ptr(),
+            _DT[positions.dtype], interleaved, inverse)
     return qo, ko
 
 

@@ -167,3 +167,25 @@ def test_oracle_agrees_with_torch_on_plain_attention():
 
 def test_library_declares_the_structs_it_is_given():
     assert ctypes.sizeof(_lib.Heads) == 32 and ctypes.sizeof(_lib.KVCache) == 17 * 8
+
+
+def test_attention_layer_has_the_parameters_of_transformers():
+    hf = pytest.importorskip("transformers.models.gpt_oss.modeling_gpt_oss")
+    cfg = pytest.importorskip("transformers").GptOssConfig(num_hidden_layers=2)
+    for i in range(2):
+        with torch.device("meta"):
+            theirs = {n: tuple(p.shape) for n, p in hf.GptOssAttention(cfg, i).named_parameters()}
+        ours = attention.B200GptOssAttention(cfg, i)
+        assert {n: tuple(p.shape) for n, p in ours.named_parameters()} == theirs
+        assert all(p.is_meta for p in ours.parameters())
+        assert ours.window == (cfg.sliding_window if cfg.layer_types[i] == "sliding_attention" else 0)
+
+
+def test_cpu_tensors_are_refused():
+    from blockstreamer_b200 import kernels
+    x = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        kernels.rope(x, None, torch.zeros(4, 32, 2), torch.zeros(1, 1, dtype=torch.int32))
+    with pytest.raises(ValueError, match="CUDA tensors only"):
+        kernels.tree_attention(x, x, x, torch.zeros(1, 1, dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
+                               torch.zeros(1, 1, dtype=torch.int32))
