@@ -26,8 +26,9 @@ int paged_cache(const char* fn, const bs_kv_cache* c, int64_t extra, bool need_v
   BS_ARG(c->k && (c->v || !need_v) && c->page_table && c->lens, "%s: null pointer in the cache", fn);
   BS_ARG(c->pages > 0 && c->page_size > 0 && c->heads > 0 && c->table_width > 0 && c->batch >= 0, "%s: bad cache sizes", fn);
   BS_ARG(c->dim > 0 && c->dim <= 128 && c->dim % 8 == 0, "%s: the head size must be a multiple of 8 up to 128", fn);
+  // (slots and their sums with a tile stay below 2^31)
   BS_ARG(c->pages < INT32_MAX && c->page_size < INT32_MAX && c->heads <= 65535 && c->batch < (1 << 24) &&
-             c->table_width * c->page_size < INT32_MAX && c->table_stride >= 0,
+             c->table_width * c->page_size < INT32_MAX - (1 << 16) && c->table_stride >= 0,
          "%s: cache sizes too large", fn);
   BS_ARG(extra >= 0 && extra <= c->table_width * c->page_size, "%s: more drafted tokens than slots in a table row", fn);
   BS_ALIGNED16(c->k, "the key cache");
@@ -76,6 +77,11 @@ int cache_maps(const bs_kv_cache* c, int rows, bool need_v, CacheMaps* o) {
 namespace {
 
 constexpr int kMaxDrafts = 256;
+// Up to so many keys an item is not cut.  At one sequence, one token and 8 kv heads:
+// 250 keys 9.5 us on the device in one launch, 10.2 cut and joined; 516 keys 11.8
+// and 10.3, but 21 and 24 us where the host launches; 900 keys 17.0 and 11.7.
+// 64 sequences with a window of 128: 18.1 and 21.5.
+constexpr int kWholeKeys = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -97,10 +103,13 @@ struct TreeArgs : SplitArgs {
 // Row tiles of MT * 16 rows on mma.sync, four warps per CTA, each streaming its
 // own units of kU keys into its own ring (no barrier between warps) and holding
 // its own (m, z, O); they meet at the end of an item.  HBM-bound: two CTAs per SM
-// keep ~190 KB per SM in flight.
-// kTma: a unit is fetched by a few TMA boxes (pages of a multiple of 8 slots);
-// else by 16-byte asynchronous copies, whose address arithmetic and issue then
-// are most of the kernel's instructions.
+// keep ~190 KB per SM in flight.  64 sequences of up to 8192 keys, 64 / 8 heads of
+// 64: 91 us, 5.9 TB/s (90% of the measured copy rate); 2 x 131072 keys: 100 us
+// where a head's slots lie together in a page, 113 us where heads are interleaved
+// (128 bytes in every KB).
+// kTma: a unit is fetched by a few TMA boxes (pages of a multiple of 8 slots); else
+// by 16-byte asynchronous copies, whose address arithmetic and issue are most of
+// the kernel's instructions then (187 us for the 64 sequences).
 template <int DP>
 struct RowsCfg {
   static constexpr int kU = DP == 64 ? 32 : 16;
@@ -497,20 +506,28 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
 // Row tiles of 128 on tcgen05: S = Q K^T (128 x 64 per half tile of keys, both
 // operands in shared memory) into tensor memory, the weights P = 2^(x - m) back
 // into the same columns as bf16, O += P V with P as the tensor-memory operand and
-// V as it lies in the cache (keys along K, the head contiguous).  Two half tiles
-// of S alternate, so that the next one is ready when a softmax step ends.
+// V as it lies in the cache (keys along K, the head contiguous).
 //
-// Two pipelines per CTA, each two groups of four softmax warps (a thread per row;
-// the groups take alternate half tiles) and an MMA warp.  Four softmax warps to a
-// scheduler hide each other's latencies: with one group per pipeline a scheduler
-// issued in 45% of its cycles.  With more than 128 rows to a kv head (kPair) they take two
-// row tiles and share every K and V tile; with fewer they take alternate tiles
-// of keys for the same rows and meet at the end of an item, where both read both
-// accumulators (same lanes of tensor memory).  One more warp fetches K and V by
-// TMA boxes of a page's slots into a ring of tiles.
+// Two pipelines per CTA.  With more than 128 rows to a kv head (kPair) they take two
+// row tiles and share every K and V tile; with fewer they take alternate tiles of
+// keys for the same rows, and both accumulators are read at the end of an item (same
+// lanes of tensor memory).  A pipeline has two (heads of 128) or three (heads of 64)
+// half tiles of S in tensor memory, so that products run ahead of the softmax; two
+// groups of four softmax warps, a thread per row, that take its half tiles in turn;
+// and a warp each that issues S and PV products.  One warp fetches K and V by TMA
+// boxes of a page's slots into a ring of tiles.
 //
-// The running maximum is only moved when a row's scores exceed it by 2^8: P stays
-// far below the bf16 range, sums are fp32, and the accumulator is rarely rescaled.
+// The groups of a pipeline settle a row's reference m half tile by half tile, in
+// turn, through shared memory.  It only moves when a row's scores exceed it by 2^8:
+// P stays far below the bf16 range, sums are fp32, and O is rarely rescaled.
+//
+// What bounds it: the softmax warps' issue slots and the special-function unit (16
+// exponentials per clock and SM).  Steps that paid, 2 x 131072 keys, 16 drafts, heads
+// of 64 (128 rows) / 8 x 16384 keys, 64 drafts, heads of 128, us: 16-byte
+// copies 257 / 257; TMA boxes 170 / 246; products issued from a converged warp 136 /
+// 202; half tiles of S ahead 125 / 156; starts of items counted in the split - / 110;
+// two softmax groups and two issuing warps per pipeline 125 / 85; registers moved to
+// the softmax warps, no spills 107 / 80.  82 and 37 us are the floors.
 template <int DP>
 struct TilesCfg {
   static constexpr int kSlot = 128 * DP * 2;             // a K or V tile, [DP / 64] panels of 128 rows x 128 bytes
@@ -530,7 +547,10 @@ constexpr int kTileThreads = 768;  // 16 softmax warps, loader, four issuing war
 // eight warps give it (512 * 96 + 256 * 48 = 768 * 80).
 constexpr int kSoftmaxRegs = 96, kOtherRegs = 48;
 constexpr float kRescale = 8.f;
-constexpr int kPolyOf = 8;  // one pair of exponentials in so many runs on the FMA pipe (none 136 us, 1/8 130, 1/4 132 at 2 x 131072 keys, 16 drafts)
+// One pair of exponentials in so many runs on the FMA pipe.  2 x 131072 keys, 16
+// drafts, heads of 64: 1/16 116.8 us, 1/8 117.2, 1/4 118.9; 8 x 16384 keys, 64
+// drafts, heads of 128: 92.0, 90.3, 89.2.
+constexpr int kPolyOf = 8;
 
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort));
@@ -1116,7 +1136,7 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
   before = sums[0] + sums[1] + sums[2] + sums[3];
   total = sums[4] + sums[5] + sums[6] + sums[7];
   const int64_t units = units_of<kU>(a, b);
-  const int64_t chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
+  const int64_t chunk = chunk_of(a, total, grid);
   const int64_t s = before + item * units, e = s + units;
   const int c0 = (int)((s + a.setup) / chunk), c1 = (int)((e - 1) / chunk);
   const int dim = a.c.dim, row0 = tile * kRows, rows = min(kRows, a.R - row0);
@@ -1168,6 +1188,7 @@ int tile_rows(int64_t R, int64_t D, bool tma) {
 
 template <int kU, int kRows>
 int launch_join(const TreeArgs& a, int grid, cudaStream_t st) {
+  if (a.fixed) return BS_OK;  // no item is cut
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.tiles), (unsigned)cdiv(std::min(kRows, a.R), kJoinRows));
   cfg.blockDim = dim3(128);
@@ -1276,6 +1297,10 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * (D / 4));
   a.min_chunk = rows <= 32 ? 4 : 2;
   a.setup = rows <= 32 ? 16 : 8;
+  // short ranges of keys (a window, a small cache): whole items to the CTAs, and no second launch
+  const int unit = rows > 32 ? 128 : D <= 64 ? RowsCfg<64>::kU : RowsCfg<128>::kU;
+  const int64_t reach = a.window ? std::min<int64_t>((int64_t)a.window - 1 + a.T + a.box - 1, a.c.capacity) : a.c.capacity;
+  if (reach <= kWholeKeys) a.fixed = (int)cdiv(reach, (int64_t)unit);
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   CacheMaps maps = {};

@@ -73,6 +73,7 @@ struct SplitArgs {
   int box;               // slots of a TMA box, or 1
   int setup;             // what starting an item costs, in units: it is counted as so many more
   int min_chunk;         // units of a CTA at least
+  int fixed;             // not 0: every item counts as so many units and no CTA's range cuts one
 };
 
 // The keys of a sequence: n committed; slots [low, hi) may be attended; units
@@ -104,8 +105,13 @@ struct Range {
 };
 template <int kU>
 __device__ __forceinline__ int64_t units_of(const SplitArgs& a, int b) {
+  if (a.fixed) return a.fixed;
   const Keys k = keys_of(a, b);
   return a.setup + (k.hi - k.lo + kU - 1) / kU;
+}
+__device__ __forceinline__ int64_t chunk_of(const SplitArgs& a, int64_t total, int grid) {
+  const int64_t chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
+  return a.fixed ? (chunk + a.fixed - 1) / a.fixed * a.fixed : chunk;
 }
 __device__ __forceinline__ void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 template <int kU>
@@ -141,7 +147,7 @@ __device__ Range locate(const SplitArgs& a, int cta, int grid, int64_t* sums /* 
     run += sums[0] + sums[1] + sums[2] + sums[3];
     if (base == 0) {
       if (a.B <= 128) total = run;
-      r.chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
+      r.chunk = chunk_of(a, total, grid);
       r.p0 = min(total, cta * r.chunk);
       r.p1 = min(total, r.p0 + r.chunk);
       if (r.p0 >= r.p1) return r;
@@ -170,9 +176,10 @@ struct Walk {
 template <int kU>
 __device__ __forceinline__ bool walk_piece(const SplitArgs& a, Walk& w, int first) {
   w.units = (w.k.hi - w.k.lo + kU - 1) / kU;
-  w.len = (int)min((int64_t)(w.units + a.setup - first), w.left);
-  w.start = max(0, first - a.setup);
-  w.end = max(0, first + w.len - a.setup);
+  const int lead = a.fixed ? a.fixed - w.units : a.setup;
+  w.len = (int)min((int64_t)(w.units + lead - first), w.left);
+  w.start = max(0, first - lead);
+  w.end = max(0, first + w.len - lead);
   return w.end > w.start;
 }
 // The next piece of the range; false at its end.
@@ -196,7 +203,7 @@ template <int kU>
 __device__ __forceinline__ bool walk_begin(const SplitArgs& a, const Range& r, Walk& w) {
   w.b = r.b;
   w.k = keys_of(a, r.b);
-  const int64_t units = a.setup + (w.k.hi - w.k.lo + kU - 1) / kU;
+  const int64_t units = units_of<kU>(a, r.b);
   const int64_t rel = r.p0 - r.before;
   const int item = (int)(rel / units);
   w.h = item / a.tiles;

@@ -8,7 +8,9 @@
 // HBM-bound: each value is read and written once (one table row of rot * 4
 // bytes per token beside the heads' Hq + Hk rows).  A group of threads takes one
 // token, each thread the same 16-byte column of several heads, so that a
-// thread's cosines and sines are loaded once per token.
+// thread's cosines and sines are loaded once per token; the loads of three heads
+// are in flight together (8192 tokens, 64 + 8 heads of 64: 36 us one after the
+// other, 28.5 us so, 5.3 TB/s or 81% of the measured copy rate).
 #include "bs_paged.cuh"
 
 namespace bs {

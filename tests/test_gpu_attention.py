@@ -230,6 +230,66 @@ def test_tree_attention(T, Hq, Hkv, D, page, lens, window, sinks, tree, head_maj
     check_attention(q, kc, vc, table, L, pos, mask, s, window)
 
 
+MORE_ROWS = [
+    # rows to a kv head: 24 and 32; 165, 200, 384 and 512 (pairs of row tiles, the last half empty)
+    (2, 12, 1, 64, 16, [70, 0], 0, True, "each"),
+    (4, 8, 1, 32, 8, [129, 64], 0, False, "each"),
+    (33, 40, 8, 128, 16, [140], 0, True, "each"),
+    (40, 10, 2, 128, 8, [3, 200], 0, False, "shared"),
+    (64, 24, 4, 128, 32, [127], 60, True, "each"),
+    (128, 4, 1, 64, 64, [65, 0], 0, True, "chain"),
+]
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,page,lens,window,sinks,tree", ATTENTION + MORE_ROWS)
+def test_tree_attention_with_its_keys_cut(T, Hq, Hkv, D, page, lens, window, sinks, tree):
+    """The same with a page table that reaches far: the keys may then be cut into pieces of
+    several CTAs and joined (without a window), however few there are."""
+    kc, vc, table, L, g = make_cache(lens, T, Hkv, D, page, T + D)
+    mask, pos = make_tree(len(lens), T, lens, g, unused=min(3, T - 1))
+    if tree == "chain":
+        mask, pos = None, torch.where(pos >= 0, L[:, None] + torch.arange(T), -1).to(torch.int32)
+    if tree == "shared":
+        mask = mask[0]
+        pos = torch.where(pos >= 0, L[:, None] + mask.sum(-1) - 1, -1).to(torch.int32)
+    poison_unused(kc, table, L, pos)
+    poison_unused(vc, table, L, pos)
+    table = torch.cat([table, torch.zeros(len(lens), 5000 // page + 1, dtype=torch.int32)], 1)
+    q = (torch.randn(len(lens), T, Hq, D, generator=g) * 2).bfloat16()
+    s = torch.randn(Hq, generator=g) if sinks else None
+    check_attention(q, kc, vc, table, L, pos, mask, s, window)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,page,lens,window,sinks,tree", MORE_ROWS)
+def test_tree_attention_of_more_rows(T, Hq, Hkv, D, page, lens, window, sinks, tree):
+    kc, vc, table, L, g = make_cache(lens, T, Hkv, D, page, T + D, head_major=True)
+    mask, pos = make_tree(len(lens), T, lens, g, unused=1)
+    poison_unused(kc, table, L, pos)
+    poison_unused(vc, table, L, pos)
+    q = (torch.randn(len(lens), T, Hq, D, generator=g) * 2).bfloat16()
+    s = torch.randn(Hq, generator=g) if sinks else None
+    check_attention(q, kc, vc, table, L, pos, mask, s, window)
+
+
+@pytest.mark.parametrize("T,Hq,Hkv,D,scale", [(20, 8, 1, 64, 30.0), (40, 8, 1, 128, 30.0), (20, 8, 1, 64, -3.0), (1, 8, 1, 64, -3.0)])
+def test_rows_whose_maximum_keeps_moving(T, Hq, Hkv, D, scale):
+    """Scores of hundreds that grow along the keys: the reference moves, and the sums and
+    outputs that were relative to it are rescaled; negative scales too.  The weights are
+    taken against fp32 scores, which are off by up to 2^-24 D max|q k| scale here."""
+    n, page = 700, 16
+    kc, vc, table, L, g = make_cache([n], T, Hkv, D, page, 3)
+    for j in range(n + T):
+        kc[int(table[0, j // page]), j % page] *= 0.02 + 0.98 * j / n
+    pos = (L[:, None] + torch.arange(T)).to(torch.int32)
+    q = torch.randn(1, T, Hq, D, generator=g).bfloat16()
+    want, lse, spread = oatt.tree_attention(q, kc, vc, table, L, pos, scale=scale / D ** 0.5)
+    got, glse = kernels.tree_attention(*to(q, kc, vc, table, L, pos), scale=scale / D ** 0.5)
+    off = 2.0 ** -24 * D * 16 * abs(scale) / D ** 0.5 * 4      # |q k| of single products up to 16, sums in fp32
+    tol = (2.0 ** -8 + 2 * off) * (want.abs() + spread) + 1e-6
+    assert bool(((got.double().cpu() - want).abs() <= tol).all())
+    assert bool(((glse.double().cpu() - lse).abs() <= off + 1e-6 * lse.abs()).all())
+
+
 def test_rows_that_attend_nothing():
     """A token whose mask is empty, with and without sinks; unused tokens; a whole sequence of them."""
     T, lens = 4, [0, 0, 5]
