@@ -321,10 +321,10 @@ int scores_launch(ScoreArgs a, const CacheMaps& maps, cudaStream_t st) {
 // ---------------------------------------------------------------- eviction
 // Selection: one cluster per (sequence, kv head), each CTA a contiguous range
 // of its slots, whose scores it holds in shared memory as unsigned keys of the
-// same order.  A radix selection over four 8-bit digits (histograms joined
-// through distributed shared memory) finds the key of the last kept slot and
-// how many slots of that very key are kept; a scan then writes the kept slots
-// in order.  Protected slots get the highest key, NaN the lowest.
+// same order.  A radix selection over digits of 11, 11 and 10 bits (histograms
+// joined through distributed shared memory) finds the key of the last kept slot
+// and how many slots of that very key are kept; a scan then writes the kept
+// slots in order.  Protected slots get the highest key, NaN the lowest.
 struct EvictArgs {
   PagedCache c;
   const float* scores;
@@ -333,6 +333,8 @@ struct EvictArgs {
   int32_t* out_lens;
   float* out_scores;
   int capacity, budget, first, last, out_width, out_capacity, held;  // held: keys a CTA has room for
+  int vec;    // scores of a (sequence, kv head) start on 16 bytes
+  int chunk;  // rows a CTA of the move takes
 };
 
 __device__ __forceinline__ uint32_t score_key(float x) {
@@ -341,147 +343,191 @@ __device__ __forceinline__ uint32_t score_key(float x) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSel = 512;  // threads of a selection CTA
+constexpr int kMoveRows = 256;
+constexpr int kSel = 512;         // threads of a selection CTA
+constexpr int kBins = 4 * kSel;   // of an 11-bit digit
 
 __device__ __forceinline__ uint32_t dsmem_u32(uint32_t addr, uint32_t rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(ptx::mapa(addr, rank)) : "memory");
   return v;
 }
+__device__ __forceinline__ uint4 dsmem_u4(uint32_t addr, uint32_t rank) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(ptx::mapa(addr, rank)) : "memory");
+  return v;
+}
 
-__global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__ EvictArgs a, int cluster) {
+// kFits: shared memory holds the CTA's keys (and those of the first digit once more);
+// longer ranges are read again for every digit.
+template <int kCluster, bool kFits>
+__global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__ EvictArgs a) {
   extern __shared__ __align__(16) uint32_t held[];
-  __shared__ uint32_t hist[2][256];
+  __shared__ __align__(16) uint32_t hist[2][kBins];
   __shared__ uint32_t found[2], totals[2], warps[2][kSel / 32];
-  const int rank = blockIdx.x % cluster, item = blockIdx.x / cluster;
+  const int rank = blockIdx.x % kCluster, item = blockIdx.x / kCluster;
   const int b = item / a.c.heads;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int n = min(a.c.len(b, 0), a.capacity);
   const int want = min(n, a.budget);
   const float* scores = a.scores + (int64_t)item * a.capacity;
-  // this CTA's slots [s0, s1)
-  const int per = ((n + cluster - 1) / cluster + 3) / 4 * 4;
-  const int s0 = min(n, rank * per), s1 = min(n, s0 + per), mine = s1 - s0;
+  // this CTA's slots [s0, s0 + mine)
+  const int per = ((n + kCluster - 1) / kCluster + 3) / 4 * 4;
+  const int s0 = min(n, rank * per), mine = min(n, s0 + per) - s0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  // each warp takes a contiguous run of slots, 32 at a time
-  const int run = ((mine + kSel / 32 - 1) / (kSel / 32) + 31) / 32 * 32;
-  const int w0 = min(mine, warp * run), steps = (min(mine, w0 + run) - w0 + 31) / 32;
-  const bool fits = per <= a.held;
+  // each warp takes a contiguous run of slots [w0, w1), 128 at a time: four neighbours a lane
+  const int run = ((mine + kSel / 32 - 1) / (kSel / 32) + 127) / 128 * 128;
+  const int w0 = min(mine, warp * run), w1 = min(mine, w0 + run), steps = (w1 - w0 + 127) / 128;
   auto key_of = [&](int s, float x) -> uint32_t { return s < a.first || s >= n - a.last ? 0xffffffffu : score_key(x); };
-  if (fits) {
-    // eight loads of a lane in flight; the loops stay short, since each is run once
-    // and its instructions come from memory too
-    for (int j = 0; j < steps; j += 8) {
-      float x[8];
+  auto load4 = [&](int i) -> float4 {  // scores of four slots, some perhaps behind the last
+    const int s = s0 + i, top = a.capacity - 1;
+    if (a.vec) return __ldg(reinterpret_cast<const float4*>(scores + min(s, top - 3)));
+    return make_float4(__ldg(scores + min(s, top)), __ldg(scores + min(s + 1, top)), __ldg(scores + min(s + 2, top)),
+                       __ldg(scores + min(s + 3, top)));
+  };
+  auto keys4 = [&](int i, float4 x) -> uint4 {
+    return make_uint4(key_of(s0 + i, x.x), key_of(s0 + i + 1, x.y), key_of(s0 + i + 2, x.z), key_of(s0 + i + 3, x.w));
+  };
+  if (kFits) {
+    for (int j = 0; j < steps; j += 4) {
+      float4 x[4];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = __ldg(scores + min(s0 + w0 + (j + e) * 32 + lane, a.capacity - 1));
+      for (int e = 0; e < 4; ++e) x[e] = load4(w0 + (j + e) * 128 + lane * 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int i = w0 + (j + e) * 32 + lane;
-        if (j + e < steps) held[i] = key_of(s0 + i, x[e]);
+      for (int e = 0; e < 4; ++e) {
+        const int i = w0 + (j + e) * 128 + lane * 4;
+        if (j + e < steps) *reinterpret_cast<uint4*>(held + i) = keys4(i, x[e]);
       }
     }
-    __syncwarp();
   }
-  // f(slot of this lane or -1, its key) for every step of the warp
+  // f(first of the lane's four slots, how many of them there are, their keys) for every
+  // step of the warp; a lane sees only what it wrote
   auto walk = [&](auto&& f) {
-    const int last = min(mine, w0 + run);
-#pragma unroll 4
-    for (int j = 0; j < steps; ++j) {
-      const int i = w0 + j * 32 + lane, c = min(i, last - 1);
-      const uint32_t k = fits ? held[c] : key_of(s0 + c, scores[s0 + c]);
-      f(i < last ? s0 + i : -1, i < last ? k : 0u);
+    constexpr int kAtOnce = kFits ? 1 : 4;
+#pragma unroll 1
+    for (int j = 0; j < steps; j += kAtOnce) {
+      const int i = w0 + j * 128 + lane * 4;
+      uint4 v[kAtOnce];
+      if constexpr (kFits) {
+        v[0] = *reinterpret_cast<const uint4*>(held + i);
+      } else {
+        float4 x[kAtOnce];
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e) x[e] = load4(i + e * 128);
+#pragma unroll
+        for (int e = 0; e < kAtOnce; ++e) v[e] = keys4(i + e * 128, x[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < kAtOnce; ++e) {
+        const uint32_t k[4] = {v[e].x, v[e].y, v[e].z, v[e].w};
+        if (j + e < steps) f(s0 + i + e * 128, w1 - i - e * 128, k);
+      }
     }
   };
 
   const uint32_t below = (1u << lane) - 1u;
   uint32_t* match = held + a.held;
   int matches = 0;
-  uint32_t gt = 0, eq = 0;  // this warp's keys above the chosen one, and equal to it
+  uint32_t gt = 0, eq = 0;  // this lane's keys above the chosen one, and equal to it
   uint32_t prefix = 0, mask = 0;
   int need = want;  // slots still to choose among those whose key matches prefix
   if (want < n) {
-    for (int pass = 0; pass < 4; ++pass) {
-      const int shift = 24 - 8 * pass;
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const uint32_t digit = pass == 2 ? 0x3ffu : 0x7ffu;
       uint32_t* hs = hist[pass & 1];
-      for (int i = threadIdx.x; i < 256; i += kSel) hs[i] = 0;
+      *reinterpret_cast<uint4*>(hs + 4 * threadIdx.x) = make_uint4(0, 0, 0, 0);
       __syncthreads();
       if (pass == 0) {
-        // sign and exponent: few digits, so a warp counts equal ones together
-        walk([&](int slot, uint32_t k) {
-          const uint32_t same = __match_any_sync(0xffffffffu, slot >= 0 ? k >> 24 : 256u);
-          if (slot >= 0 && lane == __ffs(same) - 1) atomicAdd(&hs[k >> 24], (uint32_t)__popc(same));
+        walk([&](int slot, int there, const uint32_t* k) {
+          const uint32_t d = __shfl_sync(0xffffffffu, k[0] >> 21, 0);
+          const bool one = there >= 4 && k[0] >> 21 == d && k[1] >> 21 == d && k[2] >> 21 == d && k[3] >> 21 == d;
+          if (__all_sync(0xffffffffu, one)) {  // untouched scores and protected slots: 128 of one digit
+            if (lane == 0) atomicAdd(&hs[d], 128u);
+            return;
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < there) atomicAdd(&hs[k[e] >> 21], 1u);
         });
-      } else if (fits) {
-        // the keys that still match, put together by each warp after the first digit;
-        // those above it are counted on the way
-        if (pass == 1) {
-          walk([&](int slot, uint32_t k) {
-            const bool on = slot >= 0 && (k & mask) == prefix;
+      } else if (!kFits) {
+        walk([&](int slot, int there, const uint32_t* k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < there && (k[e] & mask) == prefix) atomicAdd(&hs[k[e] >> shift & digit], 1u);
+        });
+      } else if (pass == 1) {
+        // the keys of the first digit, put together by each warp; those above it are counted
+        walk([&](int slot, int there, const uint32_t* k) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const bool on = e < there && (k[e] & mask) == prefix;
             const uint32_t m = __ballot_sync(0xffffffffu, on);
-            gt += __popc(__ballot_sync(0xffffffffu, slot >= 0 && (k & mask) > prefix));
-            if (on) match[w0 + matches + __popc(m & below)] = k;
+            gt += e < there && (k[e] & mask) > prefix;
+            if (on) {
+              match[w0 + matches + __popc(m & below)] = k[e];
+              atomicAdd(&hs[k[e] >> shift & digit], 1u);
+            }
             matches += __popc(m);
-          });
-          __syncwarp();
-        }
-        const uint32_t digit = shift == 16 ? 0u : 255u << (shift + 8);  // the last digit found
-        for (int j = 0; j < matches; j += 32) {
-          const uint32_t k = match[w0 + min(j + lane, matches - 1)];
-          const bool on = j + lane < matches, now = on && (k & mask) == prefix;
-          // among keys that matched before the last digit, those above it
-          if (pass > 1)
-            gt += __popc(__ballot_sync(0xffffffffu, on && ((k ^ prefix) & (mask & ~digit)) == 0 && (k & digit) > (prefix & digit)));
-          if (now) atomicAdd(&hs[k >> shift & 255], 1u);
-        }
-      } else {
-        walk([&](int slot, uint32_t k) {
-          if (slot >= 0 && (k & mask) == prefix) atomicAdd(&hs[k >> shift & 255], 1u);
+          }
         });
+        __syncwarp();
+      } else {
+        for (int j = lane; j < matches; j += 32) {
+          const uint32_t k = match[w0 + j];
+          if ((k & mask) == prefix) atomicAdd(&hs[k & digit], 1u);
+        }
       }
       ptx::cluster_sync();
-      // every CTA finds the digit whose bin holds the need-th highest key: a thread
-      // per bin from the top, a scan, and the one thread whose bin it is
-      uint32_t bin = 0;
-      if (threadIdx.x < 256)
-        for (int r = 0; r < cluster; ++r) bin += dsmem_u32(ptx::smem_addr(&hs[255 - threadIdx.x]), r);
-      uint32_t incl = bin;
+      // every CTA finds the digit whose bin holds the need-th highest key: a thread to
+      // four bins from the top, a scan, and the one thread whose bin it is
+      uint4 bin = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        const uint4 v = dsmem_u4(ptx::smem_addr(hs + kBins - 4 - 4 * threadIdx.x), r);
+        bin.x += v.x, bin.y += v.y, bin.z += v.z, bin.w += v.w;
+      }
+      const uint32_t sum = bin.x + bin.y + bin.z + bin.w;
+      uint32_t incl = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
         if (lane >= o) incl += v;
       }
-      if (lane == 31 && warp < 8) warps[0][warp] = incl;
+      if (lane == 31) warps[0][warp] = incl;
       __syncthreads();
-      if (threadIdx.x < 256) {
-        uint32_t above = incl - bin;
-        for (int w = 0; w < warp; ++w) above += warps[0][w];
-        if (above < (uint32_t)need && (uint32_t)need <= above + bin) found[0] = 255 - threadIdx.x, found[1] = need - above;
+      uint32_t above = incl - sum;
+#pragma unroll
+      for (int w = 0; w < kSel / 32; ++w) above += w < warp ? warps[0][w] : 0u;
+      if (above < (uint32_t)need && (uint32_t)need <= above + sum) {
+        uint32_t d = kBins - 1 - 4 * threadIdx.x, left = need - above, in = bin.w;
+        if (left > in) left -= in, in = bin.z, --d;
+        if (left > in) left -= in, in = bin.y, --d;
+        if (left > in) left -= in, --d;
+        found[0] = d, found[1] = left;
       }
       __syncthreads();
       prefix |= found[0] << shift;
-      mask |= 255u << shift;
+      mask |= digit << shift;
       need = found[1];
       // the other histogram is next: its readers passed the last cluster_sync
     }
   }
   // key == prefix: the first `need` in slot order are kept; key > prefix: all
   const bool all = want == n;
-  if (all) {
-    gt = max(0, min(mine, w0 + run) - w0);
-  } else if (fits) {
-    for (int j = 0; j < matches; j += 32) {
-      const uint32_t k = match[w0 + min(j + lane, matches - 1)];
-      const bool near = j + lane < matches && ((k ^ prefix) & 0xffffff00u) == 0;  // all but the last digit
-      gt += __popc(__ballot_sync(0xffffffffu, near && k > prefix));
-      eq += __popc(__ballot_sync(0xffffffffu, near && k == prefix));
+  if (!all && kFits) {
+    for (int j = lane; j < matches; j += 32) {
+      const uint32_t k = match[w0 + j];
+      gt += k > prefix, eq += k == prefix;
     }
-  } else {
-    walk([&](int slot, uint32_t k) {
-      gt += __popc(__ballot_sync(0xffffffffu, slot >= 0 && k > prefix));
-      eq += __popc(__ballot_sync(0xffffffffu, slot >= 0 && k == prefix));
+  } else if (!all) {
+    walk([&](int slot, int there, const uint32_t* k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) gt += e < there && k[e] > prefix, eq += e < there && k[e] == prefix;
     });
   }
+  gt = all ? w1 - w0 : __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
   __syncthreads();
   if (lane == 0) warps[0][warp] = gt, warps[1][warp] = eq;
   __syncthreads();
@@ -498,68 +544,138 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
     bg += dsmem_u32(ptx::smem_addr(&totals[0]), r);
     be += dsmem_u32(ptx::smem_addr(&totals[1]), r);
   }
+  // nobody leaves while its shared memory may be read: the wait stands at the end
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   int32_t* kept = a.kept + (int64_t)item * a.budget;
   float* out = a.out_scores + (int64_t)item * a.out_capacity;
-  walk([&](int slot, uint32_t k) {
-    const bool more = slot >= 0 && (all || k > prefix), same = slot >= 0 && !all && k == prefix;
-    const uint32_t mg = __ballot_sync(0xffffffffu, more), me = __ballot_sync(0xffffffffu, same);
-    const uint32_t eq0 = be + __popc(me & below);
-    if (more || (same && eq0 < (uint32_t)need)) {
-      const uint32_t at = bg + __popc(mg & below) + min(eq0, (uint32_t)need);
-      kept[at] = slot;
-      // the key gives the score back, but for protected slots and NaN
-      if (at < (uint32_t)a.out_capacity)
-        out[at] = k == 0xffffffffu || k == 0u ? scores[slot] : __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+  walk([&](int slot, int there, const uint32_t* k) {
+    uint32_t count = 0;  // of keys above, and equal ones in the upper half
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < there) count += all || k[e] > prefix ? 1u : k[e] == prefix ? 0x10000u : 0u;
+    uint32_t incl = count;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += v;
     }
-    bg += __popc(mg);
-    be += __popc(me);
+    uint32_t g = bg + (incl - count & 0xffffu), q = be + (incl - count >> 16);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bool more = e < there && (all || k[e] > prefix), same = e < there && !all && k[e] == prefix;
+      if (more || (same && q < (uint32_t)need)) {
+        const uint32_t at = g + min(q, (uint32_t)need);
+        kept[at] = slot + e;
+        // the key gives the score back, but for protected slots and NaN
+        if (at < (uint32_t)a.out_capacity)
+          out[at] = k[e] == 0xffffffffu || k[e] == 0u ? scores[slot + e]
+                                                      : __uint_as_float(k[e] & 0x80000000u ? k[e] ^ 0x80000000u : ~k[e]);
+      }
+      g += more, q += same;
+    }
+    const uint32_t total = __shfl_sync(0xffffffffu, incl, 31);
+    bg += total & 0xffffu, be += total >> 16;
   });
   // behind the kept slots: -1 and zero scores
-  for (int i = want + rank * kSel + threadIdx.x; i < a.budget; i += cluster * kSel) kept[i] = -1;
-  for (int i = want + rank * kSel + threadIdx.x; i < a.out_capacity; i += cluster * kSel) out[i] = 0.f;
+  for (int i = want + rank * kSel + threadIdx.x; i < a.budget; i += kCluster * kSel) kept[i] = -1;
+  for (int i = want + rank * kSel + threadIdx.x; i < a.out_capacity; i += kCluster * kSel) out[i] = 0.f;
   if (threadIdx.x == 0 && rank == 0 && item % a.c.heads == 0) {
     a.out_lens[b] = want;
     if (want > a.out_capacity) record_status(a.c.status, BS_ERR_CAPACITY);
   }
-  ptx::cluster_sync();  // nobody leaves while its shared memory may be read
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// Copies the kept rows: kLanes lanes per row, four rows of each in flight.
+constexpr int kHeldMost = 24 * 1024;  // keys
+static_assert(kHeldMost * 8 + sizeof(uint32_t) * 2 * kBins + 1024 <= 227 * 1024, "shared memory of a CTA");
+
+template <int kCluster, bool kFits>
+int select_launch(EvictArgs a, int items, cudaStream_t st) {
+  static bool set[64] = {};
+  int dev = 0;
+  BS_CUDA(cudaGetDevice(&dev));
+  if (kFits && (dev >= 64 || !set[dev])) {
+    BS_CUDA(cudaFuncSetAttribute(kv_select_kernel<kCluster, kFits>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kHeldMost * 8));
+    if (dev < 64) set[dev] = true;
+  }
+  const int per = (int)cdiv((int64_t)a.capacity, (int64_t)kCluster);
+  a.held = kFits ? (int)((per + 3) / 4 * 4 + 127) / 128 * 128 : 0;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3((unsigned)items * kCluster);
+  cfg.blockDim = dim3(kSel);
+  cfg.dynamicSmemBytes = (size_t)a.held * 8;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = kCluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  BS_CUDA(cudaLaunchKernelEx(&cfg, kv_select_kernel<kCluster, kFits>, a));
+  return BS_OK;
+}
+
+template <int kCluster>
+int select_of(const EvictArgs& a, int items, cudaStream_t st) {
+  return cdiv((int64_t)a.capacity, (int64_t)kCluster) <= kHeldMost - 128 ? select_launch<kCluster, true>(a, items, st)
+                                                                       : select_launch<kCluster, false>(a, items, st);
+}
+
+// Copies the kept rows: a CTA looks up where its rows come from and go to, a row to a
+// thread, and then copies them, dim / 8 lanes to a row.  Neighbouring CTAs take the
+// heads of the same rows, which lie side by side in caches of interleaved heads.
+// HBM-bound: 8 dim bytes a kept row and head.  64 heads of 8192 kept rows, dim 64 (268 MB):
+// 50 us, 5.3 TB/s, where a plain copy reaches 6.6; lookups by every lane for its own four
+// rows took 60 us.  CTAs of 128 / 256 / 512 / 1024 rows: 83 / 81 / 85 / 93 us with the
+// selection, heads apart instead of neighbours 82.5.  Started early, while the selection
+// runs, its waiting CTAs slowed that by 5 us, so it starts when the selection ends.
 __global__ void __launch_bounds__(256) kv_move_kernel(const __grid_constant__ EvictArgs a) {
+  __shared__ int4 place[kMoveRows];  // page and slot in it, of the source and of the copy
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int lanes = a.c.dim <= 64 ? 8 : 16;
   const int c = threadIdx.x % lanes, at_once = 256 / lanes;
-  const int b = blockIdx.y / a.c.heads, h = blockIdx.y - b * a.c.heads;
-  const int rows = min(a.budget, a.out_capacity);
-  const int32_t* kept = a.kept + (int64_t)blockIdx.y * a.budget;
-  const bool col = c * 8 < a.c.dim;
-  uint4 kv[4], vv[4];
-  int64_t dk[4], dv[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int i = blockIdx.x * at_once * 4 + j * at_once + threadIdx.x / lanes;
-    const int s = i < rows ? kept[i] : -1;
-    dk[j] = -1;
-    if (s < 0 || !col) continue;
-    int page, row, opage, orow;
-    a.c.div.split(s, page, row);
-    a.c.div.split(i, opage, orow);
-    const int64_t p = a.c.page_of(b, page), q = a.out_table[(int64_t)b * a.out_width + opage];
-    if ((uint64_t)q >= (uint64_t)a.c.pages) {
-      record_status(a.c.status, BS_ERR_CAPACITY);
-      continue;
+  const int b = blockIdx.y, chunk = blockIdx.x / a.c.heads, h = blockIdx.x - chunk * a.c.heads;
+  const int i0 = chunk * a.chunk, rows = min(a.chunk, min(a.budget, a.out_capacity) - i0);
+  const int32_t* kept = a.kept + ((int64_t)b * a.c.heads + h) * a.budget;
+  for (int r = threadIdx.x; r < rows; r += 256) {
+    const int s = kept[i0 + r];
+    int4 at = make_int4(0, 0, -1, 0);
+    if (s >= 0) {
+      int page, opage;
+      a.c.div.split(s, page, at.y);
+      a.c.div.split(i0 + r, opage, at.w);
+      at.x = a.c.page_of(b, page);
+      at.z = a.out_table[(int64_t)b * a.out_width + opage];
+      if ((unsigned)at.z >= (unsigned)a.c.pages) {
+        record_status(a.c.status, BS_ERR_CAPACITY);
+        at.z = -1;
+      }
     }
-    kv[j] = *reinterpret_cast<const uint4*>(a.c.k + p * a.c.kp + row * a.c.ks + h * a.c.kh + c * 8);
-    vv[j] = *reinterpret_cast<const uint4*>(a.c.v + p * a.c.vp + row * a.c.vs + h * a.c.vh + c * 8);
-    dk[j] = q * a.c.kp + orow * a.c.ks + h * a.c.kh + c * 8;
-    dv[j] = q * a.c.vp + orow * a.c.vs + h * a.c.vh + c * 8;
+    place[r] = at;
   }
+  __syncthreads();
+  if (c * 8 >= a.c.dim) return;
+  __nv_bfloat16* k = a.c.k + h * a.c.kh + c * 8;
+  __nv_bfloat16* v = a.c.v + h * a.c.vh + c * 8;
+  for (int r0 = threadIdx.x / lanes; r0 < rows; r0 += 4 * at_once) {
+    uint4 kv[4], vv[4];
+    int4 at[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (dk[j] >= 0) {
-      *reinterpret_cast<uint4*>(a.c.k + dk[j]) = kv[j];
-      *reinterpret_cast<uint4*>(a.c.v + dv[j]) = vv[j];
+    for (int j = 0; j < 4; ++j) {
+      const int r = r0 + j * at_once;
+      at[j] = r < rows ? place[r] : make_int4(0, 0, -1, 0);
+      if (at[j].z < 0) continue;
+      kv[j] = *reinterpret_cast<const uint4*>(k + at[j].x * a.c.kp + at[j].y * a.c.ks);
+      vv[j] = *reinterpret_cast<const uint4*>(v + at[j].x * a.c.vp + at[j].y * a.c.vs);
     }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (at[j].z < 0) continue;
+      *reinterpret_cast<uint4*>(k + at[j].z * a.c.kp + at[j].w * a.c.ks) = kv[j];
+      *reinterpret_cast<uint4*>(v + at[j].z * a.c.vp + at[j].w * a.c.vs) = vv[j];
+    }
+  }
 }
 
 }  // namespace
@@ -660,38 +776,28 @@ extern "C" int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_
   a.out_width = (int)out_width, a.out_capacity = (int)(out_width * cache->page_size);
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  // CTAs per (sequence, kv head): 8192 scores each, up to eight CTAs
+  a.vec = capacity % 4 == 0 && reinterpret_cast<uintptr_t>(scores) % 16 == 0;
+  const int items = (int)(cache->batch * cache->heads);
+  // CTAs per (sequence, kv head): 4096 scores each, as long as all clusters run at once and
+  // leave each CTA its own SM.  With 1 / 2 / 4 / 8 of them, in us with the move:
+  //     8 items of 8192 scores 16.4 / 14.3 / 14.6 / 18.8, of 32768 57 / 24 / 20 / 22, of 131072 211 / 94 / 58 / 37;
+  //    64 items of 4096 19.8 / 18.9 / 24 / 61, of 32768 105 / 69 / 71 / 106, of 131072 300 / 178 / 169 / 222;
+  //   256 items of 8192 108 / 115 / 137 / 283.
   int cluster = 1;
-  while (cluster < 8 && (int64_t)cluster * 8192 < capacity) cluster *= 2;
-  const int64_t per = cdiv(cdiv(capacity, (int64_t)cluster), (int64_t)4) * 4;
-  constexpr int kHeldMost = 24 * 1024;  // keys, twice; longer ranges are read again for every digit
-  a.held = (int)(std::min<int64_t>(per, kHeldMost) + 31) / 32 * 32;
-  static bool set[64] = {};
-  int dev = 0;
-  BS_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !set[dev]) {
-    BS_CUDA(cudaFuncSetAttribute(kv_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kHeldMost * 8));
-    if (dev < 64) set[dev] = true;
-  }
+  while (cluster < 8 && cluster * 4096 < capacity && items * cluster * 2 <= sm_count()) cluster *= 2;
+  BS_TRY(cluster == 1 ? select_of<1>(a, items, st) : cluster == 2 ? select_of<2>(a, items, st)
+         : cluster == 4 ? select_of<4>(a, items, st) : select_of<8>(a, items, st));
+  const int64_t rows = std::min<int64_t>(budget, std::min<int64_t>(capacity, a.out_capacity));
+  a.chunk = kMoveRows;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
-  const unsigned items = (unsigned)(cache->batch * cache->heads);
-  cfg.gridDim = dim3(items * cluster);
-  cfg.blockDim = dim3(kSel);
-  cfg.dynamicSmemBytes = (size_t)a.held * 8;
-  cfg.stream = st;
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  BS_CUDA(cudaLaunchKernelEx(&cfg, kv_select_kernel, a, cluster));
-  const int rows = 4 * 256 / (cache->dim <= 64 ? 8 : 16);
-  cfg.gridDim = dim3((unsigned)cdiv(std::min<int64_t>(budget, std::min<int64_t>(capacity, a.out_capacity)), (int64_t)rows), items);
+  cfg.gridDim = dim3((unsigned)(cdiv(rows, (int64_t)a.chunk) * cache->heads), (unsigned)cache->batch);
   cfg.blockDim = dim3(256);
-  cfg.dynamicSmemBytes = 0;
+  cfg.stream = st;
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   BS_CUDA(cudaLaunchKernelEx(&cfg, kv_move_kernel, a));
   return BS_OK;
 }

@@ -575,6 +575,24 @@ def test_kv_evict(lens, budget, first, last, page, D, head_major):
     check_evict(lens, torch.zeros_like(scores), budget, first, last, page, D, head_major)
 
 
+@pytest.mark.parametrize("lens,budget,first,last", [
+    ([5000, 4097], 100, 4, 8),              # two CTAs of a cluster to an item, then four and eight
+    ([9001], 130, 0, 33),
+    ([17000, 16385, 3], 300, 5, 0),
+    ([25600, 24449] + [7] * 24, 90, 2, 9),  # more items than SMs / 2, scores not held
+    ([200001], 257, 4, 64),                 # nor by eight CTAs
+])
+def test_kv_evict_of_long_caches(lens, budget, first, last):
+    g = torch.Generator().manual_seed(len(lens))
+    cap = pages_for(max(lens), 64) * 64
+    scores = torch.randn(len(lens), 3, cap, generator=g)
+    scores[0, 1] = (scores[0, 1] * 3).round()       # runs of equal scores over all the CTAs
+    scores[0, 2] = scores[0, 2].clamp(max=0.25)     # the threshold itself is met by many
+    check_evict(lens, scores, budget, first, last, 64, 8)
+    if len(lens) == 1:                              # scores that start off 16 bytes, odd capacity
+        check_evict(lens, scores[:, :, :lens[0]], budget, first, last, 64, 8)
+
+
 def test_kv_evict_special_values():
     g = torch.Generator().manual_seed(6)
     scores = torch.randn(2, 2, 64, generator=g)
