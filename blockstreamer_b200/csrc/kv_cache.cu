@@ -1,6 +1,8 @@
 // Upkeep of the paged key/value cache between decoding steps: the accepted
 // drafts moved together, the attention weight that each cached key received
 // added to its score, and the keys of lowest score evicted.
+#include <type_traits>
+
 #include "bs_paged.cuh"
 
 namespace bs {
@@ -75,8 +77,10 @@ struct ScoreCfg {
   static int smem(int rows) { return q + rows * (DP * 2 + 8) + 1024; }
 };
 
+constexpr int kScoreThreads = 160;  // four warps of keys, and one that copies
+
 template <int DP, bool kTma>
-__global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ ScoreArgs a,
+__global__ void __launch_bounds__(kScoreThreads, 2) kv_scores_kernel(const __grid_constant__ ScoreArgs a,
                                                         const __grid_constant__ CacheMaps maps) {
   using Cfg = ScoreCfg<DP>;
   constexpr int kU = Cfg::kU, KS = DP / 16, MT = kU / 16, kMine = kU / 32;
@@ -93,15 +97,40 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
 
   if constexpr (kTma) {
     if (threadIdx.x == 0) abort_flag = 0;
-    if (lane == 0) {
+    if (lane == 0 && warp < 4) {
       for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_init(bar + 8 * s, 1);
       ptx::fence_mbar_init();
     }
   } else if (a.c.dim < DP) {
-    for (int i = threadIdx.x; i < 4 * Cfg::kWarpBytes / 16; i += 128)
+    for (int i = threadIdx.x; i < 4 * Cfg::kWarpBytes / 16; i += kScoreThreads)
       reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
+  if (warp == 4) {
+    // ---- behind an item's last unit scores are only copied: an equal share of the
+    // whole array for each CTA
+    if (a.out != a.scores) {
+      const int64_t all = (int64_t)a.B * a.Hkv * a.capacity, share = (all + gridDim.x - 1) / gridDim.x;
+      const int64_t end = min(all, (blockIdx.x + 1) * share);
+      int64_t from = blockIdx.x * share;
+      int item = (int)(from / a.capacity);
+      for (; from < end; ++item) {
+        const int64_t first = (int64_t)item * a.capacity, to = min(end, first + a.capacity);
+        const int n = a.c.len(item / a.Hkv, a.T) + a.T;
+        const int64_t begin = max(from, first + min(a.capacity, (n + kU - 1) / kU * kU));
+        for (int64_t i = begin + lane; i < to; i += 16 * 32) {
+          float v[16];
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] = a.scores[min(i + j * 32, all - 1)];
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (i + j * 32 < to) a.out[i + j * 32] = v[j];
+        }
+        from = to;
+      }
+    }
+    return;
+  }
   const Range r = locate<kU>(a, blockIdx.x, gridDim.x, reinterpret_cast<int64_t*>(smem + Cfg::sums));
   Walk lw, cw;
   bool more = r.p0 < r.p1 && walk_begin<kU>(a, r, lw);
@@ -172,48 +201,8 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
   const uint32_t qaddr = ptx::smem_addr(qs);
   const int mine = lane / 4 + (lane & 3) * 8;  // the slots of a unit that this lane stores: mine, mine + 32
 
-  // ---- behind an item's last unit scores are only copied: an equal share of the
-  // whole array for each CTA, while the first keys are on their way
-  if (a.out != a.scores) {
-    const int64_t all = (int64_t)a.B * a.Hkv * a.capacity, share = (all + gridDim.x - 1) / gridDim.x;
-    const int64_t end = min(all, (blockIdx.x + 1) * share);
-    for (int64_t from = blockIdx.x * share; from < end;) {
-      const int64_t item = from / a.capacity, first = item * a.capacity;
-      const int64_t to = min(end, first + a.capacity);
-      const int n = a.c.len(item / a.Hkv, a.T) + a.T;
-      const int64_t begin = max(from, first + min(a.capacity, (n + kU - 1) / kU * kU));
-      for (int64_t i = begin + threadIdx.x; i < to; i += 16 * 128) {
-        float v[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = a.scores[min(i + j * 128, all - 1)];
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (i + j * 128 < to) a.out[i + j * 128] = v[j];
-      }
-      from = to;
-    }
-  }
-
   while (any) {
     const int64_t row0 = ((int64_t)cw.b * a.Hkv + cw.h) * a.capacity;
-    for (int i = threadIdx.x; i < rows8 * (DP / 8); i += 128) {
-      const int r = i / (DP / 8), c = i - r * (DP / 8), e = a.i0 + r / a.G;
-      uint4 v = make_uint4(0, 0, 0, 0);
-      float2 f = make_float2(INFINITY, __int_as_float(-1));
-      if (r < a.rows) {
-        const int u = a.accepted ? a.accepted[(int64_t)cw.b * a.T + e] : e;
-        if ((unsigned)u < (unsigned)a.tokens) {
-          const int hq = cw.h * a.G + r % a.G;
-          if (c * 8 < a.c.dim)
-            v = __ldg(reinterpret_cast<const uint4*>(a.q + cw.b * a.qb + u * a.qt + hq * a.qh + c * 8));
-          const float l = a.lse[((int64_t)cw.b * a.tokens + u) * a.Hq + hq];
-          if (l != -INFINITY) f = make_float2(l * kLog2e, __int_as_float(cw.k.n + e));
-        }
-      }
-      *reinterpret_cast<uint4*>(qs + qat(r, c)) = v;
-      if (c == 0) info[r] = f;
-    }
-    __syncthreads();
     // the scores to add to are asked for one unit ahead
     const int top = a.out != a.scores ? a.capacity : min(a.capacity, cw.k.hi);
     float next[kMine];
@@ -222,6 +211,26 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
       for (int e = 0; e < kMine; ++e) next[e] = __ldg(a.scores + row0 + min(u * kU + mine + 32 * e, a.capacity - 1));
     };
     ask(cw.start + warp);
+    // the token of row r, or -1: the loads below do not wait for one another
+    auto token = [&](int r) -> int {
+      const int e = a.i0 + min(r, a.rows - 1) / a.G, u = a.accepted ? __ldg(a.accepted + (int64_t)cw.b * a.T + e) : e;
+      return r < a.rows && (unsigned)u < (unsigned)a.tokens ? u : -1;
+    };
+#pragma unroll 4
+    for (int i = threadIdx.x; i < rows8 * (DP / 8); i += 128) {
+      const int r = i / (DP / 8), c = i - r * (DP / 8), u = token(r), hq = cw.h * a.G + r % a.G;
+      const bool on = u >= 0 && c * 8 < a.c.dim;
+      mma::cp_async_16_or_zero(qaddr + qat(r, c), on ? a.q + cw.b * a.qb + u * a.qt + hq * a.qh + c * 8 : a.q, on);
+    }
+    for (int r = threadIdx.x; r < rows8; r += 128) {
+      const int u = token(r), hq = cw.h * a.G + r % a.G;
+      const float l = u >= 0 ? a.lse[((int64_t)cw.b * a.tokens + u) * a.Hq + hq] : -INFINITY;
+      info[r] = l != -INFINITY ? make_float2(l * kLog2e, __int_as_float(cw.k.n + a.i0 + r / a.G))
+                               : make_float2(INFINITY, __int_as_float(-1));
+    }
+    ptx::cp_async_commit();
+    ptx::cp_async_wait_all();
+    sync128();
     for (int u = cw.start + warp; u < cw.end; u += 4) {
       const int slot0 = u * kU;
       float before[kMine];
@@ -243,29 +252,39 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
         for (int k = 0; k < KS; ++k)
           mma::ldsm_x4(kt + mma::tile_at<kU>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), kf[mt][k]);
       float sum[2 * MT] = {};  // slots slot0 + lane / 4 + 8 i
-      for (int r = 0; r < rows8; r += 8) {
-        float s[MT][4] = {};
+      // eight rows at a time, or twice eight whose chains of products run side by side
+      auto add_rows = [&](int r, auto blocks) {
+        constexpr int N = decltype(blocks)::value;
+        float s[N][MT][4] = {};
 #pragma unroll
         for (int k = 0; k < KS; k += 2) {
-          uint32_t f[4];
-          mma::ldsm_x4(qaddr + qat(r + (lane & 7), 2 * k + (lane >> 3)), f);
+          uint32_t f[N][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            mma::bf16_16816(s[mt], kf[mt][k], f[0], f[1]);
-            mma::bf16_16816(s[mt], kf[mt][k + 1], f[2], f[3]);
-          }
+          for (int x = 0; x < N; ++x) mma::ldsm_x4(qaddr + qat(r + 8 * x + (lane & 7), 2 * k + (lane >> 3)), f[x]);
+#pragma unroll
+          for (int half = 0; half < 4; half += 2)
+#pragma unroll
+            for (int x = 0; x < N; ++x)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) mma::bf16_16816(s[x][mt], kf[mt][k + half / 2], f[x][half], f[x][half + 1]);
         }
-        const float2 f0 = info[r + (lane & 3) * 2], f1 = info[r + (lane & 3) * 2 + 1];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int x = 0; x < N; ++x) {
+          const float2 f0 = info[r + 8 * x + (lane & 3) * 2], f1 = info[r + 8 * x + (lane & 3) * 2 + 1];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = e & 1 ? f1 : f0;
-            const int key = slot0 + mt * 16 + lane / 4 + (e >> 1) * 8;
-            const float p = mma::exp2_fast(s[mt][e] * a.scale2 - f.x);
-            sum[mt * 2 + (e >> 1)] += key <= __float_as_int(f.y) ? p : 0.f;
-          }
-      }
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float2 f = e & 1 ? f1 : f0;
+              const int key = slot0 + mt * 16 + lane / 4 + (e >> 1) * 8;
+              const float p = mma::exp2_fast(s[x][mt][e] * a.scale2 - f.x);
+              sum[mt * 2 + (e >> 1)] += key <= __float_as_int(f.y) ? p : 0.f;
+            }
+        }
+      };
+      int r = 0;
+      for (; r + 16 <= rows8; r += 16) add_rows(r, std::integral_constant<int, 2>());
+      if (r < rows8) add_rows(r, std::integral_constant<int, 1>());
 #pragma unroll
       for (int i = 0; i < 2 * MT; ++i) {
         sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], 1);
@@ -280,7 +299,7 @@ __global__ void __launch_bounds__(128) kv_scores_kernel(const __grid_constant__ 
       }
     }
     if (!walk_next<kU>(a, cw)) break;
-    __syncthreads();
+    sync128();
   }
   if constexpr (kTma) {
     if (*(volatile int*)&abort_flag) {
@@ -311,7 +330,7 @@ int scores_launch(ScoreArgs a, const CacheMaps& maps, cudaStream_t st) {
     a.rows = std::min(step, a.T - a.i0) * a.G;
     const int smem = Cfg::smem((a.rows + 7) / 8 * 8);
     const int grid = sm_count() * (smem <= 113 * 1024 ? 2 : 1);
-    kv_scores_kernel<DP, kTma><<<grid, 128, smem, st>>>(a, maps);
+    kv_scores_kernel<DP, kTma><<<grid, kScoreThreads, smem, st>>>(a, maps);
     BS_LAUNCHED();
     a.scores = a.out;
   }
