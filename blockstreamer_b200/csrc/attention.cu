@@ -552,9 +552,6 @@ constexpr float kRescale = 8.f;
 // drafts, heads of 128: 92.0, 90.3, 89.2.
 constexpr int kPolyOf = 8;
 
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort));
-}
 // A K x N operand whose N extent is contiguous (64 values = 128 bytes per row
 // of K, 128B-swizzled): 8-row groups 1024 bytes apart, 64-value panels `panel`.
 __device__ __forceinline__ uint64_t sdesc_nmajor_sw128(uint32_t saddr, uint32_t panel) {

@@ -113,6 +113,10 @@ __device__ __forceinline__ int64_t chunk_of(const SplitArgs& a, int64_t total, i
   const int64_t chunk = max((int64_t)a.min_chunk, (total + grid - 1) / grid);
   return a.fixed ? (chunk + a.fixed - 1) / a.fixed * a.fixed : chunk;
 }
+// A whole warp waits; false when the wait of some lane ran out.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  return __all_sync(0xffffffffu, ptx::mbar_wait(bar, parity, abort));
+}
 __device__ __forceinline__ void sync128() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 template <int kU>
 __device__ Range locate(const SplitArgs& a, int cta, int grid, int64_t* sums /* smem [6] */) {
@@ -245,14 +249,15 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return y;
 }
 // a * b + c and a + b on two values at once.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float c) {
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
   float2 r;
-  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %6};\n\t"
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
       "fma.rn.f32x2 x, x, y, z;\n\tmov.b64 {%0, %1}, x;\n\t}"
       : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c));
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
   return r;
 }
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float c) { return fma2(a, b, make_float2(c, c)); }
 __device__ __forceinline__ float2 fma2(float2 a, float b, float c) { return fma2(a, make_float2(b, b), c); }
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   float2 r;

@@ -504,6 +504,36 @@ def test_kv_scores(T, A, Hq, Hkv, D, page, lens):
         assert same is gs and torch.equal(gs, out)
 
 
+@pytest.mark.parametrize("T,A,Hq,Hkv,D,page,lens", [
+    (3, 3, 8, 1, 64, 16, [0, 125, 126, 400]),       # 24 rows: products of 16 keys
+    (5, 4, 7, 1, 64, 8, [127, 128, 0]),             # 28 rows: tiles of 128, padded to 32
+    (9, 9, 8, 4, 32, 64, [1, 300]),                 # 18
+    (3, 3, 24, 4, 128, 128, [0, 253]),              # 18 at a head of 128
+    (16, 16, 16, 2, 64, 32, [511, 5]),              # 128
+    (20, 17, 8, 1, 96, 16, [130, 64, 700]),         # 136: two launches, the second of 8 rows
+    (40, 33, 16, 2, 128, 48, [77, 129]),            # 264: three
+    (2, 2, 128, 1, 64, 16, [1000]),                 # one token to a launch
+    (40, 33, 16, 2, 128, 12, [77, 129]),            # pages without boxes
+])
+def test_kv_scores_of_many_rows(T, A, Hq, Hkv, D, page, lens):
+    test_kv_scores(T, A, Hq, Hkv, D, page, lens)
+
+
+def test_infinite_keys_reach_only_the_rows_that_count():
+    """A key of infinities in view of every row: tokens not accepted and rows that attended
+    nothing add nothing, whatever they would multiply."""
+    T, n, page, D = 4, 300, 16, 64
+    kc, _, table, L, g = make_cache([n], T, 1, D, page, 5)
+    kc[int(table[0, 7 // page]), 7 % page] = -math.inf
+    q = torch.rand(1, T, 8, D, generator=g).bfloat16() + 1
+    lse = torch.full((1, T, 8), 5.0)
+    lse[0, 1, 3] = -math.inf
+    acc = torch.tensor([[0, 1, 3, -1]], dtype=torch.int32)
+    s = torch.zeros(1, 1, table.shape[1] * page)
+    out = kernels.kv_scores_add(*to(s, q, lse, kc, table, L), accepted=acc.to(DEV)).cpu()
+    assert bool(out.isfinite().all()) and float(out[0, 0, 7]) == 0
+
+
 def test_kv_scores_of_more_rows_than_fit_at_once():
     """Many query heads and tokens: the rows are taken in several launches, with the same sums."""
     T, Hq, D, page, n = 40, 64, 128, 16, 50
