@@ -12,7 +12,9 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 // ---------------------------------------------------------------- commit
 // One CTA per (sequence, kv head): all accepted rows are read before any is
-// written (slot n + i may itself be the source of an earlier row).
+// written (slot n + i may itself be the source of an earlier row).  Bound by the
+// launch and one round trip: 5 of 16 drafts, 8 heads of 64: 2.7 us for one sequence,
+// 3.2 for 64.
 __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant__ PagedCache c, int T,
                                                           const int32_t* __restrict__ accepted, int A) {
   extern __shared__ __align__(16) uint4 rows[];
@@ -1063,12 +1065,12 @@ extern "C" int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int
   const int few = D <= 64 ? 24 : 16;
   a.box = cache_box_rows(cache, 128);
   if (a.box >= 8 && A * a.G > few) {
-    a.setup = 3;
+    a.setup = 3;  // 1 / 2 / 3 / 4 / 5: 14.7 / 13.4 / 11.1 / 10.9 / 11.2 us at 12 items of 30011 keys, 56 rows
     a.min_chunk = 2;
     BS_TRY(cache_maps(cache, a.box, false, &maps));
     return D <= 64 ? scores_tiles_launch<64>(a, maps, st) : scores_tiles_launch<128>(a, maps, st);
   }
-  a.setup = 8;
+  a.setup = 8;  // 4 / 6 / 8: 38.9 / 34.0 / 32.0 us at 256 ragged items of 8192 keys, 8 rows; 16.8 / 15.2 / 15.8 at 12
   a.min_chunk = 4;
   a.box = cache_box_rows(cache, D <= 64 ? ScoreCfg<64>::kU : ScoreCfg<128>::kU);
   if (a.box >= 8) {

@@ -6,7 +6,7 @@ MoE half: ``B200GptOssMoEBlock``), accepts one path of every tree, keeps its key
 and values, adds the attention they gave to the cached keys' scores, and cuts the
 cache to its budget when it has grown past it.
 
-    python examples/tree_decode.py [--steps 8] [--batch 4] [--drafts 12] [--budget 96]
+    python examples/tree_decode.py [--steps 12] [--batch 4] [--drafts 12] [--budget 24]
 """
 
 import argparse
@@ -57,7 +57,7 @@ def draft_tree(drafts, lens, generator):
 
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("--steps", type=int, default=8)
+    ap.add_argument("--steps", type=int, default=12)
     ap.add_argument("--batch", type=int, default=4)
     ap.add_argument("--drafts", type=int, default=12)
     ap.add_argument("--budget", type=int, default=24)
