@@ -271,6 +271,24 @@ def test_tree_attention_of_more_rows(T, Hq, Hkv, D, page, lens, window, sinks, t
     check_attention(q, kc, vc, table, L, pos, mask, s, window)
 
 
+@pytest.mark.parametrize("B,T,Hq,Hkv,D,page,far,window", [
+    (300, 1, 4, 2, 32, 8, False, 0), (300, 1, 4, 2, 32, 8, True, 0), (257, 2, 4, 1, 64, 3, True, 5),
+    (140, 5, 8, 1, 64, 8, False, 0), (140, 5, 8, 1, 64, 8, True, 0), (129, 5, 8, 1, 128, 256, True, 0),
+])
+def test_tree_attention_of_many_sequences(B, T, Hq, Hkv, D, page, far, window):
+    """More sequences than one step of the search for a CTA's range takes."""
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 12, (B,), generator=g).tolist()
+    kc, vc, table, L, g = make_cache(lens, T, Hkv, D, page, B + T)
+    mask, pos = make_tree(B, T, lens, g, unused=min(1, T - 1))
+    poison_unused(kc, table, L, pos)
+    poison_unused(vc, table, L, pos)
+    if far:
+        table = torch.cat([table, torch.zeros(B, 600 // page + 1, dtype=torch.int32)], 1)
+    q = (torch.randn(B, T, Hq, D, generator=g) * 2).bfloat16()
+    check_attention(q, kc, vc, table, L, pos, mask, torch.randn(Hq, generator=g), window)
+
+
 @pytest.mark.parametrize("T,Hq,Hkv,D,scale", [(20, 8, 1, 64, 30.0), (40, 8, 1, 128, 30.0), (20, 8, 1, 64, -3.0), (1, 8, 1, 64, -3.0)])
 def test_rows_whose_maximum_keeps_moving(T, Hq, Hkv, D, scale):
     """Scores of hundreds that grow along the keys: the reference moves, and the sums and
@@ -514,6 +532,8 @@ def test_kv_scores(T, A, Hq, Hkv, D, page, lens):
     (40, 33, 16, 2, 128, 48, [77, 129]),            # 264: three
     (2, 2, 128, 1, 64, 16, [1000]),                 # one token to a launch
     (40, 33, 16, 2, 128, 12, [77, 129]),            # pages without boxes
+    (3, 2, 4, 2, 64, 256, [6] * 150),               # more sequences than one step of the search
+    (5, 4, 8, 1, 64, 256, [3] * 131),
 ])
 def test_kv_scores_of_many_rows(T, A, Hq, Hkv, D, page, lens):
     test_kv_scores(T, A, Hq, Hkv, D, page, lens)
