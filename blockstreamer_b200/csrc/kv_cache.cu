@@ -705,6 +705,20 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   auto keys4 = [&](int i, float4 x) -> uint4 {
     return make_uint4(key_of(s0 + i, x.x), key_of(s0 + i + 1, x.y), key_of(s0 + i + 2, x.z), key_of(s0 + i + 3, x.w));
   };
+  // counts a lane's four keys by their first digit
+  auto count4 = [&](int there, const uint32_t* k) {
+    const uint32_t d = __shfl_sync(0xffffffffu, k[0] >> 21, 0);
+    const bool one = there >= 4 && k[0] >> 21 == d && k[1] >> 21 == d && k[2] >> 21 == d && k[3] >> 21 == d;
+    if (__all_sync(0xffffffffu, one)) {  // untouched scores and protected slots: 128 of one digit
+      if (lane == 0) atomicAdd(&hist[0][d], 128u);
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < there) atomicAdd(&hist[0][k[e] >> 21], 1u);
+  };
+  *reinterpret_cast<uint4*>(hist[0] + 4 * threadIdx.x) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
   if (kFits) {
     for (int j = 0; j < steps; j += 4) {
       float4 x[4];
@@ -713,7 +727,12 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = w0 + (j + e) * 128 + lane * 4;
-        if (j + e < steps) *reinterpret_cast<uint4*>(held + i) = keys4(i, x[e]);
+        if (j + e < steps) {
+          const uint4 v = keys4(i, x[e]);
+          *reinterpret_cast<uint4*>(held + i) = v;
+          const uint32_t k[4] = {v.x, v.y, v.z, v.w};
+          if (want < n) count4(w1 - i, k);
+        }
       }
     }
   }
@@ -753,20 +772,12 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t digit = pass == 2 ? 0x3ffu : 0x7ffu;
       uint32_t* hs = hist[pass & 1];
-      *reinterpret_cast<uint4*>(hs + 4 * threadIdx.x) = make_uint4(0, 0, 0, 0);
-      __syncthreads();
+      if (pass) {
+        *reinterpret_cast<uint4*>(hs + 4 * threadIdx.x) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+      }
       if (pass == 0) {
-        walk([&](int slot, int there, const uint32_t* k) {
-          const uint32_t d = __shfl_sync(0xffffffffu, k[0] >> 21, 0);
-          const bool one = there >= 4 && k[0] >> 21 == d && k[1] >> 21 == d && k[2] >> 21 == d && k[3] >> 21 == d;
-          if (__all_sync(0xffffffffu, one)) {  // untouched scores and protected slots: 128 of one digit
-            if (lane == 0) atomicAdd(&hs[d], 128u);
-            return;
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (e < there) atomicAdd(&hs[k[e] >> 21], 1u);
-        });
+        if (!kFits) walk([&](int slot, int there, const uint32_t* k) { count4(there, k); });
       } else if (!kFits) {
         walk([&](int slot, int there, const uint32_t* k) {
 #pragma unroll
