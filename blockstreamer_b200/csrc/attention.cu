@@ -78,9 +78,9 @@ namespace {
 
 constexpr int kMaxDrafts = 256;
 // Up to so many keys an item is not cut.  At one sequence, one token and 8 kv heads:
-// 250 keys 9.5 us on the device in one launch, 10.2 cut and joined; 516 keys 11.8
-// and 10.3, but 21 and 24 us where the host launches; 900 keys 17.0 and 11.7.
-// 64 sequences with a window of 128: 18.1 and 21.5.
+// 250 keys 9.5 us on the device in one launch, 10.2 cut and joined; 450 keys 12.0
+// and 10.8, but 19.7 and 21.5 where the host launches; 900 keys 16.7 and 10.5.
+// 64 sequences: 450 keys 22.4 and 24.9; with a window of 128 18.1 and 21.5.
 constexpr int kWholeKeys = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -1106,19 +1106,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
   }
 }
 
-// Joins the pieces of the items that several CTAs share, in CTA order; a block
-// takes kJoinRows rows of an item.
+// Joins the pieces of the items that several CTAs share; a block takes kJoinRows rows
+// and some groups of four columns of an item.  kSplit neighbouring lanes take every
+// kSplit-th piece of one row and group (a fixed order of the sums, so equal results on
+// every run).  Bound by latency: a lane asks for its pieces' maxima and outputs at once.
+// One sequence of 8192 / 131072 keys, 8 kv heads, 37 pieces to an item: with the kernel
+// before it 22.0 / 65 us where one lane took all pieces after their maxima, 13.0 / 54 so.
 constexpr int kJoinRows = 8;
-template <int kU, int kRows>
-__global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ TreeArgs a, int grid) {
-  __shared__ int64_t sums[8];
-  const int per = a.Hkv * a.tiles;
+template <int kSplit>
+struct JoinCfg {
+  static constexpr int kCols = kSplit == 1 ? 16 : 8, kThreads = kJoinRows * kSplit * kCols;
+};
+template <int kU, int kRows, int kSplit>
+__global__ void __launch_bounds__(JoinCfg<kSplit>::kThreads) tree_join_kernel(const __grid_constant__ TreeArgs a, int grid) {
+  constexpr int kThreads = JoinCfg<kSplit>::kThreads, kWarps = kThreads / 32;
+  __shared__ int64_t sums[2][kWarps];
+  const int per = a.Hkv * a.tiles, tid = threadIdx.x;
   const int b = blockIdx.x / per, item = blockIdx.x - b * per;
   const int h = item / a.tiles, tile = item - h * a.tiles;
   // units before this sequence, and in all (the lengths are inputs of the first
   // launch too, so nothing of this waits for it)
   int64_t before = 0, total = 0;
-  for (int i = threadIdx.x; i < a.B; i += 128) {
+  for (int i = tid; i < a.B; i += kThreads) {
     const int64_t w = units_of<kU>(a, i) * per;
     total += w;
     if (i < b) before += w;
@@ -1128,75 +1137,114 @@ __global__ void __launch_bounds__(128) tree_join_kernel(const __grid_constant__ 
     before += __shfl_xor_sync(0xffffffffu, before, o);
     total += __shfl_xor_sync(0xffffffffu, total, o);
   }
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x / 32] = before, sums[4 + threadIdx.x / 32] = total;
+  if ((tid & 31) == 0) sums[0][tid / 32] = before, sums[1][tid / 32] = total;
   __syncthreads();
-  before = sums[0] + sums[1] + sums[2] + sums[3];
-  total = sums[4] + sums[5] + sums[6] + sums[7];
+  before = total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) before += sums[0][i], total += sums[1][i];
   const int64_t units = units_of<kU>(a, b);
   const int64_t chunk = chunk_of(a, total, grid);
   const int64_t s = before + item * units, e = s + units;
   const int c0 = (int)((s + a.setup) / chunk), c1 = (int)((e - 1) / chunk);
   const int dim = a.c.dim, row0 = tile * kRows, rows = min(kRows, a.R - row0);
-  const int first = blockIdx.y * kJoinRows, last = min(rows, first + kJoinRows);
-  const int row = first + threadIdx.x % kJoinRows;  // each thread: one row, every 16th group of four columns
-  const bool joins = c0 != c1 && row < last;
-  const int t = (row0 + min(row, rows - 1)) / a.G, hq = h * a.G + row0 + min(row, rows - 1) - t * a.G;
-  const bool used = joins && a.pos[(int64_t)b * a.T + t] >= 0;
-  const float sink = joins && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
+  const int row = blockIdx.y * kJoinRows + tid % kJoinRows, mine = min(row, rows - 1);
+  const int part = tid / kJoinRows % kSplit, c = blockIdx.z * JoinCfg<kSplit>::kCols + tid / (kJoinRows * kSplit);
+  const int t = (row0 + mine) / a.G, hq = h * a.G + row0 + mine - t * a.G;
+  const bool used = c0 != c1 && a.pos[(int64_t)b * a.T + t] >= 0;
+  const float sink = c0 != c1 && a.sinks ? a.sinks[hq] * kLog2e : -INFINITY;
   // every thread waits, so that this launch does not end before the first
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!joins) return;
-  float mx = -INFINITY;
-#pragma unroll 4
-  for (int x = c0; x <= c1; ++x) mx = fmaxf(mx, a.part_ml[(2 * (int64_t)x + (x == c0)) * kRows + row].x);
+  if (c0 == c1) return;
+  constexpr int kAhead = kSplit == 1 ? 4 : 10;
+  const int col = min(c, dim / 4 - 1);
+  auto slot = [&](int x) { return 2 * (int64_t)x + (x == c0); };
+  float m = -INFINITY, z = 0.f;  // of this lane's pieces, and v relative to m
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int x = c0 + part; x <= c1; x += kAhead * kSplit) {
+    float2 mz[kAhead];
+    float4 p[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t at = slot(min(x + j * kSplit, c1));
+      mz[j] = a.part_ml[at * kRows + mine];
+      p[j] = a.part_o[(at * (dim / 4) + col) * kRows + mine];
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (x + j * kSplit <= c1) top = fmaxf(top, mz[j].x);
+    if (top == -INFINITY) continue;
+    const float f = mma::exp2_fast(m - top);
+    z *= f, v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+    m = top;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      if (x + j * kSplit > c1 || mz[j].x == -INFINITY) continue;
+      const float g = mma::exp2_fast(mz[j].x - m);
+      z += mz[j].y * g, v.x += p[j].x * g, v.y += p[j].y * g, v.z += p[j].z * g, v.w += p[j].w * g;
+    }
+  }
+  float mx = m;
+#pragma unroll
+  for (int o = kJoinRows; o < kJoinRows * kSplit; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   const float top = fmaxf(mx, sink);
   const float ref = top == -INFINITY ? 0.f : top;
-  const int64_t at = ((int64_t)b * a.T + t) * a.Hkv * a.G + hq;
-  for (int c = threadIdx.x / kJoinRows; c < dim / 4; c += 128 / kJoinRows) {
-    float den = a.sinks ? mma::exp2_fast(sink - ref) : 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int x = c0; x <= c1; ++x) {
-      const int64_t slot = 2 * (int64_t)x + (x == c0);
-      const float2 mz = a.part_ml[slot * kRows + row];
-      const float4 p = a.part_o[(slot * (dim / 4) + c) * kRows + row];
-      const float f = mz.x == -INFINITY ? 0.f : mma::exp2_fast(mz.x - ref);
-      den += mz.y * f;
-      v.x += p.x * f;
-      v.y += p.y * f;
-      v.z += p.z * f;
-      v.w += p.w * f;
-    }
-    uint2 w = make_uint2(0u, 0u);
-    if (used && mx > -INFINITY) w = make_uint2(pack_bf16x2(v.x / den, v.y / den), pack_bf16x2(v.z / den, v.w / den));
-    *reinterpret_cast<uint2*>(a.out + at * dim + c * 4) = w;
-    if (c == 0 && a.lse) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
+  const float f = m == -INFINITY ? 0.f : mma::exp2_fast(m - ref);
+  z *= f, v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+#pragma unroll
+  for (int o = kJoinRows; o < kJoinRows * kSplit; o <<= 1) {
+    z += __shfl_xor_sync(0xffffffffu, z, o);
+    v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+    v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+    v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
   }
+  if (part || row >= rows || c >= dim / 4) return;
+  const float den = z + (a.sinks ? mma::exp2_fast(sink - ref) : 0.f);
+  uint2 w = make_uint2(0u, 0u);
+  if (used && mx > -INFINITY) w = make_uint2(pack_bf16x2(v.x / den, v.y / den), pack_bf16x2(v.z / den, v.w / den));
+  const int64_t at = ((int64_t)b * a.T + t) * a.Hkv * a.G + hq;
+  *reinterpret_cast<uint2*>(a.out + at * dim + c * 4) = w;
+  if (c == 0 && a.lse) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
 }
 
-// Rows of a tile: 16 and 32 run on the HBM-bound kernel of few rows, 128 and
-// 256 (a pair of tiles) on tcgen05, which needs TMA boxes.  The workspace is
+// Rows of a tile: 16 run on the HBM-bound kernel of few rows, 128 and 256 (a pair of
+// tiles) on tcgen05, which needs TMA boxes; without them tiles of 32 (heads up to 64)
+// serve all.  24 or 32 rows, heads of 64, in tiles of 32 on mma.sync and of 128 on
+// tcgen05, us: 2 x 131072 keys 136 / 99, 8 x 8192 47 / 38, 1 x 8192 18.2 / 16.5, 64
+// ragged to 8192 162 / 131, 64 x 2000 93 / 81, but 64 x 300 33 / 39.  The workspace is
 // sized without the page size, for the larger.
 int tile_rows(int64_t R, int64_t D, bool tma) {
-  const int few = R <= 16 || D > 64 ? 16 : 32;
-  if (R <= few || !tma) return few;
+  if (R <= 16 || (!tma && D > 64)) return 16;
+  if (!tma) return 32;
   return R <= 128 ? 128 : 256;
 }
 
-template <int kU, int kRows>
+template <int kU, int kRows, int kSplit>
 int launch_join(const TreeArgs& a, int grid, cudaStream_t st) {
-  if (a.fixed) return BS_OK;  // no item is cut
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.tiles), (unsigned)cdiv(std::min(kRows, a.R), kJoinRows));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3((unsigned)(a.B * a.Hkv * a.tiles), (unsigned)cdiv(std::min(kRows, a.R), kJoinRows),
+                     (unsigned)cdiv(a.c.dim / 4, JoinCfg<kSplit>::kCols));
+  cfg.blockDim = dim3(JoinCfg<kSplit>::kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  BS_CUDA(cudaLaunchKernelEx(&cfg, tree_join_kernel<kU, kRows>, a, grid));
+  BS_CUDA(cudaLaunchKernelEx(&cfg, tree_join_kernel<kU, kRows, kSplit>, a, grid));
   return BS_OK;
+}
+template <int kU, int kRows>
+int launch_join(const TreeArgs& a, int grid, cudaStream_t st) {
+  if (a.fixed) return BS_OK;  // no item is cut
+  // four lanes to a row's pieces where an item has more than four of them, about, unless
+  // the blocks fill the GPU anyway (4 x 32768 keys, 32 tokens of 32 / 8 heads of 128: 118 us
+  // with four lanes, 107 with one)
+  const int64_t items = (int64_t)a.B * a.Hkv * a.tiles;
+  const int64_t blocks = items * cdiv(std::min(kRows, a.R), kJoinRows) * cdiv(a.c.dim / 4, JoinCfg<1>::kCols);
+  return grid > 4 * items && blocks <= 2 * sm_count() ? launch_join<kU, kRows, 4>(a, grid, st)
+                                                       : launch_join<kU, kRows, 1>(a, grid, st);
 }
 
 template <int DP, int MT, bool kTma>
@@ -1310,6 +1358,6 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   if (rows == 128) return D <= 64 ? launch_tiles<64, false>(a, maps, grid, st) : launch_tiles<128, false>(a, maps, grid, st);
   if (rows == 256) return D <= 64 ? launch_tiles<64, true>(a, maps, grid, st) : launch_tiles<128, true>(a, maps, grid, st);
   if (D > 64) return tma ? launch_rows<128, 1, true>(a, maps, grid, st) : launch_rows<128, 1, false>(a, maps, grid, st);
-  if (rows == 32) return tma ? launch_rows<64, 2, true>(a, maps, grid, st) : launch_rows<64, 2, false>(a, maps, grid, st);
+  if (rows == 32) return launch_rows<64, 2, false>(a, maps, grid, st);
   return tma ? launch_rows<64, 1, true>(a, maps, grid, st) : launch_rows<64, 1, false>(a, maps, grid, st);
 }

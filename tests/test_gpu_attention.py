@@ -231,6 +231,11 @@ def test_tree_attention(T, Hq, Hkv, D, page, lens, window, sinks, tree, head_maj
 
 
 MORE_ROWS = [
+    # pages without boxes: tiles of 32 rows, full and not, and of 16 at a head of 128
+    (4, 8, 1, 32, 12, [129, 64], 0, False, "each"),
+    (3, 20, 2, 64, 5, [100, 0], 9, True, "shared"),
+    (9, 8, 1, 64, 20, [77], 0, True, "chain"),
+    (5, 8, 1, 128, 10, [63, 64], 0, True, "each"),
     # rows to a kv head: 24 and 32; 165, 200, 384 and 512 (pairs of row tiles, the last half empty)
     (2, 12, 1, 64, 16, [70, 0], 0, True, "each"),
     (4, 8, 1, 32, 8, [129, 64], 0, False, "each"),
