@@ -125,7 +125,8 @@ struct RowsSmem {
   static constexpr int ml = merge + kBufs * kRows * DP * 4;    // [4 warps][rows] float2
   static constexpr int bits = ml + 4 * kRows * 8;              // [rows][8] words
   static constexpr int thr = bits + kRows * (kMaxDrafts / 32) * 4;
-  static constexpr int sums = (thr + kRows * 4 + 15) / 16 * 16;
+  static constexpr int q = (thr + kRows * 4 + 127) / 128 * 128;  // the item's Q
+  static constexpr int sums = q + kRows * DP * 2;
   static constexpr int bars = sums + 64;                       // [4 warps][kStages]
   static constexpr int total = bars + 4 * RowsCfg<DP>::kStages * 8 + 1024;
 };
@@ -234,52 +235,84 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
   for (int s = 0; s < Cfg::kStages - 1; ++s) load(s);
   int stage = 0, phase = 0;
 
+  // ---- what an item starts with, asked for while the item before it is worked on: its Q,
+  // and the positions and masks of the first row of bits of each warp
+  constexpr int kChunks = DP / 8, kQ = kRows * kChunks / 128;
+  const int words = (a.T + 31) / 32;
+  uint4 next_q[kQ];
+  int next_pt = -1, next_pu = -1;
+  uint8_t next_may = 0;
+  auto ask = [&](const Walk& w) {
+    const int row0 = w.tile * kRows, rows = min(kRows, a.R - row0);
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+      const int x = threadIdx.x + i * 128, row = row0 + min(x / kChunks, rows - 1), t = row / a.G, g = row - t * a.G;
+      next_q[i] = __ldg(reinterpret_cast<const uint4*>(a.q + w.b * a.qb + t * a.qt + (int64_t)(w.h * a.G + g) * a.qh +
+                                                       min(x % kChunks * 8, a.c.dim - 8)));
+    }
+    const int tl = min(warp / words, (row0 + rows - 1) / a.G - row0 / a.G), t = row0 / a.G + tl;
+    const int uc = min((warp - warp / words * words) * 32 + lane, a.T - 1);
+    const int32_t* pos = a.pos + (int64_t)w.b * a.T;
+    next_pt = __ldg(pos + t), next_pu = __ldg(pos + uc);
+    if (a.mask) next_may = __ldg(a.mask + w.b * a.mask_b + (int64_t)t * a.T + uc);
+  };
+  ask(cw);
+
   // ---- pieces
   while (true) {
     const int row0 = cw.tile * kRows, rows = min(kRows, a.R - row0);
     const int t0 = row0 / a.G, toks = (row0 + rows - 1) / a.G - t0 + 1;
+#pragma unroll
+    for (int i = 0; i < kQ; ++i) {
+      const int x = threadIdx.x + i * 128, r = x / kChunks, c = x % kChunks;
+      const bool on = r < rows && c * 8 < a.c.dim;
+      *reinterpret_cast<uint4*>(smem + Sm::q + mma::tile_at<kRows>(r, c)) = on ? next_q[i] : make_uint4(0, 0, 0, 0);
+    }
     // masks of the tile's tokens over the drafts, and each one's window
     if (a.window || cw.k.lo + cw.end * kU > cw.k.n) {
-      const int words = (a.T + 31) / 32;
       const int32_t* pos = a.pos + (int64_t)cw.b * a.T;
-#pragma unroll 4
       for (int i = warp; i < toks * words; i += 4) {
         const int tl = i / words, w = i - tl * words, t = t0 + tl, u = w * 32 + lane;
-        const int uc = min(u, a.T - 1), pt = __ldg(pos + t), pu = u < a.T ? __ldg(pos + uc) : -1;
-        const bool may = a.mask ? __ldg(a.mask + cw.b * a.mask_b + (int64_t)t * a.T + uc) != 0 : u <= t;
+        int pt = next_pt, pu = next_pu;
+        uint8_t may = next_may;
+        if (i >= 4) {
+          const int uc = min(u, a.T - 1);
+          pt = __ldg(pos + t), pu = __ldg(pos + uc);
+          if (a.mask) may = __ldg(a.mask + cw.b * a.mask_b + (int64_t)t * a.T + uc);
+        }
         const int below = a.window ? max(pt, cw.k.n) - a.window : -1;
-        const uint32_t m = __ballot_sync(0xffffffffu, may && pt >= 0 && pu >= 0 && (!a.window || pu > below));
+        const uint32_t m = __ballot_sync(0xffffffffu, u < a.T && (a.mask ? may != 0 : u <= t) && pt >= 0 && pu >= 0 &&
+                                                          (!a.window || pu > below));
         if (lane == 0) {
           bits[tl * kWords + w] = m;
           if (w == 0) thr[tl] = pt >= 0 ? below : INT_MAX;
         }
       }
     }
-    uint32_t qf[MT][KS][4];
+    // (what the rows' ends need is loaded meanwhile)
+    int tl[MT][2], pt[MT][2];
+    float sink[MT][2];
+    int64_t at[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = mt * 16 + lane / 4 + e * 8;
-        const bool on = row < rows;
-        const int t = on ? (row0 + row) / a.G : 0, g = on ? row0 + row - t * a.G : 0;
-        const __nv_bfloat16* q = a.q + cw.b * a.qb + t * a.qt + (int64_t)(cw.h * a.G + g) * a.qh + (lane & 3) * 2;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int col = k * 16 + half * 8;
-            const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(q + min(col, a.c.dim - 8)));
-            qf[mt][k][e + 2 * half] = on && col < a.c.dim ? v : 0u;
-          }
+        const int row = row0 + min(mt * 16 + lane / 4 + e * 8, rows - 1), t = row / a.G, h = cw.h * a.G + row - t * a.G;
+        tl[mt][e] = t - t0;
+        at[mt][e] = ((int64_t)cw.b * a.T + t) * a.Hkv * a.G + h;
+        pt[mt][e] = __ldg(a.pos + (int64_t)cw.b * a.T + t);
+        sink[mt][e] = a.sinks ? __ldg(a.sinks + h) : -INFINITY;
       }
-    int tl[MT][2];
+    __syncthreads();
+    uint32_t qf[MT][KS][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        tl[mt][e] = (row0 + min(mt * 16 + lane / 4 + e * 8, rows - 1)) / a.G - t0;
-    __syncthreads();
+      for (int k = 0; k < KS; ++k)
+        mma::ldsm_x4(ptx::smem_addr(smem) + Sm::q + mma::tile_at<kRows>(mt * 16 + (lane & 15), 2 * k + (lane >> 4)), qf[mt][k]);
+    Walk nw = cw;
+    const bool again = walk_next<kU>(a, nw);
+    if (again) ask(nw);
 
     float m[MT][2], z[MT][2], o[MT][DP / 8][4];
 #pragma unroll
@@ -386,22 +419,14 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
     }
 
     // ---- the warps' parts meet: common maximum, then O of warps 2, 3 to 0, 1 and of 1 to 0
-    // (what the rows' ends need is loaded meanwhile)
     const bool whole = cw.whole();
     const int64_t slot = 2 * (int64_t)blockIdx.x + (cw.start == 0 ? 1 : 0);
     const int dim = a.c.dim;
-    int64_t at[MT][2];
-    float sink[MT][2];
-    bool used[MT][2];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = min(mt * 16 + lane / 4 + e * 8, rows - 1);
-        const int t = (row0 + row) / a.G, h = cw.h * a.G + row0 + row - t * a.G;
-        at[mt][e] = ((int64_t)cw.b * a.T + t) * a.Hkv * a.G + h;
-        used[mt][e] = __ldg(a.pos + (int64_t)cw.b * a.T + t) >= 0;
-        sink[mt][e] = a.sinks ? __ldg(a.sinks + h) * kLog2e : -INFINITY;
+        sink[mt][e] *= kLog2e;
         z[mt][e] += __shfl_xor_sync(0xffffffffu, z[mt][e], 1);
         z[mt][e] += __shfl_xor_sync(0xffffffffu, z[mt][e], 2);
         if ((lane & 3) == 0) ml[warp * kRows + mt * 16 + lane / 4 + e * 8] = make_float2(m[mt][e], z[mt][e]);
@@ -478,16 +503,17 @@ __global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant
           const float ref = top == -INFINITY ? 0.f : top;
           const float f = mx == -INFINITY ? 0.f : mma::exp2_fast(mx - ref);
           const float den = z[mt][e] * f + (a.sinks ? mma::exp2_fast(sink[mt][e] - ref) : 0.f);
-          const float g = used[mt][e] && mx > -INFINITY ? f / den : 0.f;
+          const float g = pt[mt][e] >= 0 && mx > -INFINITY ? f / den : 0.f;
 #pragma unroll
           for (int d = 0; d < DP / 8; ++d)
             if (d * 8 < dim)
               *reinterpret_cast<uint32_t*>(a.out + at[mt][e] * dim + d * 8 + (lane & 3) * 2) =
                   g == 0.f ? 0u : pack_bf16x2(o[mt][d][2 * e] * g, o[mt][d][2 * e + 1] * g);
-          if ((lane & 3) == 0 && a.lse) a.lse[at[mt][e]] = used[mt][e] ? ref * kLn2 + logf(den) : -INFINITY;
+          if ((lane & 3) == 0 && a.lse) a.lse[at[mt][e]] = pt[mt][e] >= 0 ? ref * kLn2 + logf(den) : -INFINITY;
         }
     }
-    if (!walk_next<kU>(a, cw)) break;
+    if (!again) break;
+    cw = nw;
     __syncthreads();
   }
   if constexpr (kTma) {
