@@ -102,18 +102,21 @@ struct TreeArgs : SplitArgs {
 // ---------------------------------------------------------------- few rows
 // Row tiles of MT * 16 rows on mma.sync, four warps per CTA, each streaming its
 // own units of kU keys into its own ring (no barrier between warps) and holding
-// its own (m, z, O); they meet at the end of an item.  HBM-bound: two CTAs per SM
-// keep ~190 KB per SM in flight.  64 sequences of up to 8192 keys, 64 / 8 heads of
-// 64: 91 us, 5.9 TB/s (90% of the measured copy rate); 2 x 131072 keys: 100 us
+// its own (m, z, O); they meet at the end of an item.  HBM-bound for long items: two or
+// three CTAs per SM keep ~190 KB per SM in flight.  64 sequences of up to 8192 keys, 64 / 8
+// heads of 64: 91 us, 5.9 TB/s (90% of the measured copy rate); 2 x 131072 keys: 90 us
 // where a head's slots lie together in a page, 113 us where heads are interleaved
-// (128 bytes in every KB).
+// (128 bytes in every KB).  Short items are bound by the chain of an item's start, units
+// and end, some 8000 cycles, which a third CTA hides better than a third stage of the
+// rings (256 ragged sequences to 1000 keys: 68.8 us, 88 with two CTAs); heads of 128
+// would spill with three (133 us, 126 with two).
 // kTma: a unit is fetched by a few TMA boxes (pages of a multiple of 8 slots); else
 // by 16-byte asynchronous copies, whose address arithmetic and issue are most of
 // the kernel's instructions then (187 us for the 64 sequences).
 template <int DP>
 struct RowsCfg {
   static constexpr int kU = DP == 64 ? 32 : 16;
-  static constexpr int kStages = 3;
+  static constexpr int kStages = DP == 64 ? 2 : 3;
   static constexpr int kTile = kU * DP * 2;           // bytes of a K (or V) unit
   static constexpr int kWarpBytes = 2 * kTile * kStages;
 };
@@ -125,14 +128,18 @@ struct RowsSmem {
   static constexpr int ml = merge + kBufs * kRows * DP * 4;    // [4 warps][rows] float2
   static constexpr int bits = ml + 4 * kRows * 8;              // [rows][8] words
   static constexpr int thr = bits + kRows * (kMaxDrafts / 32) * 4;
-  static constexpr int q = (thr + kRows * 4 + 127) / 128 * 128;  // the item's Q
-  static constexpr int sums = q + kRows * DP * 2;
+  static constexpr int q = merge;                              // the item's Q, until its fragments are read
+  static constexpr int sums = (thr + kRows * 4 + 15) / 16 * 16;
   static constexpr int bars = sums + 64;                       // [4 warps][kStages]
   static constexpr int total = bars + 4 * RowsCfg<DP>::kStages * 8 + 1024;
 };
+static_assert(3 * (RowsSmem<64, 1>::total + 1024) <= 228 * 1024, "three CTAs per SM");
+
+// CTAs of an SM.
+constexpr int rows_ctas(int rows, int64_t dim) { return rows == 16 && dim <= 64 ? 3 : 2; }
 
 template <int DP, int MT, bool kTma>
-__global__ void __launch_bounds__(128, 2) tree_rows_kernel(const __grid_constant__ TreeArgs a,
+__global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(const __grid_constant__ TreeArgs a,
                                                            const __grid_constant__ CacheMaps maps) {
   using Cfg = RowsCfg<DP>;
   using Sm = RowsSmem<DP, MT>;
@@ -1288,7 +1295,7 @@ int launch_rows(TreeArgs& a, const CacheMaps& maps, int grid, cudaStream_t st) {
   return launch_join<RowsCfg<DP>::kU, 16 * MT>(a, grid, st);
 }
 
-int grid_for(int rows) { return rows <= 32 ? 2 * sm_count() : sm_count(); }
+int grid_for(int rows, int64_t D) { return rows <= 32 ? rows_ctas(rows, D) * sm_count() : sm_count(); }
 
 template <int DP, bool kPair>
 int launch_tiles(TreeArgs& a, const CacheMaps& maps, int grid, cudaStream_t st) {
@@ -1314,7 +1321,7 @@ extern "C" size_t bs_tree_attention_workspace_bytes(int64_t B, int64_t T, int64_
   int64_t most = 0;
   for (bool tma : {false, true}) {
     const int rows = tile_rows(T * (Hq / Hkv), D, tma);
-    most = std::max(most, 2 * (int64_t)grid_for(rows) * rows * (D * 4 + 8));
+    most = std::max(most, 2 * (int64_t)grid_for(rows, D) * rows * (D * 4 + 8));
   }
   return align_up((size_t)most, 256);
 }
@@ -1363,10 +1370,10 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   BS_ARG((int64_t)a.B * a.Hkv * a.tiles < INT32_MAX, "%s: sizes too large", fn);
   a.out = static_cast<__nv_bfloat16*>(out);
   a.lse = lse;
-  const int grid = grid_for(rows);
+  const int grid = grid_for(rows, D);
   a.part_o = static_cast<float4*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (int64_t)2 * grid * rows * (D / 4));
-  a.min_chunk = rows <= 32 ? 4 : 2;
+  a.min_chunk = rows <= 32 ? 8 : 2;  // 4 / 6 / 8 units: 13.8 / 13.4 / 12.6 us at 1 x 8192 keys, the same elsewhere
   a.setup = rows <= 32 ? 16 : 8;
   // short ranges of keys (a window, a small cache): whole items to the CTAs, and no second launch
   const int unit = rows > 32 ? 128 : D <= 64 ? RowsCfg<64>::kU : RowsCfg<128>::kU;
