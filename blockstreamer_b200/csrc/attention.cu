@@ -1241,14 +1241,17 @@ __global__ void __launch_bounds__(JoinCfg<kSplit>::kThreads) tree_join_kernel(co
   if (c == 0 && a.lse) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
 }
 
-// Rows of a tile: 16 run on the HBM-bound kernel of few rows, 128 and 256 (a pair of
-// tiles) on tcgen05, which needs TMA boxes; without them tiles of 32 (heads up to 64)
-// serve all.  24 or 32 rows, heads of 64, in tiles of 32 on mma.sync and of 128 on
-// tcgen05, us: 2 x 131072 keys 136 / 99, 8 x 8192 47 / 38, 1 x 8192 18.2 / 16.5, 64
-// ragged to 8192 162 / 131, 64 x 2000 93 / 81, but 64 x 300 33 / 39.  The workspace is
-// sized without the page size, for the larger.
-int tile_rows(int64_t R, int64_t D, bool tma) {
-  if (R <= 16 || (!tma && D > 64)) return 16;
+// Rows of a tile: 16 run on the kernel of few rows, 128 and 256 (a pair of tiles) on
+// tcgen05, which needs TMA boxes; without them tiles of 32 (heads up to 64) serve all.
+// 24 or 32 rows, heads of 64, in tiles of 32 on mma.sync and of 128 on tcgen05, us:
+// 2 x 131072 keys 136 / 99, 8 x 8192 47 / 38, 64 ragged to 8192 162 / 131.  Where no more
+// than kShortKeys are in reach, two tiles of 16 that read the keys twice end sooner: of
+// 16 and of 128, 256 x 300 keys 91 / 125, 256 ragged to 1000 135 / 165, 64 x 600 38 / 47,
+// 1 x 1000 11.5 / 13.1, 64 x 1000 55 / 56, but 64 x 2000 91 / 80.  The workspace is sized
+// without the page size and the reach, for the largest.
+constexpr int64_t kShortKeys = 1024;
+int tile_rows(int64_t R, int64_t D, bool tma, int64_t reach) {
+  if (R <= 16 || (!tma && D > 64) || (R <= 32 && D <= 64 && reach <= kShortKeys)) return 16;
   if (!tma) return 32;
   return R <= 128 ? 128 : 256;
 }
@@ -1319,10 +1322,11 @@ extern "C" size_t bs_tree_attention_workspace_bytes(int64_t B, int64_t T, int64_
   using namespace bs;
   if (B <= 0 || T <= 0 || Hq <= 0 || Hkv <= 0 || D <= 0) return 0;
   int64_t most = 0;
-  for (bool tma : {false, true}) {
-    const int rows = tile_rows(T * (Hq / Hkv), D, tma);
-    most = std::max(most, 2 * (int64_t)grid_for(rows, D) * rows * (D * 4 + 8));
-  }
+  for (bool tma : {false, true})
+    for (int64_t reach : {kShortKeys, kShortKeys + 1}) {
+      const int rows = tile_rows(T * (Hq / Hkv), D, tma, reach);
+      most = std::max(most, 2 * (int64_t)grid_for(rows, D) * rows * (D * 4 + 8));
+    }
   return align_up((size_t)most, 256);
 }
 
@@ -1365,7 +1369,8 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.B = (int)cache->batch;
   a.box = cache_box_rows(cache, 128);
   const bool tma = a.box >= 8;
-  const int rows = tile_rows(a.R, D, tma);
+  const int64_t reach = a.window ? std::min<int64_t>((int64_t)a.window - 1 + a.T + a.box - 1, a.c.capacity) : a.c.capacity;
+  const int rows = tile_rows(a.R, D, tma, reach);
   a.tiles = (int)cdiv(a.R, (int64_t)rows);
   BS_ARG((int64_t)a.B * a.Hkv * a.tiles < INT32_MAX, "%s: sizes too large", fn);
   a.out = static_cast<__nv_bfloat16*>(out);
@@ -1377,7 +1382,6 @@ extern "C" int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, in
   a.setup = rows <= 32 ? 16 : 8;
   // short ranges of keys (a window, a small cache): whole items to the CTAs, and no second launch
   const int unit = rows > 32 ? 128 : D <= 64 ? RowsCfg<64>::kU : RowsCfg<128>::kU;
-  const int64_t reach = a.window ? std::min<int64_t>((int64_t)a.window - 1 + a.T + a.box - 1, a.c.capacity) : a.c.capacity;
   if (reach <= kWholeKeys) a.fixed = (int)cdiv(reach, (int64_t)unit);
   BS_TRY(check_device());
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
