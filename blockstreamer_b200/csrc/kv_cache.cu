@@ -34,19 +34,34 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const __grid_constant_
     if (threadIdx.x == 0) record_status(c.status, BS_ERR_INVALID_ARGUMENT);
     return;
   }
-  const int n = c.len(b, T), per = c.dim / 8, items = 2 * count * per;
+  // nothing is written through a clamped index: a sequence whose length is bad stays as it is,
+  // and so does a slot that its own or its source's page would leave the pool for
+  const int n = c.lens[b], per = c.dim / 8, items = 2 * count * per;
+  if (n < 0 || n > c.capacity - T) {
+    if (threadIdx.x == 0) record_status(c.status, BS_ERR_CAPACITY);
+    return;
+  }
   auto at = [&](int i, int row) -> __nv_bfloat16* {
     const int col = i % per * 8, v = i / per & 1;
     int page, in;
     c.div.split(n + row, page, in);
-    const int64_t p = c.page_of(b, page);
+    const int p = __ldg(c.table + b * c.table_stride + page);
+    if ((unsigned)p >= (unsigned)c.pages) {
+      record_status(c.status, BS_ERR_CAPACITY);
+      return nullptr;
+    }
     return v ? c.v + p * c.vp + in * c.vs + h * c.vh + col : c.k + p * c.kp + in * c.ks + h * c.kh + col;
   };
-  for (int i = threadIdx.x; i < items; i += blockDim.x)
-    rows[i] = *reinterpret_cast<const uint4*>(at(i, acc[i / (2 * per)]));
+  uint32_t found = 0;  // which of the thread's pieces were read (32 at most: 2 * 256 rows of 128 by 256 threads)
+  for (int i = threadIdx.x, j = 0; i < items; i += blockDim.x, ++j) {
+    const __nv_bfloat16* from = at(i, acc[i / (2 * per)]);
+    if (from) rows[i] = *reinterpret_cast<const uint4*>(from), found |= 1u << j;
+  }
   __syncthreads();
-  for (int i = threadIdx.x; i < items; i += blockDim.x)
-    if (acc[i / (2 * per)] != i / (2 * per)) *reinterpret_cast<uint4*>(at(i, i / (2 * per))) = rows[i];
+  for (int i = threadIdx.x, j = 0; i < items; i += blockDim.x, ++j) {
+    if (acc[i / (2 * per)] == i / (2 * per) || !(found >> j & 1)) continue;
+    if (__nv_bfloat16* to = at(i, i / (2 * per))) *reinterpret_cast<uint4*>(to) = rows[i];
+  }
 }
 
 // ---------------------------------------------------------------- scores

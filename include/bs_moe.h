@@ -433,8 +433,9 @@ int bs_tree_attention(const bs_heads* q, const bs_kv_cache* cache, int64_t T, in
 /* After verification: moves the keys and values of the accepted drafts to
  * consecutive slots, slot lens[b] + accepted[b][i] -> lens[b] + i.  accepted
  * [B, A] int32: ascending draft indices, then negative ones; a list that is not
- * ascending records BS_ERR_INVALID_ARGUMENT and its sequence is left as it is.
- * lens is not changed.  A <= 256. */
+ * ascending records BS_ERR_INVALID_ARGUMENT and its sequence is left as it is, and
+ * so is one of a bad length; a row from or to a page outside the pool is not moved
+ * (both record BS_ERR_CAPACITY).  lens is not changed.  A <= 256. */
 int bs_tree_commit(const bs_kv_cache* cache, int64_t T, const int32_t* accepted, int64_t A,
                    void* stream);
 
