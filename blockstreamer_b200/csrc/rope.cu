@@ -92,10 +92,11 @@ __global__ void __launch_bounds__(128) rope_kernel(const __grid_constant__ RopeA
     bool write = false;
     int64_t koff = 0, voff = 0;
     if constexpr (APPEND) {
-      const int slot = a.cache.lens[b] + (int)t;
+      // (the length decides, not the slot: a bad one drops all rows of its sequence)
+      const int len = a.cache.lens[b];
+      write = used && len >= 0 && len <= a.cache.capacity - a.T_;
       int page, row;
-      a.cache.div.split(max(slot, 0), page, row);
-      write = used && slot >= 0 && slot < a.cache.capacity;
+      a.cache.div.split(write ? len + (int)t : 0, page, row);
       int p = write ? __ldg(a.cache.table + b * a.cache.table_stride + page) : 0;
       write = write && (unsigned)p < (unsigned)a.cache.pages;
       if (used && !write && lane == 0) record_status(a.status, BS_ERR_CAPACITY);

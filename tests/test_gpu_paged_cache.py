@@ -68,3 +68,53 @@ def test_commit_moves_no_row_to_or_from_a_page_outside_the_pool(bad, where):
         if where == 1:            # slot 7 to 6 lies in page 3 alone; slot 8 to 7 would come from the bad page
             want[3, 6] = c[3, 7]
         assert torch.equal(d.cpu(), want)
+
+
+def append_to(kc, vc, table, lens, g, T=3):
+    """Both caches after rows of three tokens, and the turned k and the v that were given."""
+    heads, D = kc.shape[2:]
+    q, k, v = (torch.randn(2, T, heads, D, generator=g).bfloat16() for _ in range(3))
+    pos = torch.arange(T, dtype=torch.int32).repeat(2, 1) + 5
+    cs = attention.rotary_table(16, D, device="cpu")
+    gk, gv = to(kc, vc)
+    kernels.rope_append(*to(q, k, v, cs, pos), gk, gv, *to(table, lens))
+    return gk.cpu(), gv.cpu(), oatt.rotary(k, cs, pos), v
+
+
+def check_append(kc, vc, gk, gv, kt, v, rows):
+    """``rows``: (page, slot in it) of every row that was to be written, with its (sequence, token)."""
+    wk, wv, written = kc.double(), vc.clone(), torch.zeros(kc.shape, dtype=torch.bool)
+    for (page, row), (b, t) in rows.items():
+        wk[page, row], wv[page, row], written[page, row] = kt[b, t], v[b, t], True
+    assert torch.equal(gv, wv)
+    assert torch.equal(gk[~written], kc[~written])
+    assert bool(((gk.double() - wk).abs() <= 2.0 ** -8 * wk.abs() + 2.0 ** -20).all())
+
+
+SECOND = {(2, 2): (1, 0), (2, 3): (1, 1), (2, 4): (1, 2)}   # slots 18, 19, 20 of sequence 1
+
+
+@pytest.mark.parametrize("bad", BAD_LENGTHS)
+def test_append_writes_nothing_for_a_sequence_of_bad_length(bad):
+    kc, vc, table, L, g = two_sequences()
+    got = append_to(kc, vc, table, torch.tensor([bad, 18], dtype=torch.int32), g)
+    assert kernels.device_status(clear=True) != 0
+    check_append(kc, vc, *got, SECOND)
+
+
+@pytest.mark.parametrize("good", [0, 21])
+def test_append_at_the_ends_of_a_page_table(good):
+    kc, vc, table, L, g = two_sequences()
+    got = append_to(kc, vc, table, torch.tensor([good, 18], dtype=torch.int32), g)
+    at = {(3, t): (0, t) for t in range(3)} if good == 0 else {(4, 5 + t): (0, t) for t in range(3)}
+    check_append(kc, vc, *got, {**SECOND, **at})
+
+
+@pytest.mark.parametrize("bad", [-1, -2 ** 31, 8, 99, 2 ** 31 - 1])
+def test_append_drops_the_rows_of_a_page_outside_the_pool(bad):
+    kc, vc, table, L, g = two_sequences()
+    tab = table.clone()
+    tab[0, 1] = bad
+    got = append_to(kc, vc, tab, L, g)
+    assert kernels.device_status(clear=True) != 0
+    check_append(kc, vc, *got, {**SECOND, (3, 6): (0, 0), (3, 7): (0, 1)})
