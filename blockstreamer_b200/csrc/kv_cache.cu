@@ -656,7 +656,8 @@ int scores_launch(ScoreArgs a, const CacheMaps& maps, cudaStream_t st) {
 // same order.  A radix selection over digits of 11, 11 and 10 bits (histograms
 // joined through distributed shared memory) finds the key of the last kept slot
 // and how many slots of that very key are kept; a scan then writes the kept
-// slots in order.  Protected slots get the highest key, NaN the lowest.
+// slots in order.  Protected slots get the highest key, NaN the lowest; slots behind the
+// scores' width count as 0, what an untouched key has, so that no slot is lost there.
 struct EvictArgs {
   PagedCache c;
   const float* scores;
@@ -664,7 +665,7 @@ struct EvictArgs {
   int32_t* kept;
   int32_t* out_lens;
   float* out_scores;
-  int capacity, budget, first, last, out_width, out_capacity, held;  // held: keys a CTA has room for
+  int capacity, budget, first, last, out_width, out_capacity, held;  // scores' width; held: keys a CTA has room for
   int vec;    // scores of a (sequence, kv head) start on 16 bytes
   int chunk;  // rows a CTA of the move takes
 };
@@ -700,8 +701,8 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   __shared__ uint32_t found[2], totals[2], warps[2][kSel / 32];
   const int rank = blockIdx.x % kCluster, item = blockIdx.x / kCluster;
   const int b = item / a.c.heads;
-  const int n = min(a.c.len(b, 0), a.capacity);
-  const int want = min(n, a.budget);
+  const int n = a.c.len(b, 0);
+  const int want = min(n, min(a.budget, a.out_capacity));
   const float* scores = a.scores + (int64_t)item * a.capacity;
   // this CTA's slots [s0, s0 + mine)
   const int per = ((n + kCluster - 1) / kCluster + 3) / 4 * 4;
@@ -710,7 +711,9 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   // each warp takes a contiguous run of slots [w0, w1), 128 at a time: four neighbours a lane
   const int run = ((mine + kSel / 32 - 1) / (kSel / 32) + 127) / 128 * 128;
   const int w0 = min(mine, warp * run), w1 = min(mine, w0 + run), steps = (w1 - w0 + 127) / 128;
-  auto key_of = [&](int s, float x) -> uint32_t { return s < a.first || s >= n - a.last ? 0xffffffffu : score_key(x); };
+  auto key_of = [&](int s, float x) -> uint32_t {
+    return s < a.first || s >= n - a.last ? 0xffffffffu : score_key(s < a.capacity ? x : 0.f);
+  };
   auto load4 = [&](int i) -> float4 {  // scores of four slots, some perhaps behind the last
     const int s = s0 + i, top = a.capacity - 1;
     if (a.vec) return __ldg(reinterpret_cast<const float4*>(scores + min(s, top - 3)));
@@ -910,9 +913,9 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
         const uint32_t at = g + min(q, (uint32_t)need);
         kept[at] = slot + e;
         // the key gives the score back, but for protected slots and NaN
-        if (at < (uint32_t)a.out_capacity)
-          out[at] = k[e] == 0xffffffffu || k[e] == 0u ? scores[slot + e]
-                                                      : __uint_as_float(k[e] & 0x80000000u ? k[e] ^ 0x80000000u : ~k[e]);
+        out[at] = k[e] != 0xffffffffu && k[e] != 0u ? __uint_as_float(k[e] & 0x80000000u ? k[e] ^ 0x80000000u : ~k[e])
+                  : slot + e < a.capacity           ? scores[slot + e]
+                                                    : 0.f;
       }
       g += more, q += same;
     }
@@ -924,7 +927,7 @@ __global__ void __launch_bounds__(kSel) kv_select_kernel(const __grid_constant__
   for (int i = want + rank * kSel + threadIdx.x; i < a.out_capacity; i += kCluster * kSel) out[i] = 0.f;
   if (threadIdx.x == 0 && rank == 0 && item % a.c.heads == 0) {
     a.out_lens[b] = want;
-    if (want > a.out_capacity) record_status(a.c.status, BS_ERR_CAPACITY);
+    if (want < min(n, a.budget)) record_status(a.c.status, BS_ERR_CAPACITY);
   }
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -942,7 +945,7 @@ int select_launch(EvictArgs a, int items, cudaStream_t st) {
                                  kHeldMost * 8));
     if (dev < 64) set[dev] = true;
   }
-  const int per = (int)cdiv((int64_t)a.capacity, (int64_t)kCluster);
+  const int per = (int)cdiv((int64_t)a.c.capacity, (int64_t)kCluster);
   a.held = kFits ? (int)((per + 3) / 4 * 4 + 127) / 128 * 128 : 0;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
@@ -961,7 +964,7 @@ int select_launch(EvictArgs a, int items, cudaStream_t st) {
 
 template <int kCluster>
 int select_of(const EvictArgs& a, int items, cudaStream_t st) {
-  return cdiv((int64_t)a.capacity, (int64_t)kCluster) <= kHeldMost - 128 ? select_launch<kCluster, true>(a, items, st)
+  return cdiv((int64_t)a.c.capacity, (int64_t)kCluster) <= kHeldMost - 128 ? select_launch<kCluster, true>(a, items, st)
                                                                        : select_launch<kCluster, false>(a, items, st);
 }
 
@@ -1140,10 +1143,10 @@ extern "C" int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_
   //    64 items of 4096 19.8 / 18.9 / 24 / 61, of 32768 105 / 69 / 71 / 106, of 131072 300 / 178 / 169 / 222;
   //   256 items of 8192 108 / 115 / 137 / 283.
   int cluster = 1;
-  while (cluster < 8 && cluster * 4096 < capacity && items * cluster * 2 <= sm_count()) cluster *= 2;
+  while (cluster < 8 && cluster * 4096 < a.c.capacity && items * cluster * 2 <= sm_count()) cluster *= 2;
   BS_TRY(cluster == 1 ? select_of<1>(a, items, st) : cluster == 2 ? select_of<2>(a, items, st)
          : cluster == 4 ? select_of<4>(a, items, st) : select_of<8>(a, items, st));
-  const int64_t rows = std::min<int64_t>(budget, std::min<int64_t>(capacity, a.out_capacity));
+  const int64_t rows = std::min<int64_t>(budget, std::min(a.c.capacity, a.out_capacity));
   a.chunk = kMoveRows;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

@@ -457,11 +457,13 @@ int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int64_t T, int
  * their keys and values in ascending order to slots 0.. of out_page_table
  * [B, out_width] (pages of the same pool that hold no slot being read, except
  * that a sequence with n <= budget may keep its own pages).
- * scores [B, heads, capacity] f32 contiguous.  Outputs: kept [B, heads, budget]
+ * scores [B, heads, capacity] f32 contiguous; slots from capacity on, where the
+ * page table is wider, have the score 0.  Outputs: kept [B, heads, budget]
  * int32 (the kept slots, then -1), out_lens [B] int32 = min(n, budget),
  * out_scores [B, heads, out_width * page_size] f32 (the kept scores, then 0).
  * keep_first + keep_last <= budget <= out_width * page_size, or the budget may
- * exceed that where n cannot. */
+ * exceed that where n does not (a longer sequence is cut to the output pages and
+ * records BS_ERR_CAPACITY). */
 int bs_kv_evict(const bs_kv_cache* cache, const float* scores, int64_t capacity, int64_t budget,
                 int64_t keep_first, int64_t keep_last, const int32_t* out_page_table,
                 int64_t out_width, int32_t* kept, int32_t* out_lens, float* out_scores,

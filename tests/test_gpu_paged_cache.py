@@ -118,3 +118,60 @@ def test_append_drops_the_rows_of_a_page_outside_the_pool(bad):
     got = append_to(kc, vc, tab, L, g)
     assert kernels.device_status(clear=True) != 0
     check_append(kc, vc, *got, {**SECOND, (3, 6): (0, 0), (3, 7): (0, 1)})
+
+
+@pytest.mark.parametrize("lens,width,budget,first,last", [
+    ([100, 30, 0], 64, 40, 4, 8),       # longer than the scores, shorter, empty
+    ([100, 64, 65], 64, 40, 0, 40),     # only the last ones are protected, all of them without a score
+    ([100, 90], 32, 96, 0, 0),          # one sequence fits its budget
+    ([100, 99], 1, 50, 2, 3),           # nearly nothing is scored
+    ([9000], 100, 70, 1, 5),            # several CTAs to an item
+    ([9000], 8995, 4500, 0, 2),         # and scores that do not start on 16 bytes
+    ([60000] + [9] * 25, 40, 30, 1, 2), # not held in shared memory
+])
+def test_evict_counts_slots_behind_the_scores_as_zero(lens, width, budget, first, last):
+    """The scores may be narrower than the page table: a slot without one has the score 0."""
+    page, heads, D = 16, 3, 8
+    g = torch.Generator().manual_seed(width)
+    B, P, Q = len(lens), pages_for(max(lens), page), pages_for(min(budget, max(lens)), page)
+    order = torch.randperm(B * (P + Q), generator=g).to(torch.int32)
+    table, out = order[: B * P].view(B, P), order[B * P:].view(B, Q)
+    kc = torch.randn(B * (P + Q), page, heads, D, generator=g).bfloat16()
+    vc = torch.randn(B * (P + Q), page, heads, D, generator=g).bfloat16()
+    scores = torch.randn(B, heads, width, generator=g)      # negative ones rank below a slot without a score
+    full = torch.zeros(B, heads, P * page)
+    full[..., :width] = scores
+    k, v = to(kc, vc)
+    kept, new_lens, new = kernels.kv_evict(k, v, *to(table, torch.tensor(lens, dtype=torch.int32), scores), budget,
+                                           out.to(DEV), first, last)
+    want = oatt.evict(full, lens, budget, first, last)
+    wk, wv, ws = kc.clone(), vc.clone(), torch.zeros(B, heads, Q * page)
+    assert new_lens.tolist() == [min(n, budget) for n in lens]
+    for b in range(B):
+        for h in range(heads):
+            row = want[b][h]
+            assert kept[b, h].tolist() == row + [-1] * (budget - len(row)), (b, h)
+            i, j = torch.arange(len(row)), torch.tensor(row, dtype=torch.long)
+            at, src = (out[b].long()[i // page], i % page, h), (table[b].long()[j // page], j % page, h)
+            wk[at], wv[at], ws[b, h, : len(row)] = kc[src], vc[src], full[b, h, j]
+    assert torch.equal(k.cpu(), wk) and torch.equal(v.cpu(), wv) and torch.equal(new.cpu(), ws)
+
+
+def test_evict_to_fewer_pages_than_the_budget_is_reported():
+    """A budget beyond the output pages is accepted where the scores say that no sequence
+    needs them; one that does keeps its best slots, as many as the pages hold."""
+    page, g = 8, torch.Generator().manual_seed(5)
+    kc, vc = (torch.randn(9, page, 1, 8, generator=g).bfloat16() for _ in range(2))
+    table, out = torch.arange(6, dtype=torch.int32)[None], torch.tensor([[6, 7]], dtype=torch.int32)
+    scores = torch.rand(1, 1, 16, generator=g) + 1
+    k, v = to(kc, vc)
+    kept, lens, new = kernels.kv_evict(k, v, *to(table, torch.tensor([40], dtype=torch.int32), scores), 20, out.to(DEV), 1, 2)
+    assert kernels.device_status(clear=True) != 0
+    want = oatt.evict(torch.cat([scores, torch.zeros(1, 1, 32)], 2), [40], 16, 1, 2)[0][0]
+    assert int(lens) == 16 and kept[0, 0].tolist() == want + [-1] * 4
+    src = torch.tensor(want)
+    for c, d in ((kc, k), (vc, v)):
+        full = c.clone()
+        full[6:8] = c[src // page, src % page].view(2, page, 1, 8)
+        assert torch.equal(d.cpu(), full)
+    assert new.shape == (1, 1, 16) and new[0, 0].cpu().tolist() == [float(scores[0, 0, j]) if j < 16 else 0.0 for j in want]
