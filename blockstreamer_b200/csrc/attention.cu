@@ -581,9 +581,9 @@ constexpr int kTileThreads = 768;  // 16 softmax warps, loader, four issuing war
 constexpr int kSoftmaxRegs = 96, kOtherRegs = 48;
 constexpr float kRescale = 8.f;
 // One pair of exponentials in so many runs on the FMA pipe.  2 x 131072 keys, 16
-// drafts, heads of 64: 1/16 116.8 us, 1/8 117.2, 1/4 118.9; 8 x 16384 keys, 64
-// drafts, heads of 128: 92.0, 90.3, 89.2.
-constexpr int kPolyOf = 8;
+// drafts, heads of 64: 1/16 114.3 us, 1/8 115.4, 1/4 117.3; 8 x 16384 keys, 64
+// drafts, heads of 128: 90.2, 90.5, 90.6.
+constexpr int kPolyOf = 16;
 
 // A K x N operand whose N extent is contiguous (64 values = 128 bytes per row
 // of K, 128B-swizzled): 8-row groups 1024 bytes apart, 64-value panels `panel`.

@@ -267,15 +267,31 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return r;
 }
-// 2^x on the FMA pipe, for x in [-126, 126] (smaller x give 2^-126): x = n + f
-// with n the nearest integer, a quartic for 2^f on [-1/2, 1/2] fitted here to the
-// least largest relative error (2.6e-6), and n added to the exponent.  The
-// special-function unit gives 16 exponentials per clock and SM; a share of them
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n\t.reg .b64 x, y;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\t"
+      "mul.rn.f32x2 x, x, y;\n\tmov.b64 {%0, %1}, x;\n\t}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+// The larger, NaN where either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// 2^x on the FMA pipe for x up to 126: x = n + f with n the nearest integer, a quartic
+// for 2^f on [-1/2, 1/2] fitted here to the least largest relative error (2.6e-6), times
+// 2^n, whose bits are the low ones of the rounding sum moved to the exponent.  As with
+// ex2.approx.ftz, what lies below the normal numbers is 0 (n of -127 has the exponent
+// bits 0, so a masked score of -inf has no weight at all) and NaN gives NaN.
+// The special-function unit gives 16 exponentials per clock and SM; a share of them
 // computed here shortens a softmax step, and the weights are rounded to bf16.
 __device__ __forceinline__ float2 exp2_poly(float2 x) {
-  x.x = fmaxf(x.x, -126.f);
-  x.y = fmaxf(x.y, -126.f);
-  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are n
+  x.x = max_nan(x.x, -127.f);
+  x.y = max_nan(x.y, -127.f);
+  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23 and the exponent's bias
   const float2 t = add2(x, make_float2(kRound, kRound));
   const float2 n = add2(t, make_float2(-kRound, -kRound));
   const float2 f = add2(x, make_float2(-n.x, -n.y));
@@ -283,8 +299,7 @@ __device__ __forceinline__ float2 exp2_poly(float2 x) {
   y = fma2(y, f, 0.240247443318367f);
   y = fma2(y, f, 0.6931217908859253f);
   y = fma2(y, f, 0.9999992847442627f);
-  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(y.x)),
-                     __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(y.y)));
+  return mul2(y, make_float2(__uint_as_float(__float_as_uint(t.x) << 23), __uint_as_float(__float_as_uint(t.y) << 23)));
 }
 // 16-byte asynchronous copy; zero bytes are read and zeros written when !on.
 __device__ __forceinline__ void cp_async_16_or_zero(uint32_t dst, const void* src, bool on) {
