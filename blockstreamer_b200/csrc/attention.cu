@@ -8,7 +8,9 @@
 // sum z of the softmax (base 2): with x_j = scale log2(e) q . k_j,
 //   m' = max(m, max_j x_j);  z' = z 2^(m-m') + sum_j 2^(x_j-m');
 //   O' = O 2^(m-m') + sum_j 2^(x_j-m') v_j,     out = O / (z + 2^(sink-m)).
-// Partial (m, z, O) of key ranges join by the same rule, in a fixed order.
+// Partial (m, z, O) of key ranges join by the same rule, in a fixed order.  A maximum
+// passes over NaN, a sum does not: a part has nothing to add where z is 0, not where m
+// is -inf, which a part whose every score is NaN has too.
 //
 // Work split: the keys of every (sequence, kv head, row tile) are cut into
 // units; the units of all items, in item order, are cut into equal contiguous
@@ -450,7 +452,7 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const float2 v = ml[w * kRows + row];
-          zz += v.x > -INFINITY ? v.y * mma::exp2_fast(v.x - mx) : 0.f;
+          zz += v.y != 0.f ? v.y * mma::exp2_fast(v.x - mx) : 0.f;
         }
         const float f = mx == -INFINITY ? 0.f : mma::exp2_fast(m[mt][e] - mx);
 #pragma unroll
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
           const float ref = top == -INFINITY ? 0.f : top;
           const float f = mx == -INFINITY ? 0.f : mma::exp2_fast(mx - ref);
           const float den = z[mt][e] * f + (a.sinks ? mma::exp2_fast(sink[mt][e] - ref) : 0.f);
-          const float g = pt[mt][e] >= 0 && mx > -INFINITY ? f / den : 0.f;
+          const float g = pt[mt][e] >= 0 && z[mt][e] != 0.f ? f / den : 0.f;
 #pragma unroll
           for (int d = 0; d < DP / 8; ++d)
             if (d * 8 < dim)
@@ -1031,8 +1033,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         auto both = [&](int x) {
           const float2 u = ml[2 * x * 128], v = ml[(2 * x + 1) * 128];
           const float top = fmaxf(u.x, v.x);
-          const float zz = (u.x == -INFINITY ? 0.f : u.y * mma::exp2_fast(u.x - top)) +
-                           (v.x == -INFINITY ? 0.f : v.y * mma::exp2_fast(v.x - top));
+          const float zz = (u.y == 0.f ? 0.f : u.y * mma::exp2_fast(u.x - top)) +
+                           (v.y == 0.f ? 0.f : v.y * mma::exp2_fast(v.x - top));
           return make_float2(top, zz);
         };
         float f0 = 1.f, f1 = 0.f;
@@ -1059,7 +1061,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           const float ref = top == -INFINITY ? 0.f : top;
           const float f = m == -INFINITY ? 0.f : mma::exp2_fast(m - ref);
           const float den = z * f + (a.sinks ? mma::exp2_fast(sink - ref) : 0.f);
-          scale_o = used && m > -INFINITY ? f / den : 0.f;
+          scale_o = used && z != 0.f ? f / den : 0.f;
           if (a.lse && speaks) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;
         }
         if (!whole && speaks) a.part_ml[slot * kRows + row] = make_float2(m, z);
@@ -1206,14 +1208,14 @@ __global__ void __launch_bounds__(JoinCfg<kSplit>::kThreads) tree_join_kernel(co
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (x + j * kSplit <= c1) top = fmaxf(top, mz[j].x);
-    if (top == -INFINITY) continue;
-    const float f = mma::exp2_fast(m - top);
+    const float ref = top == -INFINITY ? 0.f : top;
+    const float f = mma::exp2_fast(m - ref);
     z *= f, v.x *= f, v.y *= f, v.z *= f, v.w *= f;
     m = top;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
-      if (x + j * kSplit > c1 || mz[j].x == -INFINITY) continue;
-      const float g = mma::exp2_fast(mz[j].x - m);
+      if (x + j * kSplit > c1 || mz[j].y == 0.f) continue;
+      const float g = mma::exp2_fast(mz[j].x - ref);
       z += mz[j].y * g, v.x += p[j].x * g, v.y += p[j].y * g, v.z += p[j].z * g, v.w += p[j].w * g;
     }
   }
@@ -1235,7 +1237,7 @@ __global__ void __launch_bounds__(JoinCfg<kSplit>::kThreads) tree_join_kernel(co
   if (part || row >= rows || c >= dim / 4) return;
   const float den = z + (a.sinks ? mma::exp2_fast(sink - ref) : 0.f);
   uint2 w = make_uint2(0u, 0u);
-  if (used && mx > -INFINITY) w = make_uint2(pack_bf16x2(v.x / den, v.y / den), pack_bf16x2(v.z / den, v.w / den));
+  if (used && z != 0.f) w = make_uint2(pack_bf16x2(v.x / den, v.y / den), pack_bf16x2(v.z / den, v.w / den));
   const int64_t at = ((int64_t)b * a.T + t) * a.Hkv * a.G + hq;
   *reinterpret_cast<uint2*>(a.out + at * dim + c * 4) = w;
   if (c == 0 && a.lse) a.lse[at] = used ? ref * kLn2 + logf(den) : -INFINITY;

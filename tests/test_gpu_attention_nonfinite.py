@@ -70,3 +70,64 @@ def test_a_key_of_nan_that_is_attended_is_seen_at_every_slot(T, Hq, D, slots):
     got, lse = kernels.tree_attention(*to(q, kc, vc, far(table, page, slots) if slots else table, L, chain(L, T)))
     assert bool(got[:66].isnan().all()) and bool(lse[:66].isnan().all())
     assert bool(got[66].isfinite().all()) and bool(lse[66].isfinite().all())
+
+
+@pytest.mark.parametrize("T,Hq,D", ROWS)
+@pytest.mark.parametrize("slots", [0, 5000])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_a_row_whose_every_score_is_nan_is_nan(T, Hq, D, slots, sinks):
+    """A query of NaN, in one sequence's first row; one whose only key is NaN; rows beside
+    them keep their values."""
+    page, lens = 16, [50, 0, 333]
+    kc, vc, table, L, g = make_cache(lens, T, 1, D, page, T + D)
+    q = torch.randn(3, T, Hq, D, generator=g).bfloat16()
+    q[0, 0, 0] = math.nan
+    kc[int(table[1, 0]), 0] = math.nan
+    pos = chain(L, T)
+    s = torch.randn(Hq, generator=g) if sinks else None
+    want, wlse, spread = oatt.tree_attention(q, kc, vc, table, L, pos, None, s)
+    got, lse = kernels.tree_attention(*to(q, kc, vc, far(table, page, slots) if slots else table, L, pos), sinks=to(s)[0])
+    got, lse = got.double().cpu(), lse.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(lse.isnan(), wlse.isnan())
+    assert bool(want[0, 0, 0].isnan().all()) and bool(want[1].isnan().all())
+    ok = ~want.isnan()
+    assert bool(((got - want)[ok].abs() <= (2.0 ** -8 * (want.abs() + spread) + 1e-6)[ok]).all())
+
+
+@pytest.mark.parametrize("T,Hq,D", ROWS)
+@pytest.mark.parametrize("first,last", [(0, 1024), (1024, 2048), (0, 1500)])
+def test_a_piece_of_the_keys_that_is_all_nan_is_not_lost(T, Hq, D, first, last):
+    """Keys that several CTAs share, of which some have nothing but NaN."""
+    page, n = 64, 3000
+    g = torch.Generator(device=DEV).manual_seed(T)
+    P = -(-(n + T) // page)
+    kc, vc = (torch.randn(P, page, 1, D, generator=g, device=DEV).bfloat16() for _ in range(2))
+    kc.view(-1, 1, D)[first:last] = math.nan
+    table = torch.arange(P, dtype=torch.int32, device=DEV)[None]
+    L = torch.tensor([n], dtype=torch.int32)
+    q = torch.randn(1, T, Hq, D, generator=g, device=DEV).bfloat16()
+    got, lse = kernels.tree_attention(q, kc, vc, table, *to(L, chain(L, T)))
+    assert bool(got.isnan().all()) and bool(lse.isnan().all())
+
+
+@pytest.mark.parametrize("T,Hq,D", ROWS)
+@pytest.mark.parametrize("slots", [0, 5000])
+def test_keys_of_minus_infinity_are_as_if_they_were_not_there(T, Hq, D, slots):
+    """Scores of -inf: weight zero; where a row has no others, 0 and the sink (or -inf)."""
+    page, lens = 16, [200, 40]
+    kc, vc, table, L, g = make_cache(lens, T, 1, D, page, T + D)
+    q = torch.rand(2, T, Hq, D, generator=g).bfloat16() + 0.5
+    for j in range(150):
+        kc[int(table[0, j // page]), j % page] = -math.inf
+    for j in range(40 + T):
+        kc[int(table[1, j // page]), j % page] = -math.inf
+    pos = chain(L, T)
+    for s in (None, torch.linspace(-1, 1, Hq)):
+        want, wlse, spread = oatt.tree_attention(q, kc, vc, table, L, pos, None, s)
+        got, lse = kernels.tree_attention(*to(q, kc, vc, far(table, page, slots) if slots else table, L, pos), sinks=to(s)[0])
+        got, lse = got.double().cpu(), lse.double().cpu()
+        assert bool((got[1] == 0).all()) and bool(got[0].isfinite().all())
+        assert bool(((got - want).abs() <= 2.0 ** -8 * (want.abs() + spread) + 1e-6).all())
+        on = wlse > -math.inf
+        assert torch.equal(lse > -math.inf, on)
+        assert bool(((lse - wlse)[on].abs() <= 2e-5 * (1 + wlse[on].abs())).all())
