@@ -75,25 +75,30 @@ class _Rotary(torch.autograd.Function):
     """bs_rope forward; the gradient is the turn by the opposite angle."""
 
     @staticmethod
-    def forward(ctx, q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interleaved: bool):
+    def forward(ctx, q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interleaved: bool,
+                inverse: bool = False):
         ctx.save_for_backward(table, positions)
-        ctx.interleaved = interleaved
-        return kernels.rope(q, k, table, positions, interleaved)
+        ctx.turn = interleaved, inverse
+        return kernels.rope(q, k, table, positions, interleaved, inverse)
 
     @staticmethod
     def backward(ctx, dq: Tensor, dk: Tensor | None):
         # gradients that did not arrive are zeros here (autograd makes them); dk is None without k
         table, positions = ctx.saved_tensors
+        interleaved, inverse = ctx.turn
         dq = dq if dq.stride(-1) == 1 else dq.contiguous()
         if dk is not None and dk.stride(-1) != 1:
             dk = dk.contiguous()
-        gq, gk = kernels._rope(dq.get_device(), dq, dk, table, positions, ctx.interleaved, True)
-        return gq, gk, None, None, None
+        if torch.is_grad_enabled():  # create_graph: the turn back has a gradient of its own
+            gq, gk = _Rotary.apply(dq, dk, table, positions, interleaved, not inverse)
+        else:
+            gq, gk = kernels._rope(dq.get_device(), dq, dk, table, positions, interleaved, not inverse)
+        return gq, gk, None, None, None, None
 
 
 def apply_rotary(q: Tensor, k: Tensor | None, table: Tensor, positions: Tensor, interleaved: bool = False):
-    """Rotary positions of q and k with gradients (``kernels.rope`` both ways).
-    No gradient flows to the table."""
+    """Rotary positions of q and k with gradients of any order (``kernels.rope`` both
+    ways).  No gradient flows to the table."""
     return _Rotary.apply(q, k, table, positions, interleaved)
 
 
