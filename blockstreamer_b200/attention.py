@@ -197,7 +197,8 @@ class B200GptOssAttention(nn.Module):
     (or one token) of every sequence against the cached ones.
 
     Parameters ``q_proj``, ``k_proj``, ``v_proj``, ``o_proj`` (weight and bias) and
-    ``sinks`` have transformers' names and shapes, on ``meta`` until bound."""
+    ``sinks`` have transformers' names and shapes, on ``meta`` until bound.  It serves
+    decoding and has no backward pass: one that reaches its attention raises."""
 
     def __init__(self, config, layer_idx: int = 0, dtype: torch.dtype = torch.bfloat16) -> None:
         super().__init__()

@@ -427,7 +427,9 @@ def mxfp4_matmul_backward(grad_out: torch.Tensor, blocks: torch.Tensor, scales: 
 # ---------------------------------------------------------------- attention half of the decoder layer
 # These run at every layer of a decoding step, where the host's time counts:
 # arguments are passed as plain integers (the signatures convert them), and the
-# device context is entered only when another device is current.
+# device context is entered only when another device is current.  None of them
+# records a gradient (attention.apply_rotary does); where one is asked of an
+# input, a backward pass through the outputs raises.
 def _ptr(t: torch.Tensor | None):
     return None if t is None else t.data_ptr()
 
@@ -451,6 +453,20 @@ def _device_index(name: str, first: torch.Tensor, *others: torch.Tensor | None) 
             raise ValueError(f"{name}: tensors on {first.device} and {t.device}; blockstreamer_b200 runs on CUDA "
                              "tensors only, of one device")
     return index
+
+
+class _NoBackward(torch.autograd.Function):
+    """Outputs of an operator that records no gradient although one is asked of its inputs:
+    a backward pass that reaches them raises, where it would otherwise go on without them."""
+
+    @staticmethod
+    def forward(ctx, message: str, outputs: tuple, *inputs: torch.Tensor | None):
+        ctx.message = message
+        return outputs
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(ctx.message)
 
 
 def _heads(name: str, t: torch.Tensor | None):
@@ -519,7 +535,10 @@ def rope(q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions
     if q.dtype not in (torch.bfloat16, torch.float32):
         raise ValueError("rope: q and k must be bf16 or f32")
     _rope_table("rope", table, q.shape[-1])
-    return _rope(index, q, k, table, _positions("rope", positions, q.shape[:-2]), interleaved, inverse)
+    out = _rope(index, q, k, table, _positions("rope", positions, q.shape[:-2]), interleaved, inverse)
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+        return _NoBackward.apply("kernels.rope records no gradient: attention.apply_rotary does", out, q, k)
+    return out
 
 
 def _rope(index: int, q: torch.Tensor, k: torch.Tensor | None, table: torch.Tensor, positions: torch.Tensor,
@@ -560,6 +579,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, table: torch.
     _launch("bs_rope_append", index, _heads("rope_append", q), _heads("rope_append", k), _heads("rope_append", v),
             _heads("rope_append", qo), cache, T, Hq, _ptr(table), table.shape[0], rot, _ptr(positions),
             _DT[positions.dtype], interleaved)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _NoBackward.apply("rope_append has no backward pass: it serves decoding", (qo,), q, k, v)[0]
     return qo
 
 
@@ -598,6 +619,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _launch("bs_tree_attention", index, _heads("tree_attention", q), cache, T, Hq, _ptr(positions), _ptr(tree_mask),
             mask_stride, _ptr(sinks), window, D ** -0.5 if scale is None else scale, _ptr(out), _ptr(lse), _ptr(ws),
             ws_bytes)
+    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad
+                                    or sinks is not None and sinks.requires_grad):
+        return _NoBackward.apply("tree_attention has no backward pass: it serves decoding", (out, lse), q, k_cache,
+                                 v_cache, sinks)
     return out, lse
 
 
@@ -639,13 +664,18 @@ def kv_scores_add(scores: torch.Tensor, q: torch.Tensor, lse: torch.Tensor, k_ca
     scores, lse = _contig("kv_scores_add: scores", scores), _contig("kv_scores_add: lse", lse)
     if accepted is not None:
         accepted = _contig("kv_scores_add: accepted", accepted)
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty_like(scores)
     elif out.shape != scores.shape or out.dtype != scores.dtype or not out.is_contiguous():
         raise ValueError("kv_scores_add: out must be contiguous and of the shape of scores")
     _launch("bs_kv_scores_add", index, _heads("kv_scores_add", q), cache, T, Hq, _ptr(lse), _ptr(accepted),
             T if accepted is None else accepted.shape[1], D ** -0.5 if scale is None else scale, _ptr(scores),
             _ptr(out), scores.shape[2])
+    if fresh and torch.is_grad_enabled() and (scores.requires_grad or q.requires_grad or lse.requires_grad
+                                              or k_cache.requires_grad):
+        return _NoBackward.apply("kv_scores_add has no backward pass: it serves decoding", (out,), scores, q, lse,
+                                 k_cache)[0]
     return out
 
 
