@@ -158,6 +158,14 @@ class PagedKVCache:
     def commit(self, accepted: list[list[int]], drafted: int, q: Tensor | None = None, lse: Tensor | None = None) -> None:
         """Keeps the accepted drafts (ascending indices per sequence) and, given the
         step's turned ``q`` and its ``lse``, adds their attention to the scores."""
+        if len(accepted) != len(self.lengths):
+            raise ValueError(f"commit takes {len(self.lengths)} lists of accepted drafts, got {len(accepted)}")
+        for x, n, held in zip(accepted, self.lengths, self._held):
+            # the device would leave such a sequence as it is, but not know its new length
+            if any(v <= u for u, v in zip([-1] + x, x + [drafted])):
+                raise ValueError(f"accepted drafts must ascend from 0 to below {drafted}, got {x}")
+            if x and n + x[-1] >= len(held) * self.page_size:
+                raise ValueError(f"draft {x[-1]} behind {n} keys lies outside the {len(held)} reserved pages")
         most = max((len(x) for x in accepted), default=0)
         if most:
             rows = [x + [-1] * (most - len(x)) for x in accepted]

@@ -1,0 +1,65 @@
+"""The host side of PagedKVCache, on the CPU with the operators replaced by recorders:
+what it refuses, and that a refused call leaves the cache as it was."""
+
+import copy
+
+import pytest
+import torch
+
+from blockstreamer_b200 import attention
+from blockstreamer_b200.attention import PagedKVCache
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    made = []
+
+    class Recorder:
+        def tree_commit(self, *a, **kw):
+            made.append("commit")
+
+        def kv_scores_add(self, *a, **kw):
+            made.append("scores")
+
+    monkeypatch.setattr(attention, "kernels", Recorder())
+    return made
+
+
+def cache(batch=2, pages=12, page_size=4, max_len=24, **kw):
+    c = PagedKVCache(batch, pages, page_size, 1, 32, max_len, "cpu", **kw)
+    c.reserve(5)
+    return c
+
+
+def state(c):
+    return (list(c.lengths), c.lens.tolist(), c.page_table.tolist(), sorted(c._free), copy.deepcopy(c._held),
+            None if c.scores is None else c.scores.clone().tolist())
+
+
+@pytest.mark.parametrize("accepted,drafted,text", [
+    ([[0, 2], [1, 1]], 5, "ascend"),
+    ([[2, 1], []], 5, "ascend"),
+    ([[0], [3, 5]], 5, "ascend"),
+    ([[-1, 0], [0]], 5, "ascend"),
+    ([[0]], 5, "2 lists"),
+    ([[0], [1], [2]], 5, "2 lists"),
+    ([], 5, "2 lists"),
+    ([[0], [7, 8]], 9, "reserved"),   # two pages of four slots are
+])
+def test_commit_refuses_what_the_device_would_not_move(calls, accepted, drafted, text):
+    c = cache(track_scores=True)
+    before = state(c)
+    with pytest.raises(ValueError, match=text):
+        c.commit(accepted, drafted, torch.zeros(1), torch.zeros(1))
+    assert state(c) == before and calls == []
+
+
+def test_commit_advances_the_lengths(calls):
+    c = cache(track_scores=True)
+    c.commit([[0, 2, 4], []], 5, torch.zeros(1), torch.zeros(1))
+    assert c.lengths == [3, 0] and c.lens.tolist() == [3, 0] and calls == ["commit", "scores"]
+    c.commit([[], []], 5)
+    assert c.lengths == [3, 0] and calls == ["commit", "scores"]
+    c.reserve(2)
+    c.commit([[0, 1], [1]], 2)
+    assert c.lengths == [5, 1] and calls == ["commit", "scores", "commit"]
