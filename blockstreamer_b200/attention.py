@@ -184,7 +184,9 @@ class PagedKVCache:
         new = [-(-min(n, budget) // self.page_size) for n in self.lengths]
         if sum(new) > len(self._free):
             raise RuntimeError(f"eviction needs {sum(new)} free pages, {len(self._free)} are")
-        taken = [[self._free.pop() for _ in range(x)] for x in new]
+        # (the pages leave the free list when the call has been accepted)
+        pages = reversed(self._free)
+        taken = [[next(pages) for _ in range(x)] for x in new]
         width = max(1, max(new, default=0))
         out = torch.tensor([t + [0] * (width - len(t)) for t in taken], dtype=torch.int32, device=self.k.device)
         budget = min(budget, width * self.page_size)
@@ -192,6 +194,7 @@ class PagedKVCache:
                                            min(keep_first, budget), min(keep_last, budget - min(keep_first, budget)))
         self.scores.zero_()
         self.scores[..., : scores.shape[-1]] = scores
+        del self._free[len(self._free) - sum(new):]
         for held in self._held:
             self._free.extend(held)
         self._held = taken

@@ -63,3 +63,38 @@ def test_commit_advances_the_lengths(calls):
     c.reserve(2)
     c.commit([[0, 1], [1]], 2)
     assert c.lengths == [5, 1] and calls == ["commit", "scores", "commit"]
+
+
+def evicting(monkeypatch, refuse=False):
+    """kv_evict's shapes, or a refusal after its arguments are there."""
+    def kv_evict(k, v, page_table, lens, scores, budget, out, keep_first=0, keep_last=0):
+        made.append((budget, keep_first, keep_last, out.clone()))
+        if refuse:
+            raise ValueError("refused")
+        kept = torch.full((*scores.shape[:2], budget), -1, dtype=torch.int32)
+        return kept, lens, torch.zeros(*scores.shape[:2], out.shape[1] * k.shape[1])
+
+    made = []
+    monkeypatch.setattr(attention.kernels, "kv_evict", kv_evict)
+    return made
+
+
+def filled(lengths, pages=12, page_size=4, max_len=24):
+    c = PagedKVCache(len(lengths), pages, page_size, 1, 32, max_len, "cpu", track_scores=True)
+    c.lengths = [0] * len(lengths)
+    for b, n in enumerate(lengths):
+        c._held[b].extend(c._free.pop() for _ in range(-(-n // page_size)))
+    c.lengths = list(lengths)
+    c._upload()
+    return c
+
+
+def test_a_refused_eviction_loses_no_pages(monkeypatch):
+    made = evicting(monkeypatch, refuse=True)
+    c = filled([10, 5])
+    before = state(c)
+    with pytest.raises(ValueError, match="refused"):
+        c.evict(6, keep_first=1, keep_last=2)
+    assert len(made) == 1
+    after = state(c)
+    assert after[:3] == before[:3] and after[3] == before[3] and after[4:] == before[4:]
