@@ -176,11 +176,17 @@ class PagedKVCache:
         self.lengths = [n + len(x) for n, x in zip(self.lengths, accepted)]
         self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
 
-    def evict(self, budget: int, keep_first: int = 4, keep_last: int = 0) -> Tensor:
-        """Cuts every sequence to its ``budget`` best keys per head; returns the kept
-        slots.  Only for layers without a window: slots are no longer positions."""
+    def evict(self, budget: int, keep_first: int | None = None, keep_last: int = 0) -> Tensor:
+        """Cuts every sequence to its ``budget`` best keys per head, the first
+        ``keep_first`` (by default four, or what ``keep_last`` leaves of the budget for
+        them) and the last ``keep_last`` among them; returns the kept slots.  Only for
+        layers without a window: slots are no longer positions."""
         if self.scores is None:
             raise ValueError("PagedKVCache.evict needs track_scores=True")
+        if keep_first is None:
+            keep_first = min(4, max(0, budget - keep_last))
+        if keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
+            raise ValueError(f"keep_first {keep_first} + keep_last {keep_last} must not exceed the budget {budget}")
         new = [-(-min(n, budget) // self.page_size) for n in self.lengths]
         if sum(new) > len(self._free):
             raise RuntimeError(f"eviction needs {sum(new)} free pages, {len(self._free)} are")
@@ -189,9 +195,11 @@ class PagedKVCache:
         taken = [[next(pages) for _ in range(x)] for x in new]
         width = max(1, max(new, default=0))
         out = torch.tensor([t + [0] * (width - len(t)) for t in taken], dtype=torch.int32, device=self.k.device)
+        # a budget that no sequence reaches cuts nothing, whatever is protected
         budget = min(budget, width * self.page_size)
+        keep_first = min(keep_first, budget)
         kept, _, scores = kernels.kv_evict(self.k, self.v, self.page_table, self.lens, self.scores, budget, out,
-                                           min(keep_first, budget), min(keep_last, budget - min(keep_first, budget)))
+                                           keep_first, min(keep_last, budget - keep_first))
         self.scores.zero_()
         self.scores[..., : scores.shape[-1]] = scores
         del self._free[len(self._free) - sum(new):]

@@ -98,3 +98,36 @@ def test_a_refused_eviction_loses_no_pages(monkeypatch):
     assert len(made) == 1
     after = state(c)
     assert after[:3] == before[:3] and after[3] == before[3] and after[4:] == before[4:]
+
+
+@pytest.mark.parametrize("kw,first,last", [
+    (dict(), 4, 0),                             # by default the first four
+    (dict(keep_last=4), 2, 4),                  # or as many of them as the last ones leave
+    (dict(keep_last=6), 0, 6),
+    (dict(keep_first=2, keep_last=4), 2, 4),
+    (dict(keep_first=0), 0, 0),
+])
+def test_evict_protects_what_it_was_asked_to(monkeypatch, kw, first, last):
+    made = evicting(monkeypatch)
+    filled([10, 7]).evict(6, **kw)
+    assert [m[:3] for m in made] == [(6, first, last)]
+
+
+@pytest.mark.parametrize("kw", [dict(keep_first=7), dict(keep_last=7), dict(keep_first=3, keep_last=4),
+                                dict(keep_first=-1), dict(keep_last=-1), dict(keep_first=6, keep_last=1)])
+def test_evict_refuses_more_protected_slots_than_the_budget(monkeypatch, kw):
+    made = evicting(monkeypatch)
+    c = filled([10, 7])
+    before = state(c)
+    with pytest.raises(ValueError, match="keep_first"):
+        c.evict(6, **kw)
+    assert made == [] and state(c) == before
+
+
+def test_evict_with_a_budget_beyond_every_sequence(monkeypatch):
+    """Nothing is cut, so what is protected is all the same: the call's budget is what the pages hold."""
+    made = evicting(monkeypatch)
+    c = filled([3, 6])
+    c.evict(500, keep_first=100, keep_last=300)
+    budget, first, last, _ = made[0]
+    assert budget == 8 and first + last <= 8 and c.lengths == [3, 6]
