@@ -187,12 +187,15 @@ class PagedKVCache:
             keep_first = min(4, max(0, budget - keep_last))
         if keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
             raise ValueError(f"keep_first {keep_first} + keep_last {keep_last} must not exceed the budget {budget}")
+        # a sequence within the budget keeps the pages of its slots; the others' new ones
+        # leave the free list when the call has been accepted
         new = [-(-min(n, budget) // self.page_size) for n in self.lengths]
-        if sum(new) > len(self._free):
-            raise RuntimeError(f"eviction needs {sum(new)} free pages, {len(self._free)} are")
-        # (the pages leave the free list when the call has been accepted)
+        need = sum(x for x, n in zip(new, self.lengths) if n > budget)
+        if need > len(self._free):
+            raise RuntimeError(f"eviction needs {need} free pages, {len(self._free)} are")
         pages = reversed(self._free)
-        taken = [[next(pages) for _ in range(x)] for x in new]
+        taken = [[next(pages) for _ in range(x)] if n > budget else held[:x]
+                 for x, n, held in zip(new, self.lengths, self._held)]
         width = max(1, max(new, default=0))
         out = torch.tensor([t + [0] * (width - len(t)) for t in taken], dtype=torch.int32, device=self.k.device)
         # a budget that no sequence reaches cuts nothing, whatever is protected
@@ -202,9 +205,9 @@ class PagedKVCache:
                                            keep_first, min(keep_last, budget - keep_first))
         self.scores.zero_()
         self.scores[..., : scores.shape[-1]] = scores
-        del self._free[len(self._free) - sum(new):]
-        for held in self._held:
-            self._free.extend(held)
+        del self._free[len(self._free) - need:]
+        for x, n, held in zip(new, self.lengths, self._held):
+            self._free.extend(held if n > budget else held[x:])
         self._held = taken
         self.lengths = [min(n, budget) for n in self.lengths]
         self._upload()

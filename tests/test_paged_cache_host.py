@@ -131,3 +131,34 @@ def test_evict_with_a_budget_beyond_every_sequence(monkeypatch):
     c.evict(500, keep_first=100, keep_last=300)
     budget, first, last, _ = made[0]
     assert budget == 8 and first + last <= 8 and c.lengths == [3, 6]
+
+
+def test_evict_needs_pages_only_for_what_it_cuts(monkeypatch):
+    """Sequences within the budget keep their pages, those of their slots; a nearly full
+    pool, where eviction is wanted, is enough for the others."""
+    made = evicting(monkeypatch)
+    c = filled([16, 6, 0, 8], pages=10)     # 4 + 2 + 0 + 2 pages held, 2 free
+    c._held[3].append(c._free.pop())        # and one reserved behind sequence 3: one free
+    with pytest.raises(RuntimeError, match="needs 2 free pages, 1 are"):
+        c.evict(8)
+    own = [list(h) for h in c._held]
+    assert made == []
+    c._free.append(c._held[3].pop())
+    spare = sorted(c._free)
+    c.evict(8)
+    out = made[0][3]
+    assert c.lengths == [8, 6, 0, 8] and sorted(c._held[0]) == spare
+    assert c._held[1] == own[1] and c._held[2] == [] and c._held[3] == own[3][:2]
+    assert out[1].tolist() == own[1] and out[3].tolist() == own[3][:2] and out[0].tolist() == c._held[0]
+    assert sorted(c._free) == sorted(own[0])
+    assert c.page_table[3, :2].tolist() == own[3][:2] and c.lens.tolist() == [8, 6, 0, 8]
+
+
+def test_evict_frees_pages_reserved_behind_a_short_sequence(monkeypatch):
+    evicting(monkeypatch)
+    c = filled([3])
+    c.reserve(9)
+    assert len(c._held[0]) == 3
+    first = c._held[0][0]
+    c.evict(100)
+    assert c._held == [[first]] and len(c._free) == 11
