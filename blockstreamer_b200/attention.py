@@ -108,7 +108,8 @@ class PagedKVCache:
     Pages are [page, head, slot, dim] in memory, so that a head's slots of a page
     lie together.  The host keeps the lengths and hands out the pages; what the
     kernels read (``page_table``, ``lens``) is on the device.  ``scores`` (with
-    ``track_scores``) accumulates the attention weight of every cached key."""
+    ``track_scores``) accumulates the attention weight of every cached key; scores and
+    eviction are for layers without a window."""
 
     def __init__(self, batch: int, pages: int, page_size: int, heads: int, dim: int, max_len: int, device="cuda",
                  track_scores: bool = False) -> None:
@@ -125,6 +126,8 @@ class PagedKVCache:
         self.lengths = [0] * batch                      # the host's copy of lens
         self._free = list(range(pages - 1, -1, -1))
         self._held: list[list[int]] = [[] for _ in range(batch)]
+        self._windowed = False                          # a window has left keys out
+        self._cut = False                               # slots are no longer positions
 
     def _upload(self) -> None:
         rows = [h + [0] * (self.width - len(h)) for h in self._held]
@@ -152,12 +155,19 @@ class PagedKVCache:
     def attend(self, q: Tensor, positions: Tensor, tree_mask: Tensor | None = None, sinks: Tensor | None = None,
                window: int = 0):
         """(out, lse) of the drafted tokens whose keys ``append`` wrote."""
+        if window:
+            if self._cut:
+                raise ValueError("attend: after evict slots are no longer positions, by which a window goes")
+            self._windowed = self._windowed or max(self.lengths, default=0) + q.shape[1] > window
         return kernels.tree_attention(q, self.k, self.v, self.page_table, self.lens, positions, tree_mask, sinks,
                                       window)
 
     def commit(self, accepted: list[list[int]], drafted: int, q: Tensor | None = None, lse: Tensor | None = None) -> None:
         """Keeps the accepted drafts (ascending indices per sequence) and, given the
         step's turned ``q`` and its ``lse``, adds their attention to the scores."""
+        scored = self.scores is not None and q is not None and lse is not None
+        if scored and self._windowed:
+            raise ValueError("commit: keys outside a window got no weight that could be added to their scores")
         if len(accepted) != len(self.lengths):
             raise ValueError(f"commit takes {len(self.lengths)} lists of accepted drafts, got {len(accepted)}")
         for x, n, held in zip(accepted, self.lengths, self._held):
@@ -171,7 +181,7 @@ class PagedKVCache:
             rows = [x + [-1] * (most - len(x)) for x in accepted]
             acc = torch.tensor(rows, dtype=torch.int32, device=self.k.device)
             kernels.tree_commit(self.k, self.v, self.page_table, self.lens, acc, drafted)
-            if self.scores is not None and q is not None and lse is not None:
+            if scored:
                 kernels.kv_scores_add(self.scores, q, lse, self.k, self.page_table, self.lens, acc, out=self.scores)
         self.lengths = [n + len(x) for n, x in zip(self.lengths, accepted)]
         self.lens.copy_(torch.tensor(self.lengths, dtype=torch.int32))
@@ -183,6 +193,8 @@ class PagedKVCache:
         layers without a window: slots are no longer positions."""
         if self.scores is None:
             raise ValueError("PagedKVCache.evict needs track_scores=True")
+        if self._windowed:
+            raise ValueError("evict is for layers without a window")
         if keep_first is None:
             keep_first = min(4, max(0, budget - keep_last))
         if keep_first < 0 or keep_last < 0 or keep_first + keep_last > budget:
@@ -209,6 +221,7 @@ class PagedKVCache:
         for x, n, held in zip(new, self.lengths, self._held):
             self._free.extend(held if n > budget else held[x:])
         self._held = taken
+        self._cut = self._cut or need > 0
         self.lengths = [min(n, budget) for n in self.lengths]
         self._upload()
         return kept

@@ -162,3 +162,44 @@ def test_evict_frees_pages_reserved_behind_a_short_sequence(monkeypatch):
     first = c._held[0][0]
     c.evict(100)
     assert c._held == [[first]] and len(c._free) == 11
+
+
+def attending(monkeypatch):
+    monkeypatch.setattr(attention.kernels, "tree_attention", lambda *a: ("out", "lse"), raising=False)
+
+
+def test_scores_and_eviction_are_not_for_windowed_layers(calls, monkeypatch):
+    """A key outside the window got no weight, so its score would be wrong; an eviction
+    would go by such scores."""
+    attending(monkeypatch)
+    monkeypatch.setattr(attention.kernels, "kv_evict", None, raising=False)
+    made = evicting(monkeypatch)
+    c = cache(track_scores=True)
+    q = torch.zeros(2, 5, 4, 32)
+    pos = torch.zeros(2, 5, dtype=torch.int32)
+    assert c.attend(q, pos, window=5) == ("out", "lse")     # nothing is outside it yet
+    c.commit([[0, 1], [0]], 5, q, pos)
+    assert calls == ["commit", "scores"]
+    c.attend(q, pos, window=6)
+    before = state(c)
+    with pytest.raises(ValueError, match="window"):
+        c.commit([[0], [0]], 5, q, pos)
+    with pytest.raises(ValueError, match="window"):
+        c.evict(2)
+    assert state(c) == before and calls == ["commit", "scores"] and made == []
+    c.commit([[0], [0]], 5)                                 # without scores it goes on
+    assert c.lengths == [3, 2] and calls == ["commit", "scores", "commit"]
+
+
+def test_a_window_after_an_eviction_is_refused(monkeypatch):
+    """The window is told by slots, which are no positions any more."""
+    attending(monkeypatch)
+    evicting(monkeypatch)
+    c = filled([7, 3])
+    q, pos = torch.zeros(2, 1, 4, 32), torch.zeros(2, 1, dtype=torch.int32)
+    c.evict(8)
+    assert c.attend(q, pos, window=20) == ("out", "lse")    # nothing was cut
+    c.evict(4)
+    with pytest.raises(ValueError, match="evict"):
+        c.attend(q, pos, window=20)
+    assert c.attend(q, pos) == ("out", "lse")
