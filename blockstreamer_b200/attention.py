@@ -30,7 +30,9 @@ def rotary_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = N
     "factor": f, "original_max_position_embeddings": n, "beta_fast": 32,
     "beta_slow": 1, "truncate": bool, "attention_factor": optional}`` keeps the
     pairs that turn more than beta_fast times in n positions, stretches those
-    that turn less than beta_slow times and blends linearly between."""
+    that turn less than beta_slow times and blends linearly between.  The factor
+    is ``attention_factor``, or 0.1 m ln f + 1 with m = 1, or, where both are
+    given, that of m = ``mscale`` over that of m = ``mscale_all_dim``."""
     if rot <= 0 or rot % 2:
         raise ValueError(f"rot must be even and positive, got {rot}")
     freq = base ** (-torch.arange(0, rot, 2, dtype=torch.float64) / rot)
@@ -57,7 +59,11 @@ def rotary_frequencies(rot: int, base: float = 10000.0, scaling: dict | None = N
     stretch = ((torch.arange(rot // 2, dtype=torch.float64) - low) / (high - low)).clamp(0, 1)
     factor_out = scaling.get("attention_factor")
     if factor_out is None:
-        factor_out = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+        def grown(m: float) -> float:
+            return 0.1 * m * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+        m, all_dim = scaling.get("mscale"), scaling.get("mscale_all_dim")
+        factor_out = grown(m) / grown(all_dim) if m and all_dim else grown(1.0)
     return freq * (1 - stretch) + freq / factor * stretch, float(factor_out)
 
 
