@@ -21,6 +21,7 @@
 #include <type_traits>
 
 #include "bs_paged.cuh"
+#include "bs_ring.cuh"
 
 namespace bs {
 
@@ -180,6 +181,7 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
   const int box = kTma ? min(a.box, kU) : 1, boxes = kU / box;
   lw.u = lw.start + warp;
   bool more = true;
+  Ring<Cfg::kStages> ring;
   int next_page = 0, next_row = -1;  // row < 0: no key there
   auto find = [&]() {
     while (more && lw.u >= lw.end) {
@@ -241,8 +243,10 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
   };
   find();
 #pragma unroll
-  for (int s = 0; s < Cfg::kStages - 1; ++s) load(s);
-  int stage = 0, phase = 0;
+  for (int s = 0; s < Cfg::kStages - 1; ++s) {
+    ring.place(more);
+    load(s);
+  }
 
   // ---- what an item starts with, asked for while the item before it is worked on: its Q,
   // and the positions and masks of the first row of bits of each warp
@@ -332,10 +336,14 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
       for (int d = 0; d < DP / 8; ++d) o[mt][d][0] = o[mt][d][1] = o[mt][d][2] = o[mt][d][3] = 0.f;
     }
     for (int u = cw.start + warp; u < cw.end; u += 4) {
-      const uint32_t kt = base + stage * 2 * Cfg::kTile, vt = kt + Cfg::kTile;
+      const uint32_t kt = base + ring.stage * 2 * Cfg::kTile, vt = kt + Cfg::kTile;
       const int slot0 = cw.k.lo + u * kU;
       if constexpr (kTma) {
-        ptx::mbar_wait(bar + 8 * stage, phase, &abort_flag);  // a wait that ran out is reported at the end
+        // (a wait that ran out is reported at the end)
+        more = ring.take([&](int s, int parity, bool again) {
+          volatile int gone = 0;
+          return warp_wait(bar + 8 * s, parity, again ? &gone : &abort_flag);
+        }) && more;
         if (slot0 < cw.k.low || slot0 + kU > cw.k.n) {
           // a box brings all its slots: those that hold no key become zeros in V
           if (lane < kU && !holds_key(a, cw.b, cw.k, slot0 + lane)) {
@@ -350,8 +358,8 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
         ptx::cp_async_wait<Cfg::kStages - 2>();
       }
       __syncwarp();
-      load((stage + Cfg::kStages - 1) % Cfg::kStages);
-      if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
+      load(ring.place(more));
+      ring.next();
 
       float s[MT][NT][4];
 #pragma unroll
@@ -526,12 +534,7 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
     __syncthreads();
   }
   if constexpr (kTma) {
-    if (*(volatile int*)&abort_flag) {
-      if (threadIdx.x == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
-      // copies in flight end before the CTA's memory is given back
-      volatile int gone = 0;
-      for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_wait(bar + 8 * s, phase ^ 1, &gone);
-    }
+    if (lane == 0 && *(volatile int*)&abort_flag) record_status(a.c.status, BS_ERR_TIMEOUT);
   } else {
     ptx::cp_async_wait_all();
   }
@@ -770,11 +773,9 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           }
         }
       }
-      if (!ok) {
-        // copies in flight end before the CTA's memory is given back
-        volatile int gone = 0;
-        for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
-      }
+      // copies in flight end before the CTA's memory is given back, whichever warp gave up
+      volatile int gone = 0;
+      for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
     } else if (warp >= 17 && warp < 21) {
       // ------------------------------------------------ MMA issue: S and PV of each pipeline have a
       // warp each.  One thread gets about one product or commit out per 95 cycles whatever its
@@ -850,8 +851,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
           more = walk_next<kU>(a, w);
         }
       }
-      if (!ok && elected) {
-        // products in flight end before tensor memory is given back
+      // products in flight end before tensor memory is given back, whichever warp gave up
+      if (elected) {
         volatile int gone = 0;
         ptx::tc_commit(drain(warp - 17));
         ptx::mbar_wait(drain(warp - 17), 0, &gone);
@@ -1127,6 +1128,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
         base += n;
         more = walk_next<kU>(a, w);
       }
+      if (!ok) ptx::tmem_wait_st();
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     }

@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "bs_paged.cuh"
+#include "bs_ring.cuh"
 
 namespace bs {
 namespace {
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) kv_scores_kernel(const __gri
   // ---- loading: lane g holds where the next unit's g-th box (or slot) lies
   const int box = kTma ? a.box : 1, boxes = kU / box;
   if (any) lw.u = lw.start + warp;
+  Ring<Cfg::kStages> ring;
   int next_page[kMine] = {}, next_row[kMine];  // row < 0: no key there
   auto find = [&]() {
     while (more && lw.u >= lw.end) {
@@ -219,8 +221,10 @@ __global__ void __launch_bounds__(kScoreThreads, 2) kv_scores_kernel(const __gri
   };
   find();
 #pragma unroll
-  for (int s = 0; s < Cfg::kStages - 1; ++s) load(s);
-  int stage = 0, phase = 0;
+  for (int s = 0; s < Cfg::kStages - 1; ++s) {
+    ring.place(more);
+    load(s);
+  }
   const uint32_t qaddr = ptx::smem_addr(qs);
   const int mine = lane / 4 + (lane & 3) * 8;  // the slots of a unit that this lane stores: mine, mine + 32
 
@@ -260,14 +264,18 @@ __global__ void __launch_bounds__(kScoreThreads, 2) kv_scores_kernel(const __gri
 #pragma unroll
       for (int e = 0; e < kMine; ++e) before[e] = next[e];
       ask(u + 4);
-      const uint32_t kt = base + stage * Cfg::kTile;
+      const uint32_t kt = base + ring.stage * Cfg::kTile;
       if constexpr (kTma)
-        ptx::mbar_wait(bar + 8 * stage, phase, &abort_flag);  // a wait that ran out is reported at the end
+        // (a wait that ran out is reported at the end)
+        more = ring.take([&](int s, int parity, bool again) {
+          volatile int gone = 0;
+          return warp_wait(bar + 8 * s, parity, again ? &gone : &abort_flag);
+        }) && more;
       else
         ptx::cp_async_wait<Cfg::kStages - 2>();
       __syncwarp();
-      load((stage + Cfg::kStages - 1) % Cfg::kStages);
-      if (++stage == Cfg::kStages) stage = 0, phase ^= 1;
+      load(ring.place(more));
+      ring.next();
       uint32_t kf[MT][KS][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
@@ -325,12 +333,7 @@ __global__ void __launch_bounds__(kScoreThreads, 2) kv_scores_kernel(const __gri
     sync128();
   }
   if constexpr (kTma) {
-    if (*(volatile int*)&abort_flag) {
-      if (lane == 0) record_status(a.c.status, BS_ERR_TIMEOUT);
-      // copies in flight end before the CTA's memory is given back
-      volatile int gone = 0;
-      for (int s = 0; s < Cfg::kStages; ++s) ptx::mbar_wait(bar + 8 * s, phase ^ 1, &gone);
-    }
+    if (lane == 0 && *(volatile int*)&abort_flag) record_status(a.c.status, BS_ERR_TIMEOUT);
   } else {
     ptx::cp_async_wait_all();
   }
@@ -454,11 +457,9 @@ __global__ void __launch_bounds__(kScoreTileThreads, 1) kv_scores_tiles_kernel(c
             ptx::tma_load_4d(sbase + at * Cfg::kSlot + c * 16384 + lane * a.box * 128, &maps.k, full(at), c * 64, y, z, x);
         }
       }
-      if (!ok) {
-        // copies in flight end before the CTA's memory is given back
-        volatile int gone = 0;
-        for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
-      }
+      // copies in flight end before the CTA's memory is given back, whichever warp gave up
+      volatile int gone = 0;
+      for (int k = max(0, s - Cfg::kSlots); k < s; ++k) ptx::mbar_wait(full(k % Cfg::kSlots), (k / Cfg::kSlots) & 1, &gone);
     } else if (warp == kScoreWarps + 1) {
       // ------------------------------------------------ MMA issue, by one elected thread
       const uint32_t idesc = ptx::idesc_bf16_f32(128, rows16);
@@ -488,8 +489,8 @@ __global__ void __launch_bounds__(kScoreTileThreads, 1) kv_scores_tiles_kernel(c
         tiles += n;
         more = walk_next<kU>(a, w);
       }
-      if (!ok && elected) {
-        // products in flight end before tensor memory is given back
+      // products in flight end before tensor memory is given back, whichever warp gave up
+      if (elected) {
         volatile int gone = 0;
         ptx::tc_commit(drain);
         ptx::mbar_wait(drain, 0, &gone);
