@@ -18,11 +18,10 @@ struct Ring {
 
   // Waits for the next unit's copy.  When the wait runs out, those in flight are waited
   // for once more, each with its own limit, so that none lands after its memory has gone
-  // to another use; the caller asks for no more then, and nothing is waited for again.
-  // wait(stage, parity, again) says whether the phase has ended.
+  // to another use; the caller asks for no more then.  wait(stage, parity, again) says
+  // whether the phase has ended, at once where another wait ran out before.
   template <class Wait>
   BS_HD bool take(Wait&& wait) {
-    if (flying <= 0) return false;
     if (wait(stage, phase, false)) return true;
     for (int j = 0; j < flying; ++j) wait((stage + j) % S, phase ^ (stage + j >= S), true);
     flying = 0;

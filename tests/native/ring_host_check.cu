@@ -22,6 +22,7 @@ static long run(int units, unsigned late, long* worked) {
   long bad = 0;
   bs::Ring<S> ring;
   int asked = 0;
+  bool ran_out = false;
   bool more = units > 0;
   auto load = [&](int at) {
     if (!more) return;
@@ -39,11 +40,11 @@ static long run(int units, unsigned late, long* worked) {
     more = ring.take([&](int s, int parity, bool again) {
       Stage& x = st[s];
       if (x.parity != parity) return true;   // that phase has ended
-      if (!x.armed) {                        // nothing will ever end it
-        ++bad;
+      if (!x.armed) {                        // nothing will ever end it: no wait, once one ran out
+        bad += again || !ran_out;
         return false;
       }
-      if (x.late && !again) return false;
+      if (x.late && !again) return ran_out = true, false;
       if (!again) mine = x.unit == u;
       land(s);
       return true;
