@@ -201,8 +201,12 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
     if (more) {
       const uint32_t kd = base + stage * 2 * Cfg::kTile, vd = kd + Cfg::kTile;
       if (next_row >= 0 && (unsigned)next_page >= (unsigned)a.c.pages) {
-        record_status(a.c.status, BS_ERR_CAPACITY);
-        next_page = next_page < 0 ? 0 : a.c.pages - 1;
+        if (!kTma || box_in_use(a, lw.b, lw.k.n, lw.k.lo + lw.u * kU + lane * box)) {
+          record_status(a.c.status, BS_ERR_CAPACITY);
+          next_page = next_page < 0 ? 0 : a.c.pages - 1;
+        } else {
+          next_row = -1;
+        }
       }
       if constexpr (kTma) {
         if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * stage, 2 * Cfg::kTile);
@@ -749,8 +753,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
       if (more) find();
       while (more && ok) {
         if (row >= 0 && (unsigned)page >= (unsigned)a.c.pages) {
-          record_status(a.c.status, BS_ERR_CAPACITY);
-          page = page < 0 ? 0 : a.c.pages - 1;
+          if (box_in_use(a, w.b, w.k.n, w.k.lo + i * kU + lane * a.box)) {
+            record_status(a.c.status, BS_ERR_CAPACITY);
+            page = page < 0 ? 0 : a.c.pages - 1;
+          } else {
+            row = -1;
+          }
         }
         // a box behind the last slot lies outside the descriptor's pages: zeros
         const int y = w.h, x = row >= 0 ? page : a.c.pages, z = max(row, 0);

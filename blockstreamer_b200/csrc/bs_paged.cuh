@@ -93,6 +93,15 @@ __device__ __forceinline__ Keys keys_of(const SplitArgs& a, int b) {
 __device__ __forceinline__ bool holds_key(const SplitArgs& a, int b, const Keys& k, int slot) {
   return slot >= k.low && (slot < k.n || (slot < k.hi && __ldg(a.pos + (int64_t)b * a.T + slot - k.n) >= 0));
 }
+// Whether the box from `slot` on holds a committed key or a draft in use.  Asked where its
+// page lies outside the pool: the page table may hold anything behind the last one.
+__device__ __forceinline__ bool box_in_use(const SplitArgs& a, int b, int n, int slot) {
+  bool used = slot < n;
+  const int end = min(slot - n + a.box, a.T);
+#pragma unroll 1
+  for (int u = slot - n; u < end && !used; ++u) used = __ldg(a.pos + (int64_t)b * a.T + u) >= 0;
+  return used;
+}
 
 // Where the work of CTA `cta` of `grid` lies: its range [p0, p1) of the units of
 // all items, item by item, and the sequence that holds unit p0.  An item has

@@ -97,6 +97,16 @@ struct ScoreCfg {
   static int smem(int rows) { return q + rows * (DP * 2 + 8) + 1024; }
 };
 
+// Whether a slot from `slot` on has a row that sees it.  Asked where its page lies outside
+// the pool: the page table may hold anything behind the accepted tokens.
+__device__ __forceinline__ bool seen_from(const ScoreArgs& a, int b, int n, int slot) {
+  bool any = slot < n;
+#pragma unroll 1
+  for (int i = max(slot - n, 0); i < a.T && !any; ++i)
+    any = !a.accepted || (unsigned)__ldg(a.accepted + (int64_t)b * a.T + i) < (unsigned)a.tokens;
+  return any;
+}
+
 // Behind an item's last unit scores are only copied: an equal share of the whole array
 // for the one warp of each CTA that does it.
 template <int kU>
@@ -188,8 +198,12 @@ __global__ void __launch_bounds__(kScoreThreads, 2) kv_scores_kernel(const __gri
 #pragma unroll
       for (int e = 0; e < kMine; ++e)
         if (next_row[e] >= 0 && (unsigned)next_page[e] >= (unsigned)a.c.pages) {
-          record_status(a.c.status, BS_ERR_CAPACITY);
-          next_page[e] = next_page[e] < 0 ? 0 : a.c.pages - 1;
+          if (seen_from(a, lw.b, lw.k.n, lw.u * kU + (lane + 32 * e) * box)) {
+            record_status(a.c.status, BS_ERR_CAPACITY);
+            next_page[e] = next_page[e] < 0 ? 0 : a.c.pages - 1;
+          } else {
+            next_row[e] = -1;
+          }
         }
       if constexpr (kTma) {  // at most kU / 8 <= 32 boxes: the first of a lane's places
         if (lane == 0) ptx::mbar_arrive_expect_tx(bar + 8 * stage, Cfg::kTile);
@@ -437,8 +451,12 @@ __global__ void __launch_bounds__(kScoreTileThreads, 1) kv_scores_tiles_kernel(c
       if (more) find();
       for (; more; ++s) {
         if (row >= 0 && (unsigned)page >= (unsigned)a.c.pages) {
-          record_status(a.c.status, BS_ERR_CAPACITY);
-          page = page < 0 ? 0 : a.c.pages - 1;
+          if (seen_from(a, w.b, w.k.n, i * kU + lane * a.box)) {
+            record_status(a.c.status, BS_ERR_CAPACITY);
+            page = page < 0 ? 0 : a.c.pages - 1;
+          } else {
+            row = -1;
+          }
         }
         // a box behind the last slot lies outside the descriptor's pages: zeros
         const int y = w.h, x = row >= 0 ? page : a.c.pages, z = max(row, 0), at = s % Cfg::kSlots;

@@ -175,3 +175,41 @@ def test_evict_to_fewer_pages_than_the_budget_is_reported():
         full[6:8] = c[src // page, src % page].view(2, page, 1, 8)
         assert torch.equal(d.cpu(), full)
     assert new.shape == (1, 1, 16) and new[0, 0].cpu().tolist() == [float(scores[0, 0, j]) if j < 16 else 0.0 for j in want]
+
+
+@pytest.mark.parametrize("behind", [-1, -2 ** 31, 10 ** 6])
+@pytest.mark.parametrize("T,Hq,D,page,slots", [
+    (8, 1, 64, 8, 0), (8, 2, 32, 5, 0), (8, 2, 128, 8, 0), (8, 2, 128, 8, 1000),    # few rows: boxes, copies, cut
+    (8, 4, 64, 16, 2000), (20, 4, 128, 8, 0), (20, 8, 64, 8, 0), (20, 8, 64, 6, 0),  # tiles
+])
+def test_pages_behind_the_last_used_draft_are_not_looked_at(T, Hq, D, page, slots, behind):
+    """A page table may hold anything where a sequence has no slot in use: its drafts not in
+    use have no pages, nor have the entries behind the accepted ones."""
+    heads, B, n, used = 2, 2, 13, [3, 2]
+    g = torch.Generator().manual_seed(T)
+    P = pages_for(n + T, page) + slots // page
+    kc, vc = (torch.randn(B * P, page, heads, D, generator=g).bfloat16().to(DEV) for _ in range(2))
+    table = torch.randperm(B * P, generator=g).to(torch.int32).view(B, P)
+    L = torch.tensor([n, n + 1], dtype=torch.int32)
+    pos = (L[:, None] + torch.arange(T)).to(torch.int32)
+    bad = table.clone()
+    for b in range(B):
+        pos[b, used[b]:] = -1
+        bad[b, pages_for(int(L[b]) + used[b], page):] = behind
+    q = torch.randn(B, T, Hq * heads, D, generator=g).bfloat16()
+    q, table, bad, L, pos = to(q, table, bad, L, pos)
+    want, lse = kernels.tree_attention(q, kc, vc, table, L, pos)
+    got, lse1 = kernels.tree_attention(q, kc, vc, bad, L, pos)
+    assert torch.equal(got, want) and torch.equal(lse, lse1)
+    acc = torch.full((B, T - 1), -1, dtype=torch.int32)
+    acc[0, :2], acc[1, :1] = torch.tensor([0, 2]), torch.tensor([1])
+    scores = torch.rand(B, heads, P * page, generator=g).to(DEV)
+    a, b = (kernels.kv_scores_add(scores, q, lse, kc, t, L, accepted=acc.to(DEV)) for t in (table, bad))
+    assert torch.equal(a, b)
+    assert kernels.device_status(clear=False) == 0
+    # where a used draft has no page it is reported still
+    bad[0, int(L[0]) // page] = behind
+    kernels.tree_attention(q, kc, vc, bad, L, pos)
+    assert kernels.device_status(clear=True) != 0
+    kernels.kv_scores_add(scores, q, lse, kc, bad, L, accepted=acc.to(DEV))
+    assert kernels.device_status(clear=True) != 0
