@@ -84,7 +84,8 @@ def main():
             tokens = [n + len(p) for n, p in zip(tokens, accepted)]
             cut = max(cache.lengths) > a.budget
             if cut:
-                cache.evict(a.budget, keep_first=2, keep_last=4)
+                first = min(2, a.budget)
+                cache.evict(a.budget, keep_first=first, keep_last=min(4, a.budget - first))
             print(f"step {step}: accepted {[len(p) for p in accepted]}, positions {tokens}, "
                   f"cached {cache.lengths}{' (cut)' if cut else ''}, output rms {y.float().pow(2).mean().sqrt():.3f}")
     status = kernels.device_status()
