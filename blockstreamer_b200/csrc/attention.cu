@@ -12,6 +12,14 @@
 // passes over NaN, a sum does not: a part has nothing to add where z is 0, not where m
 // is -inf, which a part whose every score is NaN has too.
 //
+// Statistics, sums and O are 32 bits.  The weights are rounded to bf16 for the product
+// with V, whose values are bf16 (both operands of it have one type): off by 2^-8 of each
+// weight at most, which adds to the output's own rounding.  Against 64 bits, relative
+// to the whole output: 16-token trees over 131072 keys 2.3e-3, one token over 500 keys
+// 1.9e-3, where weights of 32 bits and the same last rounding give 1.7e-3.
+// It is a product of matrices: a value of infinity or NaN in a slot that some row of
+// the kv head may attend reaches the other rows as 0 times itself.
+//
 // Work split: the keys of every (sequence, kv head, row tile) are cut into
 // units; the units of all items, in item order, are cut into equal contiguous
 // ranges, one per CTA, from the lengths on the device (no host read, no idle
@@ -80,10 +88,13 @@ int cache_maps(const bs_kv_cache* c, int rows, bool need_v, CacheMaps* o) {
 namespace {
 
 constexpr int kMaxDrafts = 256;
-// Up to so many keys an item is not cut.  At one sequence, one token and 8 kv heads:
-// 250 keys 9.5 us on the device in one launch, 10.2 cut and joined; 450 keys 12.0
-// and 10.8, but 19.7 and 21.5 where the host launches; 900 keys 16.7 and 10.5.
-// 64 sequences: 450 keys 22.4 and 24.9; with a window of 128 18.1 and 21.5.
+// Where no more than so many keys are in reach an item is not cut, and there is one
+// launch.  The reach is known on the host: the window, or the width of the page table
+// (lengths are on the device), so a table for longer sequences has its items cut however
+// short they are.  Uncut / cut, us, tables of the very length and for 131072 slots, 8 kv
+// heads, one token: 256 x 300 keys 49 / 54, 64 x 450 24 / 22, 8 x 450 12.2 / 12.5,
+// 1 x 450 12.1 / 11.3 on the device, where the second launch costs the host 1.8 more
+// (19.7 / 21.5 a call); 900 keys 16.7 / 10.5; 64 x 450 with a window of 128 18.1 / 21.5.
 constexpr int kWholeKeys = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -105,9 +116,11 @@ struct TreeArgs : SplitArgs {
 // ---------------------------------------------------------------- few rows
 // Row tiles of MT * 16 rows on mma.sync, four warps per CTA, each streaming its
 // own units of kU keys into its own ring (no barrier between warps) and holding
-// its own (m, z, O); they meet at the end of an item.  HBM-bound for long items: two or
-// three CTAs per SM keep ~190 KB per SM in flight.  64 sequences of up to 8192 keys, 64 / 8
-// heads of 64: 91 us, 5.9 TB/s (90% of the measured copy rate); 2 x 131072 keys: 90 us
+// its own (m, z, O); they meet at the end of an item.  HBM-bound for long items: of each
+// warp's ring all stages but the one that is worked on are in flight, 96 KB per SM in
+// three CTAs of two stages, 128 KB in two of three.  64 sequences of up to 8192 keys, 64 / 8
+// heads of 64: 92 us, 5.9 TB/s (90% of the measured copy rate); heads of 128: 176 to 180 us,
+// 6.0 TB/s; heads of 80 and 96, which are worked on as 128: 162 us.  2 x 131072 keys: 90 us
 // where a head's slots lie together in a page, 113 us where heads are interleaved
 // (128 bytes in every KB).  Short items are bound by the chain of an item's start, units
 // and end, some 8000 cycles, which a third CTA hides better than a third stage of the
@@ -115,7 +128,8 @@ struct TreeArgs : SplitArgs {
 // would spill with three (133 us, 126 with two).
 // kTma: a unit is fetched by a few TMA boxes (pages of a multiple of 8 slots); else
 // by 16-byte asynchronous copies, whose address arithmetic and issue are most of
-// the kernel's instructions then (187 us for the 64 sequences).
+// the kernel's instructions then (pages of 12 slots: 119 us for the 64 sequences, 250 with
+// heads of 128).
 template <int DP>
 struct RowsCfg {
   static constexpr int kU = DP == 64 ? 32 : 16;
@@ -414,7 +428,7 @@ __global__ void __launch_bounds__(128, rows_ctas(16 * MT, DP)) tree_rows_kernel(
             const float y0 = mma::exp2_fast(s[mt][nt][2 * e] - ref);
             const float y1 = mma::exp2_fast(s[mt][nt][2 * e + 1] - ref);
             sum += y0 + y1;
-            p[nt][e] = pack_bf16x2(y0, y1);
+            p[nt][e] = pack_bf16x2(y0, y1);  // (the choice of bf16: at the top)
           }
           z[mt][e] = z[mt][e] * f + sum;
           if (__any_sync(0xffffffffu, f != 1.f)) {
@@ -997,7 +1011,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) tree_tiles_kernel(const __gri
                     x.y = mma::exp2_fast(x.y);
                   }
                   sum[e & 1] = mma::add2(sum[e & 1], x);
-                  pk[e] = pack_bf16x2(x.x, x.y);
+                  pk[e] = pack_bf16x2(x.x, x.y);  // (the choice of bf16: at the top)
                 }
                 ptx::tmem_st_32x32b_x16(s_col + c * 16, pk);
               }
@@ -1259,8 +1273,11 @@ __global__ void __launch_bounds__(JoinCfg<kSplit>::kThreads) tree_join_kernel(co
 // 2 x 131072 keys 136 / 99, 8 x 8192 47 / 38, 64 ragged to 8192 162 / 131.  Where no more
 // than kShortKeys are in reach, two tiles of 16 that read the keys twice end sooner: of
 // 16 and of 128, 256 x 300 keys 91 / 125, 256 ragged to 1000 135 / 165, 64 x 600 38 / 47,
-// 1 x 1000 11.5 / 13.1, 64 x 1000 55 / 56, but 64 x 2000 91 / 80.  The workspace is sized
-// without the page size and the reach, for the largest.
+// 1 x 1000 11.5 / 13.1, 64 x 1000 55 / 56, but 64 x 2000 91 / 80.  (The reach is the page
+// table's: behind one of 131072 slots 256 x 300 keys take 139, 64 x 900 60 instead of 53.)
+// Without boxes and over heads of 64 the tiles stay at 16 rows (of 255 registers they take
+// 241) and read the keys once for each: 64 rows of 128 over 4 x 8192 keys 130 us, 41 with boxes.
+// The workspace is sized without the page size and the reach, for the largest.
 constexpr int64_t kShortKeys = 1024;
 int tile_rows(int64_t R, int64_t D, bool tma, int64_t reach) {
   if (R <= 16 || (!tma && D > 64) || (R <= 32 && D <= 64 && reach <= kShortKeys)) return 16;

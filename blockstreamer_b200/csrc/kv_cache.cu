@@ -1109,7 +1109,9 @@ extern "C" int bs_kv_scores_add(const bs_heads* q, const bs_kv_cache* cache, int
   // 64 keys share ragged lengths better.  In us, those and tiles of 128 keys: dim 64, 32
   // sequences of 5000 keys, 8 heads: 8 rows 34.0 / 37.2, 24 rows 38.5 / 38.9, 32 rows 42.8 /
   // 38.1, 128 rows 149 / 61; ragged to 8192 keys, 8 rows 32 / 42.  Dim 128, 2 sequences of
-  // 131072 keys: 8 rows 89.7 / 89.2, 16 rows 91.1 / 88.6, 32 rows 102 / 88.8, 128 rows 368 / 102.
+  // 131072 keys: 8 rows 89.7 / 89.2, 16 rows 91.1 / 88.6, 32 rows 102 / 88.8, 128 rows 368 / 99.
+  // Pages without boxes stay on the former, with 16-byte copies: 514 us for those 128 rows, and
+  // 132 for 64 rows of 64 over 2 x 131072 keys where boxes take 57.
   const int few = D <= 64 ? 24 : 16;
   a.box = cache_box_rows(cache, 128);
   if (a.box >= 8 && A * a.G > few) {

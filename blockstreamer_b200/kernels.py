@@ -3,8 +3,9 @@
 Every function launches on ``torch.cuda.current_stream()`` of its inputs'
 device, allocates outputs and workspaces through the torch caching allocator
 (so ``record_stream`` semantics hold for callers such as StreamedModel's pool),
-reads ``data_ptr()`` on every call (no cached pointers), and never mutates its
-inputs.  All tensors must be CUDA tensors: there is no CPU path.
+reads ``data_ptr()`` on every call (no cached pointers), and mutates no input but
+the caches that ``rope_append``, ``tree_commit`` and ``kv_evict`` write and an
+``out`` that is given.  All tensors must be CUDA tensors: there is no CPU path.
 """
 
 from __future__ import annotations

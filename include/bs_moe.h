@@ -417,7 +417,10 @@ int bs_rope_append(const bs_heads* q, const bs_heads* k, const bs_heads* v, cons
  * x_j = scale q . k_j;  z = sum exp(x_j) + exp(sinks[h]) (sinks may be NULL);
  * out = sum exp(x_j) v_j / z;  lse = log z.  A row that attends nothing gives
  * out 0 and lse sinks[h] (-inf without sinks); a row of negative position gives
- * out 0 and lse -inf.  Slots that no row may attend are not read.
+ * out 0 and lse -inf.  What slots that no row may attend hold is not used, nor are
+ * page table entries behind the last draft in use.  A score of NaN makes the rows
+ * that attend it NaN.  The sum over v_j is a matrix product: where a slot that some
+ * row of a kv head may attend holds an infinity or NaN in v, the others may get NaN.
  * q, out bf16 [B, T, Hq, dim] (out contiguous), Hq a multiple of cache->heads;
  * mask uint8 [T, T] per sequence with mask_stride_b between sequences (0: one
  * tree for all), NULL for a chain (u <= t); sinks [Hq] f32; positions [B, T]
