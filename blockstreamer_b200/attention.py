@@ -176,11 +176,14 @@ class PagedKVCache:
             raise ValueError("commit: keys outside a window got no weight that could be added to their scores")
         if len(accepted) != len(self.lengths):
             raise ValueError(f"commit takes {len(self.lengths)} lists of accepted drafts, got {len(accepted)}")
+        page = self.page_size
         for x, n, held in zip(accepted, self.lengths, self._held):
             # the device would leave such a sequence as it is, but not know its new length
-            if any(v <= u for u, v in zip([-1] + x, x + [drafted])):
+            if not x:
+                continue
+            if x[0] < 0 or x[-1] >= drafted or (len(x) > 1 and sorted(set(x)) != x):
                 raise ValueError(f"accepted drafts must ascend from 0 to below {drafted}, got {x}")
-            if x and n + x[-1] >= len(held) * self.page_size:
+            if n + x[-1] >= len(held) * page:
                 raise ValueError(f"draft {x[-1]} behind {n} keys lies outside the {len(held)} reserved pages")
         most = max((len(x) for x in accepted), default=0)
         if most:
